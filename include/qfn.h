@@ -246,6 +246,79 @@ int qfn_deltanet_step(const uint16_t* q, const uint16_t* k, const uint16_t* v, c
                       int dk, int dv, qfn_stream_t stream);
 
 /*
+ * qfn_deltanet_step_batch -- the gated delta rule (formula of
+ * qfn_deltanet_step) for one token of each of `rows` requests, their states
+ * in slots of a pool.
+ *   q, k: bf16 rows of n_key_heads x dk; v: bf16 rows of n_heads x dv; g: f32
+ *   and beta: bf16 rows of n_heads.  strides: host array of 10, in elements:
+ *   {q row, q head, k row, k head, v row, v head, g row, g head, beta row,
+ *   beta head}; the last dimension of q, k and v is dense.
+ *   state_index: int32[rows] device, row r's slot, or NULL (slot r).  A
+ *   negative one marks a padding row (out = 0, no state touched); one that is
+ *   not below n_slots, or that an earlier row names, gives NaN in the row's
+ *   out and touches no state.
+ *   state_in, state_out: f32[n_slots][n_heads][dk][dv], 16-byte aligned, the
+ *   same array or two that do not overlap; slots no row names are not written.
+ *   out: bf16[rows][n_heads][dv].  dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.
+ */
+int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* g,
+                            const uint16_t* beta, const int64_t* strides, const int32_t* state_index,
+                            int64_t n_slots, const float* state_in, float* state_out, uint16_t* out, int64_t rows,
+                            int n_heads, int n_key_heads, int dk, int dv, qfn_stream_t stream);
+
+/*
+ * qfn_deltanet_chunk -- the gated delta rule (formula of qfn_deltanet_step)
+ * over n_seqs sequences of a prompt batch.
+ *   Rows of q, k, v, g, beta and out are the `tokens` tokens of all sequences
+ *   (layouts and strides as qfn_deltanet_step_batch).  cu_seqlens:
+ *   int32[n_seqs + 1] device, sequence n = rows cu_seqlens[n] up to
+ *   cu_seqlens[n + 1], rising within [0, tokens]; NULL: sequences of
+ *   tokens / n_seqs rows each.  Rows outside every sequence are not written.
+ *   Bounds that do not rise: no row is written and every final state is NaN.
+ *   state_in: f32[n_seqs][n_heads][dk][dv] or NULL (zeros); state_out: the
+ *   same shape, state_in itself or an array that does not overlap it; both
+ *   16-byte aligned.  dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.
+ *   workspace: device scratch of qfn_deltanet_chunk_workspace(...) bytes,
+ *   256-byte aligned (may be NULL where that is 0).  Calls that can overlap
+ *   on the device need workspaces of their own.
+ */
+size_t qfn_deltanet_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk, int dv);
+int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* g,
+                       const uint16_t* beta, const int64_t* strides, const int32_t* cu_seqlens, int64_t n_seqs,
+                       int64_t tokens, const float* state_in, float* state_out, uint16_t* out, int n_heads,
+                       int n_key_heads, int dk, int dv, void* workspace, size_t workspace_bytes,
+                       qfn_stream_t stream);
+
+/*
+ * qfn_gated_norm -- the norm of the linear attention's heads with the output
+ * gate: y = x * rsqrt(mean x^2 + eps) * w * silu(z) over `dim`, fp32 inside.
+ *   x, z: bf16, row and head strides in elements; w: [dim] of w_dtype;
+ *   y: bf16[rows][heads][dim].  Any dim >= 1 and any alignment; rows whose
+ *   bases and strides are multiples of 16 bytes, with dim % 8 == 0 and dim <=
+ *   256, run the wide path.
+ */
+int qfn_gated_norm(const uint16_t* x, int64_t x_row, int64_t x_head, const uint16_t* z, int64_t z_row,
+                   int64_t z_head, const void* w, int w_dtype, uint16_t* y, int64_t rows, int heads, int dim,
+                   float eps, qfn_stream_t stream);
+
+/*
+ * qfn_norm_residual -- between two blocks, in one pass over `rows` rows:
+ *   p  = block * rsqrt(mean block^2 + eps) * w_post     (block itself if w_post is NULL)
+ *   r  = residual + scale * a(gate) * p                 (a: sigmoid if gate_sigmoid, else identity)
+ *   n  = r * rsqrt(mean r^2 + eps) * w_next             (not formed if w_next is NULL)
+ *   gate_kind: 0 none, 1 one value per row (gate[row * gate_row]), 2 one per element.
+ *   block, residual, gate, w_post, w_next: f32 or bf16 by their dtype codes,
+ *   row strides in elements.  residual_out: [rows][dim] of residual's type
+ *   (the residual's own array if that is dense); normed: bf16[rows][dim].
+ *   n is formed from r before its rounding.  1 <= dim <= 32768.
+ */
+int qfn_norm_residual(const void* block, int block_dtype, int64_t block_row, const void* residual,
+                      int residual_dtype, int64_t residual_row, const void* w_post, int post_dtype, const void* gate,
+                      int gate_kind, int gate_dtype, int64_t gate_row, int gate_sigmoid, float scale,
+                      const void* w_next, int next_dtype, void* residual_out, uint16_t* normed, int64_t rows, int dim,
+                      float eps, qfn_stream_t stream);
+
+/*
  * qfn_gemv_e4m3 -- replaces fp8gemv.gemv (fp8gemv.py:20-26).
  *   y[n] = s[n] * sum_k e4m3(q[n][k]) * x[k], fp32 accumulation.
  *   q: u8[N][K] (float8_e4m3fn bytes) device, 16-byte aligned, K % 16 == 0.

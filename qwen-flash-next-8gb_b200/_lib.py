@@ -1,7 +1,7 @@
 """Bindings of libqfn.so, the C ABI declared in include/qfn.h: ctypes for every
 entry point (lib()), and the thin torch extension over the same ABI for the
 hot-path operators (ops(): torch.ops.qfn.moe_decode / moe_prefill / gemv /
-linear).
+linear / deltanet_chunk / deltanet_step / gated_norm / norm_residual).
 
 Both libraries are loaded from this directory (built in-tree by build.py).
 There is no fallback: if a library is missing or the device is not an sm_100
@@ -48,9 +48,16 @@ SIGNATURES = {
     "qfn_shared_expert_gate_up": [_P, _I64, _P, _P, _P, _I, _P, _P, _P],
     "qfn_shared_expert_down": [_P, _I, _I64, _P, _P, _P, _P, _P],
     "qfn_deltanet_step": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "qfn_deltanet_step_batch": [_P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _I, _I, _I, _I, _P],
+    "qfn_deltanet_chunk_workspace": [_I64, _I64, _I, _I, _I, _I],
+    "qfn_deltanet_chunk": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _I, _I, _I, _I, _P, ctypes.c_size_t, _P],
+    "qfn_gated_norm": [_P, _I64, _I64, _P, _I64, _I64, _P, _I, _P, _I64, _I, _I, ctypes.c_float, _P],
+    "qfn_norm_residual": [_P, _I, _I64, _P, _I, _I64, _P, _I, _P, _I, _I, _I64, _I, ctypes.c_float, _P, _I, _P, _P,
+                          _I64, _I, ctypes.c_float, _P],
 }
 # entry points whose return value is not an int status
-RESTYPES = {"qfn_moe_prefill_workspace": ctypes.c_size_t, "qfn_moe_prefill_ep_workspace": ctypes.c_size_t}
+RESTYPES = {"qfn_moe_prefill_workspace": ctypes.c_size_t, "qfn_moe_prefill_ep_workspace": ctypes.c_size_t,
+            "qfn_deltanet_chunk_workspace": ctypes.c_size_t}
 
 
 class QfnError(RuntimeError):
@@ -86,7 +93,8 @@ TORCH_EXT_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqf
 
 def ops():
     """torch.ops.qfn: the thin torch extension over the C ABI (moe_decode,
-    moe_prefill, gemv, linear).  Loads libqfn_torch.so (built next to libqfn.so by
+    moe_prefill, gemv, linear, deltanet_chunk, deltanet_step, gated_norm,
+    norm_residual).  Loads libqfn_torch.so (built next to libqfn.so by
     build.py); there is no fallback when it is missing."""
     global _ops
     if _ops is None:

@@ -1,0 +1,310 @@
+// The norms of a layer around its blocks (RMSNorm in fp32, one rounding per
+// output):
+//
+//   qfn_gated_norm     y = x * rsqrt(mean x^2 + eps) * w * silu(z), per head
+//   qfn_norm_residual  p  = block * rsqrt(mean block^2 + eps) * w_post
+//                      r' = residual + scale * gate * p
+//                      n  = r' * rsqrt(mean r'^2 + eps) * w_next
+//
+// Both are bound by memory: a row is read once, held in registers as fp32
+// through its sums, and written once.  n is formed from r' before its
+// rounding, so each output carries one rounding.  Rows whose bases, strides and length allow it move
+// in 16-byte pieces of 8 elements (two for fp32); the others go element by element.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "host.cuh"
+
+namespace qfn {
+
+// Element types of one operand.
+__device__ __forceinline__ float load1(const void* p, int dtype, int64_t i) {
+  return dtype == QFN_DTYPE_F32 ? static_cast<const float*>(p)[i]
+                                : bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+__device__ __forceinline__ void store1(void* p, int dtype, int64_t i, float v) {
+  if (dtype == QFN_DTYPE_F32) {
+    static_cast<float*>(p)[i] = v;
+  } else {
+    const __nv_bfloat16 b = __float2bfloat16_rn(v);
+    static_cast<uint16_t*>(p)[i] = *reinterpret_cast<const uint16_t*>(&b);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Eight neighbouring elements, 16-byte aligned (32 bytes for fp32).
+__device__ __forceinline__ void unpack8(uint4 u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8(const void* p, int dtype, int64_t i, float (&v)[8]) {
+  if (dtype == QFN_DTYPE_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i), v);
+  }
+}
+__device__ __forceinline__ void store8(void* p, int dtype, int64_t i, const float (&v)[8]) {
+  if (dtype == QFN_DTYPE_F32) {
+    float* f = static_cast<float*>(p) + i;
+    *reinterpret_cast<float4*>(f) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(f + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+        make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+  }
+}
+
+__device__ __forceinline__ float sigmoidf(float x) { return 1.f / (1.f + expf(-x)); }
+
+// ------------------------------------------------------------------ gated norm
+struct GatedNorm {
+  const uint16_t *x, *z;
+  const void* w;
+  uint16_t* y;   // [rows][heads][dim], contiguous
+  int64_t x_row, x_head, z_row, z_head, n;   // n = rows * heads
+  int w_dtype, heads, dim;
+  float eps;
+};
+
+// LANES lanes of a warp share one row of dim <= 8 LANES; a warp carries
+// 32 / LANES rows.
+template <int LANES>
+__global__ void __launch_bounds__(256) gated_norm_kernel(const GatedNorm a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
+  const int c = static_cast<int>(threadIdx.x % LANES) * 8;
+  const bool in = i < a.n && c < a.dim;
+  const int64_t row = i / a.heads;
+  const int h = static_cast<int>(i % a.heads);
+  float x[8] = {}, z[8], w[8], ss = 0.f;
+  if (in) {
+    load8(a.x, QFN_DTYPE_BF16, row * a.x_row + h * a.x_head + c, x);
+    load8(a.z, QFN_DTYPE_BF16, row * a.z_row + h * a.z_head + c, z);
+    load8(a.w, a.w_dtype, c, w);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (!in) return;
+  const float r = rsqrtf(ss / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j] * (z[j] * sigmoidf(z[j]));
+  store8(a.y, QFN_DTYPE_BF16, i * a.dim + c, x);
+}
+
+// Any dim and alignment: a warp per row, read twice (the second time from L1).
+__global__ void __launch_bounds__(256) gated_norm_any_kernel(const GatedNorm a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
+  if (i >= a.n) return;
+  const int lane = threadIdx.x & 31;
+  const uint16_t* x = a.x + i / a.heads * a.x_row + i % a.heads * a.x_head;
+  const uint16_t* z = a.z + i / a.heads * a.z_row + i % a.heads * a.z_head;
+  float ss = 0.f;
+  for (int c = lane; c < a.dim; c += 32) {
+    const float v = bf16_bits_to_f32(x[c]);
+    ss = fmaf(v, v, ss);
+  }
+  const float r = rsqrtf(warp_sum(ss) / static_cast<float>(a.dim) + a.eps);
+  for (int c = lane; c < a.dim; c += 32) {
+    const float g = bf16_bits_to_f32(z[c]);
+    store1(a.y, QFN_DTYPE_BF16, i * a.dim + c, bf16_bits_to_f32(x[c]) * r * load1(a.w, a.w_dtype, c) * (g * sigmoidf(g)));
+  }
+}
+
+// ------------------------------------------------------------------ norm, gate, residual, norm
+struct NormResidual {
+  const void *block, *residual, *w_post, *gate, *w_next;
+  void* r_out;
+  uint16_t* n_out;
+  int64_t block_row, residual_row, gate_row;
+  int block_dtype, residual_dtype, post_dtype, gate_dtype, next_dtype;
+  int gate_kind;   // 0 none, 1 a value per row, 2 a value per element
+  int sigmoid, dim;
+  float scale, eps;
+};
+
+// Sum over the block of up to 32 warps; every thread gets it.  red: 33 floats.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  v = warp_sum(v);
+  if (lane == 0) red[w] = v;
+  __syncthreads();
+  float t = lane < nw ? red[lane] : 0.f;
+  return warp_sum(t);
+}
+
+// CTA = one row; a thread holds PARTS pieces of WIDTH neighbouring elements
+// (8, or 1 where alignment or dim rule 16-byte pieces out), blockDim.x pieces apart.
+template <int WIDTH, int PARTS>
+__global__ void __launch_bounds__(1024) norm_residual_kernel(const NormResidual a) {
+  __shared__ float red[2][32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  float b[PARTS][WIDTH], ss = 0.f;
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const int c = (p * blockDim.x + threadIdx.x) * WIDTH;
+    if (c < a.dim) {
+      if constexpr (WIDTH == 8) load8(a.block, a.block_dtype, row * a.block_row + c, b[p]);
+      else b[p][0] = load1(a.block, a.block_dtype, row * a.block_row + c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < WIDTH; ++j) b[p][j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) ss = fmaf(b[p][j], b[p][j], ss);
+  }
+  float m = a.scale;
+  if (a.gate_kind == 1) {
+    const float g = load1(a.gate, a.gate_dtype, row * a.gate_row);
+    m *= a.sigmoid ? sigmoidf(g) : g;
+  }
+  if (a.w_post) m *= rsqrtf(block_sum(ss, red[0]) / static_cast<float>(a.dim) + a.eps);
+  float s2 = 0.f;
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const int c = (p * blockDim.x + threadIdx.x) * WIDTH;
+    if (c >= a.dim) continue;
+    float r[WIDTH], w[WIDTH], g[WIDTH];
+    if constexpr (WIDTH == 8) {
+      load8(a.residual, a.residual_dtype, row * a.residual_row + c, r);
+      if (a.w_post) load8(a.w_post, a.post_dtype, c, w);
+      if (a.gate_kind == 2) load8(a.gate, a.gate_dtype, row * a.gate_row + c, g);
+    } else {
+      r[0] = load1(a.residual, a.residual_dtype, row * a.residual_row + c);
+      if (a.w_post) w[0] = load1(a.w_post, a.post_dtype, c);
+      if (a.gate_kind == 2) g[0] = load1(a.gate, a.gate_dtype, row * a.gate_row + c);
+    }
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) {
+      float v = b[p][j] * m;
+      if (a.w_post) v *= w[j];
+      if (a.gate_kind == 2) v *= a.sigmoid ? sigmoidf(g[j]) : g[j];
+      b[p][j] = r[j] + v;
+      s2 = fmaf(b[p][j], b[p][j], s2);
+    }
+    if constexpr (WIDTH == 8) store8(a.r_out, a.residual_dtype, row * a.dim + c, b[p]);
+    else store1(a.r_out, a.residual_dtype, row * a.dim + c, b[p][0]);
+  }
+  if (!a.w_next) return;
+  const float rn = rsqrtf(block_sum(s2, red[1]) / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const int c = (p * blockDim.x + threadIdx.x) * WIDTH;
+    if (c >= a.dim) continue;
+    float w[WIDTH];
+    if constexpr (WIDTH == 8) load8(a.w_next, a.next_dtype, c, w);
+    else w[0] = load1(a.w_next, a.next_dtype, c);
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) w[j] *= b[p][j] * rn;
+    if constexpr (WIDTH == 8) store8(a.n_out, QFN_DTYPE_BF16, row * a.dim + c, w);
+    else store1(a.n_out, QFN_DTYPE_BF16, row * a.dim + c, w[0]);
+  }
+}
+
+namespace {
+
+template <typename Kernel, typename Args>
+int launch(const char* what, Kernel kernel, int64_t blocks, int threads, qfn_stream_t stream, const Args& args) {
+  QFN_REQUIRE(blocks <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many rows", what);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = as_stream(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+bool dtype_ok(int d) { return d == QFN_DTYPE_F32 || d == QFN_DTYPE_BF16; }
+
+// Whether rows of `dim` elements at p, row_a and row_b elements apart, can be moved 8 elements at a time.
+bool wide(const void* p, int dtype, int64_t row_a, int64_t row_b) {
+  return !p || (aligned(p, 16) && (row_a * (dtype == QFN_DTYPE_F32 ? 4 : 2)) % 16 == 0 &&
+                (row_b * (dtype == QFN_DTYPE_F32 ? 4 : 2)) % 16 == 0);
+}
+
+}  // namespace
+
+}  // namespace qfn
+
+using namespace qfn;
+
+extern "C" int qfn_gated_norm(const uint16_t* x, int64_t x_row, int64_t x_head, const uint16_t* z, int64_t z_row,
+                              int64_t z_head, const void* w, int w_dtype, uint16_t* y, int64_t rows, int heads,
+                              int dim, float eps, qfn_stream_t stream) {
+  constexpr const char* what = "qfn_gated_norm";
+  QFN_REQUIRE(rows >= 0 && heads >= 1 && dim >= 1, QFN_ERR_INVALID_ARG, "%s: rows=%lld, heads=%d, dim=%d", what,
+              static_cast<long long>(rows), heads, dim);
+  QFN_REQUIRE(dtype_ok(w_dtype), QFN_ERR_INVALID_ARG, "%s: w_dtype=%d", what, w_dtype);
+  if (rows == 0) return QFN_OK;
+  QFN_REQUIRE(x && z && w && y, QFN_ERR_INVALID_ARG, "%s: null pointer", what);
+  DeviceInfo* dev;
+  const int rc = current_device(&dev);
+  if (rc) return rc;
+  const GatedNorm a{x, z, w, y, x_row, x_head, z_row, z_head, rows * heads, w_dtype, heads, dim, eps};
+  const bool v = dim % 8 == 0 && dim <= 256 && wide(x, QFN_DTYPE_BF16, x_row, x_head) &&
+                 wide(z, QFN_DTYPE_BF16, z_row, z_head) && wide(w, w_dtype, 0, 0) && aligned(y, 16);
+  if (!v) return launch(what, gated_norm_any_kernel, (a.n + 7) / 8, 256, stream, a);
+  if (dim <= 64) return launch(what, gated_norm_kernel<8>, (a.n + 31) / 32, 256, stream, a);
+  if (dim <= 128) return launch(what, gated_norm_kernel<16>, (a.n + 15) / 16, 256, stream, a);
+  return launch(what, gated_norm_kernel<32>, (a.n + 7) / 8, 256, stream, a);
+}
+
+extern "C" int qfn_norm_residual(const void* block, int block_dtype, int64_t block_row, const void* residual,
+                                 int residual_dtype, int64_t residual_row, const void* w_post, int post_dtype,
+                                 const void* gate, int gate_kind, int gate_dtype, int64_t gate_row, int gate_sigmoid,
+                                 float scale, const void* w_next, int next_dtype, void* residual_out,
+                                 uint16_t* normed, int64_t rows, int dim, float eps, qfn_stream_t stream) {
+  constexpr const char* what = "qfn_norm_residual";
+  QFN_REQUIRE(rows >= 0 && dim >= 1, QFN_ERR_INVALID_ARG, "%s: rows=%lld, dim=%d", what, static_cast<long long>(rows),
+              dim);
+  QFN_REQUIRE(dim <= 32768, QFN_ERR_UNSUPPORTED, "%s: dim=%d (at most 32768)", what, dim);
+  QFN_REQUIRE(dtype_ok(block_dtype) && dtype_ok(residual_dtype) && dtype_ok(post_dtype) && dtype_ok(gate_dtype) &&
+                  dtype_ok(next_dtype) && gate_kind >= 0 && gate_kind <= 2,
+              QFN_ERR_INVALID_ARG, "%s: unknown dtype or gate kind", what);
+  if (rows == 0) return QFN_OK;
+  QFN_REQUIRE(block && residual && residual_out && (gate || !gate_kind) && (normed || !w_next), QFN_ERR_INVALID_ARG,
+              "%s: null pointer", what);
+  DeviceInfo* dev;
+  const int rc = current_device(&dev);
+  if (rc) return rc;
+  const NormResidual a{block, residual, w_post, gate, w_next, residual_out, normed, block_row, residual_row, gate_row,
+                       block_dtype, residual_dtype, post_dtype, gate_dtype, next_dtype, gate_kind, gate_sigmoid, dim,
+                       scale, eps};
+  const bool v = dim % 8 == 0 && wide(block, block_dtype, block_row, 0) &&
+                 wide(residual, residual_dtype, residual_row, 0) && wide(w_post, post_dtype, 0, 0) &&
+                 (gate_kind != 2 || wide(gate, gate_dtype, gate_row, 0)) && wide(w_next, next_dtype, 0, 0) &&
+                 aligned(residual_out, 16) && aligned(normed, 16);
+  const int pieces = v ? dim / 8 : dim;
+  const int parts = (pieces + 1023) / 1024;   // pieces of a thread
+  const int per = (pieces + parts - 1) / parts;
+  const int threads = (per + 31) / 32 * 32;
+  auto kernel = v ? (parts <= 1 ? norm_residual_kernel<8, 1> : parts <= 2 ? norm_residual_kernel<8, 2>
+                                                                          : norm_residual_kernel<8, 4>)
+                  : (parts <= 1 ? norm_residual_kernel<1, 1> : parts <= 4 ? norm_residual_kernel<1, 4>
+                                                             : parts <= 8 ? norm_residual_kernel<1, 8>
+                                                                          : norm_residual_kernel<1, 32>);
+  return launch(what, kernel, rows, threads, stream, a);
+}

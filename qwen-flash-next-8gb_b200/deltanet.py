@@ -1,11 +1,25 @@
-"""One-token gated delta rule of the DeltaNet layers on B200 (libqfn's
-qfn_deltanet_step): a drop-in for qwen_engine.recurrent_gated_delta_rule at
-T == 1 (qwen_engine.py:158-174), the call QwenEngine.deltanet makes for every
-linear-attention layer of every decoded token (qwen_engine.py:718-719).
+"""Gated delta rule of the DeltaNet (linear-attention) layers on B200.
+
+recurrent_gated_delta_rule (libqfn's qfn_deltanet_step) is a drop-in for
+qwen_engine.recurrent_gated_delta_rule at T == 1 (qwen_engine.py:158-174), the
+call QwenEngine.deltanet makes for every linear-attention layer of every
+decoded token (qwen_engine.py:718-719).
+
+chunk_gated_delta_rule (qfn_deltanet_chunk) runs the same rule over prompts:
+sequences of any length, ragged batches of them, with a state carried in and
+out.  step_gated_delta_rule (qfn_deltanet_step_batch) runs one token for each
+request of a batch, with the requests' states in slots of a pool.
+
+Per token and value head (value head h uses key head h // (H // Hq)), in fp32:
+
+    q = l2norm(q) / sqrt(dk);  k = l2norm(k)       l2norm: x * rsqrt(sum x^2 + 1e-6)
+    S = exp(g) * S;  d = beta * (v - S^T k);  S = S + k d^T;  out = bf16(S^T q)
+
+All three are forward only.
 """
 import torch
 
-from _lib import check, lib, on_device, require_cuda, stream_of
+from _lib import check, lib, on_device, ops, require_cuda, stream_of
 
 
 def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state):
@@ -34,3 +48,57 @@ def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state):
                                      stream_of(out))
     check(rc, "qfn_deltanet_step")
     return out, initial_state
+
+
+def chunk_gated_delta_rule(query, key, value, g, beta, initial_state=None, cu_seqlens=None, final_state=None,
+                           out=None):
+    """The gated delta rule over whole sequences -> (out, final_state).
+
+    query, key [B, T, Hq, dk] bf16 (dk 64, 128 or 256) . value [B, T, H, dv] bf16
+    (dv a multiple of 32, H a multiple of Hq) . g [B, T, H] fp32 (log of the
+    decay; -inf clears the state) . beta [B, T, H] bf16 -> out [B, T, H, dv]
+    bf16 and final_state [N, H, dk, dv] fp32.
+
+    Without cu_seqlens the N = B rows of the batch are the sequences.  With it
+    (int32 [N + 1] on the device, rising from >= 0 to <= T; B must be 1) sequence n
+    is the tokens cu_seqlens[n] up to cu_seqlens[n + 1]; rows of out outside every
+    sequence are left as they were.  Bounds that do not rise leave out unwritten
+    and every final state NaN.  A sequence may have no token (its state passes
+    through).
+
+    initial_state [N, H, dk, dv] fp32 (None: zeros).  final_state and out may be
+    given to be written; final_state may be initial_state itself.  Views with any
+    row and head strides are taken as they are."""
+    if query.dim() != 4:
+        raise ValueError(f"query must be [B, T, heads, dk], got {tuple(query.shape)}")
+    B, T = query.shape[:2]
+    if cu_seqlens is not None and B != 1:
+        raise ValueError(f"cu_seqlens takes one batch row holding every sequence, got {B}")
+    for name, t, dim in (("key", key, 4), ("value", value, 4), ("g", g, 3), ("beta", beta, 3)):
+        if t.dim() != dim or t.shape[:2] != (B, T):
+            raise ValueError(f"{name} must be [{B}, {T}, ...] with {dim} dimensions, got {tuple(t.shape)}")
+    if out is not None:
+        if tuple(out.shape) != (B, T) + tuple(value.shape[2:]) or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous [{B}, {T}, {value.shape[2]}, {value.shape[3]}], "
+                             f"got {tuple(out.shape)}")
+        out = out.view(B * T, *out.shape[2:])
+    o, S = ops().deltanet_chunk(query.flatten(0, 1), key.flatten(0, 1), value.flatten(0, 1), g.flatten(0, 1),
+                                beta.flatten(0, 1), B, cu_seqlens, initial_state, final_state, out)
+    return o.view(B, T, *o.shape[1:]), S
+
+
+def step_gated_delta_rule(query, key, value, g, beta, state, state_index=None, out_state=None, out=None):
+    """One token of the gated delta rule for each of R requests -> (out, out_state).
+
+    query, key [R, Hq, dk] bf16 . value [R, H, dv] bf16 . g [R, H] fp32 . beta
+    [R, H] bf16 . state [slots, H, dk, dv] fp32 -> out [R, H, dv] bf16.
+
+    Row r's state is state[state_index[r]] (int32 [R] on the device; None: slot
+    r).  A negative index is a padding row: its out is zero and no state is
+    touched.  An index past the pool, or one that an earlier row names too, gives NaN in
+    that row's out and touches no state.  The new states are written to the same slots of out_state
+    (None: state itself, in place); slots that no row names are left as they were."""
+    if out_state is None:
+        out_state = state
+    o = ops().deltanet_step(query, key, value, g, beta, state, state_index, out_state, out)
+    return o, out_state

@@ -11,6 +11,10 @@
 //   qfn::moe_prefill -> qfn_moe_prefill         (the expert loop of QwenEngine.moe, qwen_engine.py:835-852)
 //   qfn::gemv        -> qfn_gemv_e4m3           (fp8gemv.gemv, fp8gemv.py:5-26)
 //   qfn::linear      -> qfn_linear_e4m3         (Lin.__call__ for T > 1, qwen_engine.py:79-83)
+//   qfn::deltanet_chunk  -> qfn_deltanet_chunk      (the gated delta rule over prompts)
+//   qfn::deltanet_step   -> qfn_deltanet_step_batch (one token for each request of a batch)
+//   qfn::gated_norm      -> qfn_gated_norm
+//   qfn::norm_residual   -> qfn_norm_residual
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -157,6 +161,233 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s)
   return y;
 }
 
+// A CUDA tensor of type dt on ref's device; views pass.
+void req_view(const at::Tensor& t, const char* name, at::ScalarType dt, const at::Tensor& ref, const char* ref_name) {
+  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor (libqfn has no CPU path)");
+  req_type(t, name, dt);
+  same_device(t, name, ref, ref_name);
+}
+
+int dtype_code(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name,
+                   " must be bf16 or fp32, got ", t.scalar_type());
+  return t.scalar_type() == at::kFloat ? QFN_DTYPE_F32 : QFN_DTYPE_BF16;
+}
+
+// Whether two tensors' memory (as dense as their sizes say) shares a byte.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.data_ptr()), y = reinterpret_cast<uintptr_t>(b.data_ptr());
+  int64_t na = 0, nb = 0;
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  for (int64_t i = 0; i < a.dim(); ++i) na += (a.size(i) - 1) * a.stride(i);
+  for (int64_t i = 0; i < b.dim(); ++i) nb += (b.size(i) - 1) * b.stride(i);
+  return x < y + (nb + 1) * b.element_size() && y < x + (na + 1) * a.element_size();
+}
+
+// q, k [R, Hq, dk], v [R, H, dv], g, beta [R, H] of the batched delta rule: views of any row and head stride whose
+// last dimension is dense (others are copied).
+struct DeltaRows {
+  at::Tensor q, k, v, g, beta;
+  int64_t strides[10];
+  int H, Hq, dk, dv;
+  DeltaRows(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& g_,
+            const at::Tensor& beta_)
+      : q(q_), k(k_), v(v_), g(g_), beta(beta_) {
+    req_view(q, "query", at::kBFloat16, q, "query");
+    req_view(k, "key", at::kBFloat16, q, "query");
+    req_view(v, "value", at::kBFloat16, q, "query");
+    req_view(g, "g", at::kFloat, q, "query");
+    req_view(beta, "beta", at::kBFloat16, q, "query");
+    TORCH_CHECK_VALUE(q.dim() == 3 && k.sizes() == q.sizes(),
+                      "query and key must have the same shape, with heads and dk last; got ", q_.sizes(), ", ",
+                      k_.sizes());
+    const int64_t R = q.size(0);
+    TORCH_CHECK_VALUE(v.dim() == 3 && v.size(0) == R && q.size(1) >= 1 && v.size(1) >= 1 && v.size(1) % q.size(1) == 0,
+                      "value must hold a multiple of query's ", q.size(1), " heads for its ", R, " tokens; got ",
+                      v_.sizes());
+    TORCH_CHECK_VALUE(g.dim() == 2 && g.size(0) == R && g.size(1) == v.size(1) && beta.sizes() == g.sizes(),
+                      "g and beta must hold ", R, " x ", v.size(1), " values; got ", g_.sizes(), ", ", beta_.sizes());
+    if (q.stride(2) != 1) q = q.contiguous();
+    if (k.stride(2) != 1) k = k.contiguous();
+    if (v.stride(2) != 1) v = v.contiguous();
+    H = static_cast<int>(v.size(1));
+    Hq = static_cast<int>(q.size(1));
+    dk = static_cast<int>(q.size(2));
+    dv = static_cast<int>(v.size(2));
+    const at::Tensor* all[] = {&q, &k, &v, &g, &beta};
+    for (int i = 0; i < 5; ++i) {
+      strides[2 * i] = all[i]->stride(0);
+      strides[2 * i + 1] = all[i]->stride(1);
+    }
+  }
+};
+
+const uint16_t* u16(const at::Tensor& t) { return static_cast<const uint16_t*>(t.data_ptr()); }
+
+void req_state(const at::Tensor& S, const char* name, int64_t n, const DeltaRows& r) {
+  req_view(S, name, at::kFloat, r.q, "query");
+  TORCH_CHECK_VALUE(S.dim() == 4 && (n < 0 || S.size(0) == n) && S.size(1) == r.H && S.size(2) == r.dk &&
+                        S.size(3) == r.dv && S.is_contiguous(),
+                    name, " must be a contiguous fp32 [", n < 0 ? std::string("slots") : std::to_string(n), ", ", r.H, ", ",
+                    r.dk, ", ", r.dv, "], got ", S.sizes());
+}
+
+at::Tensor req_out(const std::optional<at::Tensor>& out, const DeltaRows& r) {
+  if (!out) return at::empty({r.q.size(0), r.H, r.dv}, r.q.options());
+  req_view(*out, "out", at::kBFloat16, r.q, "query");
+  TORCH_CHECK_VALUE(out->is_contiguous() && out->dim() == 3 && out->size(0) == r.q.size(0) && out->size(1) == r.H &&
+                        out->size(2) == r.dv,
+                    "out must be a contiguous bf16 [..., ", r.q.size(0), ", ", r.H, ", ", r.dv, "], got ", out->sizes());
+  TORCH_CHECK_VALUE(!overlap(*out, r.q) && !overlap(*out, r.k) && !overlap(*out, r.v) && !overlap(*out, r.g) &&
+                        !overlap(*out, r.beta),
+                    "out overlaps an input");
+  return *out;
+}
+
+// Rows are the tokens of all sequences; n_seqs sequences of equal length, or those of cu_seqlens.
+std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                  const at::Tensor& g, const at::Tensor& beta, int64_t n_seqs,
+                                                  const std::optional<at::Tensor>& cu,
+                                                  const std::optional<at::Tensor>& s_in,
+                                                  const std::optional<at::Tensor>& s_out,
+                                                  const std::optional<at::Tensor>& out_) {
+  const DeltaRows r(q, k, v, g, beta);
+  if (cu) {
+    req_cuda(*cu, "cu_seqlens");
+    req_type(*cu, "cu_seqlens", at::kInt);
+    same_device(*cu, "cu_seqlens", q, "query");
+    TORCH_CHECK_VALUE(cu->dim() == 1 && cu->size(0) >= 1, "cu_seqlens must be int32 [sequences + 1], got ",
+                      cu->sizes());
+    n_seqs = cu->size(0) - 1;
+  }
+  if (s_in) req_state(*s_in, "initial_state", n_seqs, r);
+  if (s_out) req_state(*s_out, "final_state", n_seqs, r);
+  c10::cuda::CUDAGuard guard(q.device());
+  const int64_t R = q.size(0);
+  at::Tensor out = req_out(out_, r);
+  at::Tensor S = s_out ? *s_out : at::empty({n_seqs, r.H, r.dk, r.dv}, g.options());
+  const size_t nbytes = qfn_deltanet_chunk_workspace(R, n_seqs, r.H, r.Hq, r.dk, r.dv);
+  at::Tensor ws;
+  if (nbytes) ws = at::empty({static_cast<int64_t>(nbytes)}, q.options().dtype(at::kByte));
+  check_rc(qfn_deltanet_chunk(u16(r.q), u16(r.k), u16(r.v), r.g.data_ptr<float>(), u16(r.beta), r.strides,
+                              cu ? cu->data_ptr<int32_t>() : nullptr, n_seqs, R,
+                              s_in ? s_in->data_ptr<float>() : nullptr, S.data_ptr<float>(),
+                              static_cast<uint16_t*>(out.data_ptr()), r.H, r.Hq, r.dk, r.dv,
+                              nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(q)),
+           "qfn_deltanet_chunk");
+  return {out, S};
+}
+
+at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
+                         const at::Tensor& beta, const at::Tensor& state, const std::optional<at::Tensor>& index,
+                         at::Tensor out_state, const std::optional<at::Tensor>& out_) {
+  const DeltaRows r(q, k, v, g, beta);
+  const int64_t R = q.size(0);
+  req_state(state, "state", -1, r);
+  req_state(out_state, "out_state", state.size(0), r);
+  TORCH_CHECK_VALUE(R == 0 || state.size(0) >= 1, "state has no slots");
+  if (index) {
+    req_cuda(*index, "state_index");
+    req_type(*index, "state_index", at::kInt);
+    same_device(*index, "state_index", q, "query");
+    TORCH_CHECK_VALUE(index->dim() == 1 && index->size(0) == R, "state_index must be int32 [", R, "], got ",
+                      index->sizes());
+  }
+  TORCH_CHECK_VALUE(index || R <= state.size(0), "state has ", state.size(0), " slots for ", R,
+                    " tokens (pass state_index)");
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = req_out(out_, r);
+  if (R == 0) return out;
+  check_rc(qfn_deltanet_step_batch(u16(r.q), u16(r.k), u16(r.v), r.g.data_ptr<float>(), u16(r.beta), r.strides,
+                                   index ? index->data_ptr<int32_t>() : nullptr, state.size(0),
+                                   state.data_ptr<float>(), out_state.data_ptr<float>(),
+                                   static_cast<uint16_t*>(out.data_ptr()), R, r.H, r.Hq, r.dk, r.dv, stream_of(q)),
+           "qfn_deltanet_step_batch");
+  return out;
+}
+
+// x, z [R, H, D], w [D] -> [R, H, D]
+at::Tensor gated_norm(const at::Tensor& x_, const at::Tensor& z_, const at::Tensor& w, double eps) {
+  at::Tensor x = x_, z = z_;
+  req_view(x, "x", at::kBFloat16, x, "x");
+  req_view(z, "z", at::kBFloat16, x, "x");
+  req_cuda(w, "weight");
+  same_device(w, "weight", x, "x");
+  TORCH_CHECK_VALUE(x.dim() == 3 && z.sizes() == x.sizes() && w.dim() == 1 && w.size(0) == x.size(2),
+                    "x and z must have the same shape and weight their last size; got ", x.sizes(), ", ", z.sizes(),
+                    ", ", w.sizes());
+  if (x.stride(2) != 1) x = x.contiguous();
+  if (z.stride(2) != 1) z = z.contiguous();
+  const int wd = dtype_code(w, "weight");
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  if (y.numel() == 0) return y;
+  check_rc(qfn_gated_norm(u16(x), x.stride(0), x.stride(1), u16(z), z.stride(0), z.stride(1), w.data_ptr(), wd,
+                          static_cast<uint16_t*>(y.data_ptr()), x.size(0), static_cast<int>(x.size(1)),
+                          static_cast<int>(x.size(2)), static_cast<float>(eps), stream_of(y)),
+           "qfn_gated_norm");
+  return y;
+}
+
+// block, residual [T, D]; gate [T, 1] or [T, D]; residual_out: residual's type, contiguous.
+std::tuple<at::Tensor, at::Tensor> norm_residual(const at::Tensor& block_, const at::Tensor& residual_,
+                                                 const std::optional<at::Tensor>& post,
+                                                 const std::optional<at::Tensor>& gate_, bool sigmoid, double scale,
+                                                 const std::optional<at::Tensor>& next, double eps,
+                                                 const std::optional<at::Tensor>& r_out) {
+  at::Tensor block = block_, residual = residual_, gate;
+  TORCH_CHECK_VALUE(block.is_cuda(), "block must be a CUDA tensor (libqfn has no CPU path)");
+  TORCH_CHECK_VALUE(residual.is_cuda(), "residual must be a CUDA tensor (libqfn has no CPU path)");
+  same_device(residual, "residual", block, "block");
+  TORCH_CHECK_VALUE(block.dim() == 2 && residual.sizes() == block.sizes(),
+                    "block and residual must have the same shape; got ", block.sizes(), ", ", residual.sizes());
+  const int64_t T = block.size(0), D = block.size(1);
+  const int bd = dtype_code(block, "block"), rd = dtype_code(residual, "residual");
+  if (block.stride(1) != 1) block = block.contiguous();
+  if (residual.stride(1) != 1) residual = residual.contiguous();
+  int kind = 0, gd = QFN_DTYPE_BF16, pd = QFN_DTYPE_BF16, nd = QFN_DTYPE_BF16;
+  if (gate_) {
+    gate = *gate_;
+    TORCH_CHECK_VALUE(gate.is_cuda(), "gate must be a CUDA tensor (libqfn has no CPU path)");
+    same_device(gate, "gate", block, "block");
+    gd = dtype_code(gate, "gate");
+    TORCH_CHECK_VALUE(gate.dim() == 2 && gate.size(0) == T && (gate.size(1) == 1 || gate.size(1) == D),
+                      "gate must be [", T, ", 1] or [", T, ", ", D, "], got ", gate.sizes());
+    kind = gate.size(1) == D ? 2 : 1;
+    if (kind == 2 && D > 1 && gate.stride(1) != 1) gate = gate.contiguous();
+  }
+  for (const auto& w : {std::make_pair(&post, "post_weight"), std::make_pair(&next, "next_weight")}) {
+    if (!*w.first) continue;
+    req_cuda(**w.first, w.second);
+    same_device(**w.first, w.second, block, "block");
+    TORCH_CHECK_VALUE((*w.first)->dim() == 1 && (*w.first)->size(0) == D, w.second, " must be [", D, "], got ",
+                      (*w.first)->sizes());
+  }
+  if (post) pd = dtype_code(*post, "post_weight");
+  if (next) nd = dtype_code(*next, "next_weight");
+  c10::cuda::CUDAGuard guard(block.device());
+  at::Tensor r = r_out ? *r_out : at::empty({T, D}, residual.options());
+  if (r_out) {
+    req_view(r, "out", residual.scalar_type(), block, "block");
+    TORCH_CHECK_VALUE(r.is_contiguous() && r.sizes() == block.sizes(), "out must be a contiguous [", T, ", ", D,
+                      "], got ", r.sizes());
+    // in place of the residual itself is fine: a thread writes what it has read
+    TORCH_CHECK_VALUE((r.data_ptr() == residual.data_ptr() && residual.is_contiguous()) || !overlap(r, residual),
+                      "out overlaps the residual without being it");
+    TORCH_CHECK_VALUE(!overlap(r, block) && !(kind && overlap(r, gate)), "out overlaps block or gate");
+  }
+  at::Tensor n = next ? at::empty({T, D}, block.options().dtype(at::kBFloat16)) : at::Tensor();
+  if (T == 0 || D == 0) return {r, next ? n : r};
+  check_rc(qfn_norm_residual(block.data_ptr(), bd, block.stride(0), residual.data_ptr(), rd, residual.stride(0),
+                             post ? post->data_ptr() : nullptr, pd, kind ? gate.data_ptr() : nullptr, kind, gd,
+                             kind ? gate.stride(0) : 0, sigmoid, static_cast<float>(scale),
+                             next ? next->data_ptr() : nullptr, nd, r.data_ptr(),
+                             next ? static_cast<uint16_t*>(n.data_ptr()) : nullptr, T, static_cast<int>(D),
+                             static_cast<float>(eps), stream_of(r)),
+           "qfn_norm_residual");
+  return {r, next ? n : r};
+}
+
 }  // namespace
 
 // Catch-all kernels (not per dispatch key): a CPU tensor reaches the checks
@@ -167,4 +398,14 @@ TORCH_LIBRARY(qfn, m) {
   m.def("moe_prefill(Tensor x, Tensor ti, Tensor tv, Tensor table, Tensor s2, int L) -> Tensor", &moe_prefill);
   m.def("gemv(Tensor q, Tensor s, Tensor x, bool out_f32) -> Tensor", &gemv);
   m.def("linear(Tensor x, Tensor q, Tensor s) -> Tensor", &linear);
+  m.def("deltanet_chunk(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, int n_seqs, Tensor? cu_seqlens, "
+        "Tensor? initial_state, Tensor(a!)? final_state, Tensor(b!)? out) -> (Tensor, Tensor)",
+        &deltanet_chunk);
+  m.def("deltanet_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor state, Tensor? state_index, "
+        "Tensor(a!) out_state, Tensor(b!)? out) -> Tensor",
+        &deltanet_step);
+  m.def("gated_norm(Tensor x, Tensor z, Tensor weight, float eps) -> Tensor", &gated_norm);
+  m.def("norm_residual(Tensor block, Tensor residual, Tensor? post_weight, Tensor? gate, bool sigmoid, float scale, "
+        "Tensor? next_weight, float eps, Tensor(a!)? out) -> (Tensor, Tensor)",
+        &norm_residual);
 }
