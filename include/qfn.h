@@ -153,8 +153,8 @@ int qfn_moe_decode_noalloc(const uint8_t* table, int64_t n_blocks, const int32_t
 
 /*
  * qfn_device_status -- read (and with clear != 0, reset) the device status
- * words of the decode, GEMV and FP8 linear kernels of the current device,
- * OR-ed: bit 0 = a bounded wait on a shared-memory barrier ran out (the
+ * words of the decode, GEMV, FP8 linear and chunked delta rule kernels of the
+ * current device, OR-ed: bit 0 = a bounded wait on a shared-memory barrier ran out (the
  * outputs of that call are invalid).
  * Synchronous (a device-to-host copy).  No counterpart in the reference,
  * whose kernels have no waits.

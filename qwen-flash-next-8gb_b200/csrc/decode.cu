@@ -356,11 +356,12 @@ extern "C" int qfn_device_status(unsigned int* status, int clear) {
     e = cudaMemcpyToSymbol(g_decode_status, &zero, sizeof(unsigned int));
   }
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "qfn_device_status: %s", cudaGetErrorString(e));
-  // the GEMV's and the FP8 linear layer's words (same bit meanings)
-  unsigned int g = 0, l = 0;
+  // the GEMV's, the FP8 linear layer's and the chunked delta rule's words (same bit meanings)
+  unsigned int g = 0, l = 0, d = 0;
   int rc = gemv_status(&g, clear != 0);
   if (rc == QFN_OK) rc = linear_status(&l, clear != 0);
-  *status |= g | l;
+  if (rc == QFN_OK) rc = dn_chunk_status(&d, clear != 0);
+  *status |= g | l | d;
   return rc;
 }
 

@@ -16,6 +16,7 @@
 // thread's rows, then two shuffles and four warps through shared memory in a
 // fixed order: results do not depend on the batch.
 #include "deltanet_batch.cuh"
+#include "deltanet_chunk.cuh"
 
 namespace qfn {
 
@@ -270,7 +271,8 @@ extern "C" int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, con
 
 extern "C" size_t qfn_deltanet_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk,
                                                int dv) {
-  return 0;
+  if (tokens < 0 || n_seqs < 1 || n_heads < 1 || n_key_heads < 1 || !dn_chunk_takes(tokens, dk)) return 0;
+  return dn_chunk_workspace(tokens, n_seqs, n_heads, n_key_heads, dk);
 }
 
 extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* g,
@@ -292,9 +294,18 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
   QFN_REQUIRE(tokens < (int64_t{1} << 31) - 64, QFN_ERR_UNSUPPORTED, "%s: tokens=%lld", what,
               static_cast<long long>(tokens));
   if (n_seqs == 0) return QFN_OK;
+  const bool chunked = dn_chunk_takes(tokens, dk);
+  if (chunked) {
+    const size_t need = dn_chunk_workspace(tokens, n_seqs, n_heads, n_key_heads, dk);
+    QFN_REQUIRE(workspace && workspace_bytes >= need, QFN_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what,
+                workspace ? workspace_bytes : size_t{0}, need);
+    QFN_REQUIRE(aligned(workspace, 256), QFN_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", what);
+    QFN_REQUIRE(aligned(out, 4), QFN_ERR_ALIGNMENT, "%s: out must be 4-byte aligned", what);
+  }
   DeviceInfo* dev;
   rc = current_device(&dev);
   if (rc) return rc;
+  if (chunked) return dn_chunk(a, cu_seqlens, n_seqs, tokens, dk, workspace, stream);
   const int64_t blocks = n_seqs * n_heads * (dv / kDbCols);
   auto kernel = dk == 64 ? deltanet_recurrence_kernel<64>
                          : dk == 128 ? deltanet_recurrence_kernel<128> : deltanet_recurrence_kernel<256>;

@@ -20,6 +20,7 @@ import math
 import pytest
 import torch
 
+import _lib
 import deltanet
 import fp8gemv
 import norms
@@ -28,6 +29,12 @@ import synthetic
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 U = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    assert _lib.device_status() == 0
 
 
 def inputs(tokens, H, Hk, dk, dv, seed, strided=True):
@@ -108,6 +115,11 @@ def test_chunk_matches_recurrence(lens, H, Hk, dk, dv):
 @pytest.mark.parametrize("carried", [False, True])
 def test_chunk_long_sequence(carried):
     run_ragged([2049], 2, 1, 128, 128, seed=5, carried=carried)
+
+
+def test_chunk_more_than_one_segment():
+    """More chunks than one workspace holds: the state goes from segment to segment through memory."""
+    run_ragged([100, 6000, 0, 40], 32, 32, 128, 32, seed=8, carried=True)
 
 
 def test_chunk_many_short_sequences():

@@ -47,6 +47,10 @@ def test_chunk_refusals():
     assert chunk(s_in=ODD) == 2
     assert chunk(s_out=ctypes.c_void_p(0x10100)) == 1
     assert chunk(T=2 ** 31) == 4
+    need = _lib.lib().qfn_deltanet_chunk_workspace(100, 2, 4, 2, 128, 128)
+    assert need > 0 and chunk(bytes_=need - 1) == 5 and chunk(ws=None) == 5
+    assert chunk(ws=ctypes.c_void_p(0x7f0000000010)) == 2
+    assert _lib.lib().qfn_deltanet_chunk_workspace(100, 0, 4, 2, 128, 128) == 0
     assert chunk(n=0, T=0) == 0 and chunk(n=0, T=0, q=None, s_out=None) == 0
 
 
