@@ -29,14 +29,14 @@ constexpr int kCols = 32;        // state columns of a block
 constexpr int kStages = 3;       // chunks of what the recurrence reads
 constexpr int kOutStages = 2;    // chunks of what only the outputs read
 constexpr int kPrepThreads = 256;
-constexpr int kThreads = 9 * 32; // 4 warps of the recurrence, 4 of the outputs, 1 of the copies
+constexpr int kThreads = 13 * 32; // 8 warps of the recurrence, 4 of the outputs, 1 of the copies
 constexpr int kGS = 68;          // row pitch of the 64 x 64 fp32 matrices of dn_prep_kernel
 
 // Per chunk and value head: T hi, T lo (f16, 128-byte rows, swizzled), the
 // tokens' factors and the chunk's scales, then P (as T).
 constexpr int kMat = C * C * 2;
 enum { kFA = 0, kFB = C, kFQ = 2 * C, kFW = 3 * C, kFEnd = 4 * C };   // -beta e^G ck, beta, e^G cq, e^(G64 - G) ck
-constexpr int kFactors = 4 * C + 4;   // + e^G64, scale of T, scale of P
+constexpr int kFactors = 4 * C + 4;   // + e^G64, scale of T, scale of P, largest row sum of e^(G64 - G) ck |T|
 constexpr int kRecBytes = 2 * kMat + kFactors * 4;
 constexpr int kHeadBytes = kRecBytes + kMat;
 
@@ -109,17 +109,6 @@ __device__ __forceinline__ uint32_t swz(int row, int ch) {
 }
 
 // ------------------------------------------------------------------ what needs no state
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {   // kPrepThreads threads
-  v = __reduce_max_sync(0xffffffffu, v);
-  __syncthreads();   // red may still be read from the last call
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint32_t m = red[0];
-#pragma unroll
-  for (int i = 1; i < kPrepThreads / 32; ++i) m = max(m, red[i]);
-  return m;
-}
-
 template <int DK>
 struct PrepSmem {
   union {
@@ -127,126 +116,128 @@ struct PrepSmem {
       unsigned char k[C * DK * 2], q[C * DK * 2];   // f16 rows, swizzled
     };
     struct {
-      float t[C * kGS];        // A, then T
-      float y[3 * 16 * 20];    // a level's sums
+      float t[C * kGS];     // A, then T
+      float y[32 * 36];     // A21 T11
     };
   };
   float gk[C * kGS], gq[C * kGS];   // k_i . k_j, q_i . k_j of the scaled rows
-  double g[C];
-  float ck[C], cq[C], beta[C];
-  uint32_t red[kPrepThreads / 32];
+  float g_hi[C], g_lo[C], ck[C], cq[C], beta[C], w[C];
+  uint32_t red[2][kPrepThreads / 32];
+  float p_scale;
 };
 
-// The inverse of I + A, A strictly lower triangular in t: 16 x 16 blocks on
-// the diagonal by substitution, then T_ij = -T_ii sum_k A_ik T_kj diagonal by
-// diagonal, in fp32.  Block T_ij below the diagonal is left at block (j, i),
-// since A_ij is still needed: t_at gives an element's place.
-__device__ __forceinline__ int t_at(int i, int j) { return ((j & ~15) + (i & 15)) * kGS + (i & ~15) + (j & 15); }
-
+// The inverse of I + A, A strictly lower triangular in t, in fp32: the two 32 x 32 halves of the
+// diagonal by substitution, a column per lane, then T21 = -T22 (A21 T11) by the whole block.
 template <int DK>
 __device__ __forceinline__ void invert(PrepSmem<DK>& sm) {
-  const int tid = threadIdx.x;
-  float x[16];
-  const int b = tid >> 4, c = tid & 15;   // block, column (the first 64 threads)
-  if (tid < 64) {
+  const int tid = threadIdx.x, w = tid >> 5, c = tid & 31;
+  if (w < 2) {
+    float* t = sm.t + w * 32 * (kGS + 1);
+    float x[32];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == c ? 1.f : 0.f;
+    for (int i = 0; i < 32; ++i) {
+      float s[4] = {i == c ? 1.f : 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < i; ++j) s = fmaf(-sm.t[(b * 16 + i) * kGS + b * 16 + j], x[j], s);
-      x[i] = s;
+      for (int j = 0; j < i; j += 4) {
+        const float4 r = *reinterpret_cast<const float4*>(t + i * kGS + j);   // zero from the diagonal on
+        s[0] = fmaf(-r.x, x[j], s[0]);
+        if (j + 1 < i) s[1] = fmaf(-r.y, x[j + 1], s[1]);
+        if (j + 2 < i) s[2] = fmaf(-r.z, x[j + 2], s[2]);
+        if (j + 3 < i) s[3] = fmaf(-r.w, x[j + 3], s[3]);
+      }
+      x[i] = (s[0] + s[1]) + (s[2] + s[3]);
     }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t[i * kGS + c] = x[i];
   }
   __syncthreads();
-  if (tid < 64) {
+  // a thread: row r, columns c4 .. c4 + 3
+  const int r = tid >> 3, c4 = (tid & 7) * 4;
+  auto product = [&](const float* row, const float* m, int pitch) {
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int k = 0; k < 32; k += 4) {
+      const float4 av = *reinterpret_cast<const float4*>(row + k);
+      const float ak[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sm.t[(b * 16 + i) * kGS + b * 16 + c] = x[i];
-  }
-  // 64 threads per block of a diagonal: row r, columns c4 .. c4 + 3
-  const int u = tid >> 6, r = (tid >> 2) & 15, c4 = (tid & 3) * 4;
-#pragma unroll 1
-  for (int d = 1; d < 4; ++d) {
-    __syncthreads();
-    const int bi = u + d, bj = u;
-    const bool on = u < 4 - d;
-    if (on) {
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = bj * 16; k < bi * 16; ++k) {
-        const float a = sm.t[(bi * 16 + r) * kGS + k];
-        const float4 w = *reinterpret_cast<const float4*>(&sm.t[t_at(k, bj * 16 + c4)]);
-        y.x = fmaf(a, w.x, y.x); y.y = fmaf(a, w.y, y.y); y.z = fmaf(a, w.z, y.z); y.w = fmaf(a, w.w, y.w);
+      for (int i = 0; i < 4; ++i) {
+        const float4 b = *reinterpret_cast<const float4*>(m + (k + i) * pitch + c4);
+        y.x = fmaf(ak[i], b.x, y.x); y.y = fmaf(ak[i], b.y, y.y); y.z = fmaf(ak[i], b.z, y.z); y.w = fmaf(ak[i], b.w, y.w);
       }
-      *reinterpret_cast<float4*>(&sm.y[u * 320 + r * 20 + c4]) = y;
     }
-    __syncthreads();
-    if (on) {
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float a = -sm.t[(bi * 16 + r) * kGS + bi * 16 + k];
-        const float4 w = *reinterpret_cast<const float4*>(&sm.y[u * 320 + k * 20 + c4]);
-        y.x = fmaf(a, w.x, y.x); y.y = fmaf(a, w.y, y.y); y.z = fmaf(a, w.z, y.z); y.w = fmaf(a, w.w, y.w);
-      }
-      *reinterpret_cast<float4*>(&sm.t[t_at(bi * 16 + r, bj * 16 + c4)]) = y;
-    }
-  }
+    return y;
+  };
+  *reinterpret_cast<float4*>(&sm.y[r * 36 + c4]) = product(sm.t + (32 + r) * kGS, sm.t, kGS);
+  __syncthreads();
+  const float4 y = product(sm.t + (32 + r) * kGS + 32, sm.y, 36);
+  *reinterpret_cast<float4*>(&sm.t[(32 + r) * kGS + c4]) = make_float4(-y.x, -y.y, -y.z, -y.w);
   __syncthreads();
 }
 
-// One bf16 row of q or k (zero behind the sequence's end) as f16: the row's
-// scale 2^e, its factor (1 / norm) 2^-e, the swizzled row in shared memory.
+// DK / 8 bf16 of a row, 16 bytes at a time.
 template <int DK>
-__device__ __forceinline__ void f16_row(const float (&x)[DK / 32], unsigned char* tile, int row, float* factor,
-                                        float divide) {
-  const int lane = threadIdx.x & 31;
-  float ss = 0.f;
-  uint32_t m = 0;
+__device__ __forceinline__ void load_row(const uint16_t* p, bool in, bool vec, uint4 (&x)[DK / 64]) {
 #pragma unroll
-  for (int i = 0; i < DK / 32; ++i) {
-    ss = fmaf(x[i], x[i], ss);
-    m = max(m, finite_bits(x[i]));
-  }
-  ss = warp_sum(ss);
-  m = __reduce_max_sync(0xffffffffu, m);
-  const int e = scale_exp(m);
-  const float s = exp2i(e);
-  // lane holds elements lane * (DK / 32) ...
-  constexpr int kPer = DK / 32;
-  const uint32_t at = swz<DK * 2>(row, lane * kPer / 8) + (lane * kPer % 8) * 2;
+  for (int i = 0; i < DK / 64; ++i) {
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (!in) continue;
+    if (vec) {
+      x[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      uint32_t u[4];
 #pragma unroll
-  for (int i = 0; i < kPer; i += 2)
-    *reinterpret_cast<uint32_t*>(tile + at + i * 2) = pack_h2(x[i] * s, x[i + 1] * s);
-  // a row of zeros counts for nothing: its factor, up to 1000, would take the others' digits.  (An
-  // infinity has m = 0 too where nothing else is finite; its sum keeps it.)
-  if (lane == 0) *factor = ss == 0.f ? 0.f : rsqrtf(ss + 1e-6f) / divide * exp2i(-e);
-}
-
-template <int DK>
-__device__ __forceinline__ void load_row(const uint16_t* p, bool in, bool vec, float (&x)[DK / 32]) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = DK / 32;
-  if (!in) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = 0.f;
-    return;
-  }
-  p += lane * kPer;
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < kPer; i += 2) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p + i);
-      x[i] = __uint_as_float(w << 16);
-      x[i + 1] = __uint_as_float(w & 0xffff0000u);
+      for (int j = 0; j < 4; ++j) u[j] = p[i * 8 + 2 * j] | static_cast<uint32_t>(p[i * 8 + 2 * j + 1]) << 16;
+      x[i] = make_uint4(u[0], u[1], u[2], u[3]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = bf16_bits_to_f32(p[i]);
   }
 }
 
+// Eight lanes hold a bf16 row of q or k: as f16 after a power-of-two scale 2^e (bf16 is exact in f16 then) to
+// shared memory and to the workspace, both swizzled; the row's factor (1 / norm) 2^-e.
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads) dn_prep_kernel(const DnRows a, const Plan plan, const Work work,
-                                                               int64_t slot0, bool vec) {
+__device__ __forceinline__ void f16_row(const uint4 (&x)[DK / 64], unsigned char* tile, unsigned char* copy, int row,
+                                        float* factor, float divide) {
+  const int part = threadIdx.x & 7;
+  constexpr int N = DK / 8;
+  float v[N], ss[2] = {0.f, 0.f}, m[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < DK / 64; ++i) {
+    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[i * 8 + 2 * j] = __uint_as_float(u[j] << 16);
+      v[i * 8 + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    ss[i & 1] = fmaf(v[i], v[i], ss[i & 1]);
+    m[i & 1] = fmaxf(m[i & 1], fabsf(v[i]));
+  }
+  float s = ss[0] + ss[1], mm = fmaxf(m[0], m[1]);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  }
+  const int e = scale_exp(__float_as_uint(mm));
+  const float sc = exp2i(e);
+#pragma unroll
+  for (int i = 0; i < DK / 64; ++i) {
+    const uint4 h = make_uint4(pack_h2(v[i * 8] * sc, v[i * 8 + 1] * sc), pack_h2(v[i * 8 + 2] * sc, v[i * 8 + 3] * sc),
+                               pack_h2(v[i * 8 + 4] * sc, v[i * 8 + 5] * sc), pack_h2(v[i * 8 + 6] * sc, v[i * 8 + 7] * sc));
+    const uint32_t at = swz<DK * 2>(row, part * (DK / 64) + i);
+    *reinterpret_cast<uint4*>(tile + at) = h;
+    *reinterpret_cast<uint4*>(copy + at) = h;
+  }
+  // a row of zeros counts for nothing: its factor, up to 1000, would take the others' digits
+  if (part == 0) *factor = s == 0.f ? 0.f : rsqrtf(s + 1e-6f) / divide * exp2i(-e);
+}
+
+template <int DK>
+__global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a, const Plan plan, const Work work,
+                                                                  int64_t slot0, bool vec) {
   extern __shared__ __align__(1024) unsigned char raw[];
   PrepSmem<DK>& sm = *reinterpret_cast<PrepSmem<DK>*>(raw);
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
@@ -264,44 +255,38 @@ __global__ void __launch_bounds__(kPrepThreads) dn_prep_kernel(const DnRows a, c
     n = count - 1;
     if (n < 0 || !dn_plan_ok(plan.cu, plan.n_seqs, plan.tokens)) return;
   } else {
-    n = min(slot * C / (plan.tokens / plan.n_seqs + C) , plan.n_seqs - 1);
+    n = min(slot * C / (plan.tokens / plan.n_seqs + C), plan.n_seqs - 1);
     while (n + 1 < plan.n_seqs && plan.slot(n + 1) <= slot) ++n;
   }
   const int64_t t0 = plan.begin(n) + (slot - plan.slot(n)) * C;
   const int cnt = static_cast<int>(min(static_cast<int64_t>(C), plan.end(n) - t0));
   if (cnt <= 0) return;
 
-  // k and q rows: 8 of each per warp
+  // k and q rows: a warp takes four rows at a time, eight of each in all
   {
-    const uint16_t* src[2] = {a.k + hk * a.k_head, a.q + hk * a.q_head};
-    const int64_t row[2] = {a.k_row, a.q_row};
+    const uint16_t* src[2] = {a.k + hk * a.k_head + (lane & 7) * (DK / 8), a.q + hk * a.q_head + (lane & 7) * (DK / 8)};
+    const int64_t pitch[2] = {a.k_row, a.q_row};
+    unsigned char* copy = work.kq + ((slot - slot0) * key_heads + hk) * (2 * C * DK * 2);
+    uint4 x[4][DK / 64];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      float x[8][DK / 32];
+    for (int i = 0; i < 4; ++i) {
+      const int r = w * 8 + (i & 1) * 4 + (lane >> 3);
+      load_row<DK>(src[i >> 1] + (t0 + r) * pitch[i >> 1], r < cnt, vec, x[i]);
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = w * 8 + i;
-        load_row<DK>(src[m] + (t0 + r) * row[m], r < cnt, vec, x[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        f16_row<DK>(x[i], m ? sm.q : sm.k, w * 8 + i, m ? &sm.cq[w * 8 + i] : &sm.ck[w * 8 + i], m ? a.q_scale : 1.f);
+    for (int i = 0; i < 4; ++i) {
+      const int r = w * 8 + (i & 1) * 4 + (lane >> 3);
+      f16_row<DK>(x[i], i < 2 ? sm.k : sm.q, copy + (i < 2 ? 0 : C * DK * 2), r, i < 2 ? &sm.ck[r] : &sm.cq[r],
+                  i < 2 ? 1.f : a.q_scale);
     }
   }
   __syncthreads();
-  // the rows to the workspace, as they lie
-  {
-    uint4* dst = reinterpret_cast<uint4*>(work.kq + ((slot - slot0) * key_heads + hk) * (2 * C * DK * 2));
-    const uint4* src = reinterpret_cast<const uint4*>(sm.k);
-#pragma unroll
-    for (int i = 0; i < 2 * C * DK * 2 / 16 / kPrepThreads; ++i) dst[i * kPrepThreads + tid] = src[i * kPrepThreads + tid];
-  }
   // k_i . k_j (warps 0-3) and q_i . k_j (warps 4-7), 16 rows per warp, up to the diagonal's block
   {
-    const int m = w & 3;
+    const int m = w & 3, g = lane >> 2, t = lane & 3;
     const uint32_t rows = smem_u32(w < 4 ? sm.k : sm.q), cols = smem_u32(sm.k);
     float acc[8][4] = {};
-#pragma unroll
+#pragma unroll 2
     for (int kt = 0; kt < DK / 16; ++kt) {
       uint32_t x[4];
       ldsm4(x, rows + swz<DK * 2>(m * 16 + (lane & 15), kt * 2 + (lane >> 4)));
@@ -315,7 +300,6 @@ __global__ void __launch_bounds__(kPrepThreads) dn_prep_kernel(const DnRows a, c
       }
     }
     float* dst = w < 4 ? sm.gk : sm.gq;
-    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (j / 2 > m) continue;
@@ -323,22 +307,23 @@ __global__ void __launch_bounds__(kPrepThreads) dn_prep_kernel(const DnRows a, c
       *reinterpret_cast<float2*>(&dst[(m * 16 + g + 8) * kGS + j * 8 + 2 * t]) = make_float2(acc[j][2], acc[j][3]);
     }
   }
-  __syncthreads();   // the k and q tiles are free for A and T from here
+  // the k and q tiles are free for A and T after the barrier below
 
 #pragma unroll 1
   for (int hv = 0; hv < a.ratio; ++hv) {
     const int h = hk * a.ratio + hv;
     unsigned char* dst = work.heads + ((slot - slot0) * a.heads + h) * static_cast<int64_t>(kHeadBytes);
     float* factors = reinterpret_cast<float*>(dst + 2 * kMat);
-    // Running sum of g in 64 bits: differences of far tokens' sums keep their
+    // Running sum of g in 64 bits, kept as two floats: differences of far tokens' sums keep their
     // digits.  exp(-200) is 0 in fp32, and a finite sum keeps exp(G_i - G_j) a number.
     if (w == 0) {
       double s[2];
-      float bt[2];
+      float bt[2], rise = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = 2 * lane + i;
         const float gv = r < cnt ? a.g[(t0 + r) * a.g_row + h * a.g_head] : 0.f;
+        rise += fmaxf(gv, 0.f);
         s[i] = gv < -200.f ? -200.f : gv;
         bt[i] = r < cnt ? bf16_bits_to_f32(a.beta[(t0 + r) * a.b_row + h * a.b_head]) : 0.f;
       }
@@ -348,81 +333,125 @@ __global__ void __launch_bounds__(kPrepThreads) dn_prep_kernel(const DnRows a, c
         const double up = __shfl_up_sync(0xffffffffu, run, o);
         if (lane >= o) run += up;
       }
+      rise = warp_sum(rise);
       const double G[2] = {run - s[1], run};
       const double last = __shfl_sync(0xffffffffu, run, 31);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = 2 * lane + i;
-        sm.g[r] = G[i];
+        const float hi = static_cast<float>(G[i]);
+        sm.g_hi[r] = hi;
+        sm.g_lo[r] = static_cast<float>(G[i] - hi);
         sm.beta[r] = bt[i];
-        const float eg = expf(static_cast<float>(G[i]));
+        const float eg = expf(hi), wt = expf(static_cast<float>(last - G[i])) * sm.ck[r];
+        sm.w[r] = wt;
         factors[kFA + r] = -bt[i] * eg * sm.ck[r];
         factors[kFB + r] = bt[i];
         factors[kFQ + r] = eg * sm.cq[r];
-        factors[kFW + r] = expf(static_cast<float>(last - G[i])) * sm.ck[r];
+        factors[kFW + r] = wt;
       }
-      if (lane == 0) factors[kFEnd] = expf(static_cast<float>(last));
+      if (lane == 0) {
+        // |q_i . k_j| <= 1 / q_scale after the norms, and no decay is above the sum of the rises
+        const float bound = expf(rise) / a.q_scale * 1.01f;
+        const int e = bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
+        sm.p_scale = exp2i(e);
+        factors[kFEnd] = expf(static_cast<float>(last));
+        factors[kFEnd + 2] = exp2i(-e);
+      }
     }
     __syncthreads();
-    // A into t; P from registers
-    float p[2][8];
-    uint32_t pm = 0;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int i = s * 32 + (tid >> 3), j0 = (tid & 7) * 8;
-      const double gi = sm.g[i];
-      const float bi = sm.beta[i] * sm.ck[i], qi = sm.cq[i];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int jj = j0 + j;
-        float av = 0.f, pv = 0.f;
-        if (jj <= i) {
-          const float f = expf(static_cast<float>(gi - sm.g[jj])) * sm.ck[jj];
-          pv = f * qi * sm.gq[i * kGS + jj];
-          if (jj < i) av = f * bi * sm.gk[i * kGS + jj];
-        }
-        sm.t[i * kGS + jj] = av;
-        p[s][j] = pv;
-        pm = max(pm, finite_bits(pv));
-      }
-    }
-    const int ep = scale_exp(block_max(pm, sm.red));
+    // A into t and P out: eight columns j0 .. j0 + 7 a warp, a row per lane
+    const int j0 = w * 8;
     {
-      const float sc = exp2i(ep);
+      const float psc = sm.p_scale;
+#pragma unroll 1
+      for (int s = 0; s < 2; ++s) {
+        const int i = s * 32 + lane;
+        float av[8], pv[8];
+        if (j0 < (s + 1) * 32) {
+          const float gh = sm.g_hi[i], gl = sm.g_lo[i], bi = sm.beta[i] * sm.ck[i], qi = sm.cq[i] * psc;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        *reinterpret_cast<uint4*>(dst + kRecBytes + swz<128>(s * 32 + (tid >> 3), tid & 7)) =
-            make_uint4(pack_h2(p[s][0] * sc, p[s][1] * sc), pack_h2(p[s][2] * sc, p[s][3] * sc),
-                       pack_h2(p[s][4] * sc, p[s][5] * sc), pack_h2(p[s][6] * sc, p[s][7] * sc));
-    }
-    invert(sm);
-    uint32_t tm = 0;
+          for (int j4 = 0; j4 < 8; j4 += 4) {
+            const float4 h4 = *reinterpret_cast<const float4*>(&sm.g_hi[j0 + j4]);
+            const float4 l4 = *reinterpret_cast<const float4*>(&sm.g_lo[j0 + j4]);
+            const float4 c4 = *reinterpret_cast<const float4*>(&sm.ck[j0 + j4]);
+            const float4 k4 = *reinterpret_cast<const float4*>(&sm.gk[i * kGS + j0 + j4]);
+            const float4 q4 = *reinterpret_cast<const float4*>(&sm.gq[i * kGS + j0 + j4]);
+            const float hj[4] = {h4.x, h4.y, h4.z, h4.w}, lj[4] = {l4.x, l4.y, l4.z, l4.w},
+                        cj[4] = {c4.x, c4.y, c4.z, c4.w}, kj[4] = {k4.x, k4.y, k4.z, k4.w},
+                        qj[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int i = s * 32 + (tid >> 3), j0 = (tid & 7) * 8;
+            for (int j = 0; j < 4; ++j) {
+              const int jj = j0 + j4 + j;
+              const float f = expf((gh - hj[j]) + (gl - lj[j])) * cj[j];
+              pv[j4 + j] = jj <= i ? f * qi * qj[j] : 0.f;
+              av[j4 + j] = jj < i ? f * bi * kj[j] : 0.f;
+            }
+          }
+        } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[s][j] = j0 + j <= i ? sm.t[t_at(i, j0 + j)] : 0.f;
-        tm = max(tm, finite_bits(p[s][j]));
+          for (int j = 0; j < 8; ++j) av[j] = pv[j] = 0.f;
+        }
+        *reinterpret_cast<float4*>(&sm.t[i * kGS + j0]) = make_float4(av[0], av[1], av[2], av[3]);
+        *reinterpret_cast<float4*>(&sm.t[i * kGS + j0 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
+        *reinterpret_cast<uint4*>(dst + kRecBytes + swz<128>(i, w)) =
+            make_uint4(pack_h2(pv[0], pv[1]), pack_h2(pv[2], pv[3]), pack_h2(pv[4], pv[5]), pack_h2(pv[6], pv[7]));
       }
     }
-    const int et = scale_exp(block_max(tm, sm.red));
+    __syncthreads();
+    invert(sm);
+    // T's scale, and a bound of the weighted d for the walk: the largest row sum of w |T| (eight lanes a row)
+    float tv[2][8];
+    uint32_t tm = 0, wm = 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int i = s * 32 + (tid >> 3), jt = (tid & 7) * 8;
+      float sum = 0.f;
+#pragma unroll
+      for (int j4 = 0; j4 < 8; j4 += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(&sm.t[i * kGS + jt + j4]);
+        tv[s][j4] = v.x; tv[s][j4 + 1] = v.y; tv[s][j4 + 2] = v.z; tv[s][j4 + 3] = v.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (jt + j > i) tv[s][j] = 0.f;
+        const uint32_t b = finite_bits(tv[s][j]);
+        tm = max(tm, b);
+        sum += __uint_as_float(b);
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      wm = max(wm, finite_bits(sum * sm.w[i]));
+    }
+    tm = __reduce_max_sync(0xffffffffu, tm);
+    wm = __reduce_max_sync(0xffffffffu, wm);
+    if (lane == 0) {
+      sm.red[0][w] = tm;
+      sm.red[1][w] = wm;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPrepThreads / 32; ++i) {
+      tm = max(tm, sm.red[0][i]);
+      wm = max(wm, sm.red[1][i]);
+    }
+    const int et = scale_exp(tm);
     const float sc = exp2i(et);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split2(p[s][2 * j] * sc, p[s][2 * j + 1] * sc, hi[j], lo[j]);
+      for (int j = 0; j < 4; ++j) split2(tv[s][2 * j] * sc, tv[s][2 * j + 1] * sc, hi[j], lo[j]);
       const uint32_t at = swz<128>(s * 32 + (tid >> 3), tid & 7);
       *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       *reinterpret_cast<uint4*>(dst + kMat + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     if (tid == 0) {
       factors[kFEnd + 1] = exp2i(-et);
-      factors[kFEnd + 2] = exp2i(-ep);
-      factors[kFEnd + 3] = 0.f;
+      factors[kFEnd + 3] = __uint_as_float(wm) * 1.0001f;   // the sum's own rounding
     }
-    // the next head's A overwrites t only after the barriers before it
+    // the next head's factors overwrite this one's only after every thread has passed the barrier above,
+    // its A only after the next one
   }
 }
 
@@ -444,13 +473,14 @@ template <int DK>
 struct ChunkSmem {
   Stage<DK> stage[kStages];
   OutStage<DK> out_stage[kOutStages];
-  uint4 s_hi[2][2][2][DK / 32][32];   // [buffer][columns][half of dk][k tile][lane]
-  uint4 d_hi[2][2][2][2][32];         // [buffer][columns][half of the tokens][tile][lane]
-  float4 x[2][2][4][32];              // partial S^T k [columns][half][..][lane]
-  uint4 rx[2][2][2][2][32];           // R [columns][half][tile][hi, lo][lane]
-  uint4 dx[2][2][2][2][32];           // weighted d, likewise
+  uint4 s_hi[2][2][4][DK / 64][32];   // [buffer][columns][quarter of dk][k tile][lane]
+  uint4 d_hi[2][2][4][32];            // [buffer][columns][token block][lane]
+  float4 x[2][4][3][2][32];           // partial S^T k [columns][quarter][block - quarter - 1][tile][lane]
+  uint4 rx[2][4][2][32];              // R [columns][token block][hi, lo][lane]
+  uint4 dx[2][4][2][32];              // weighted d, likewise
   int bad[2][2][16];                  // [buffer][columns][column] first token whose R is not finite, or C
-  float s_inv[2][2][2], d_inv[2][2][2], r_inv[2][2], dx_inv[2][2];
+  float s_inv[2][2][4], d_inv[2][2][4], r_inv[2][4];
+  uint32_t r_max[2][4];
   uint64_t full[kStages], empty[kStages], out_full[kOutStages], out_empty[kOutStages];
   uint64_t s_full[2][2], d_full[2][2], out_done[2][2];   // [buffer][columns]
 };
@@ -466,20 +496,22 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-__device__ __forceinline__ void pair_sync(int id) {
+// The four warps of 16 columns.
+__device__ __forceinline__ void quad_sync(int id) {
   __syncwarp();
-  asm volatile("bar.sync %0, 64;" ::"r"(id + 1) : "memory");
+  asm volatile("bar.sync %0, 128;" ::"r"(id + 1) : "memory");
 }
 
-// Largest finite magnitude of a warp's values as float bits.
+// Largest finite magnitude of a warp's values as float bits.  Four chains of maxima: the recurrence's
+// warps run alone on their schedulers, so a chain's latency counts.
 template <int N>
 __device__ __forceinline__ uint32_t warp_max(const float (&v)[N][4]) {
-  float m = 0.f;
+  float m[4] = {};
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(v[i][j]));
-  uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
+  uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
   if (b >= 0x7f800000u) {   // an infinity somewhere: the other columns keep their own scale
     b = 0;
 #pragma unroll
@@ -489,6 +521,17 @@ __device__ __forceinline__ uint32_t warp_max(const float (&v)[N][4]) {
     b = __reduce_max_sync(0xffffffffu, b);
   }
   return b;
+}
+
+// The same with NaN counted: 0x7f800000 or more if any value is not finite.
+template <int N>
+__device__ __forceinline__ uint32_t warp_max_any(const float (&v)[N][4]) {
+  uint32_t m[4] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = max(m[j], __float_as_uint(v[i][j]) & 0x7fffffffu);
+  return __reduce_max_sync(0xffffffffu, max(max(m[0], m[1]), max(m[2], m[3])));
 }
 
 // Accumulators of two neighbouring 16 x 8 tiles as the hi and lo fragments of a 16 x 16 operand.
@@ -503,18 +546,18 @@ __device__ __forceinline__ void frag_split(const float (&a)[4], const float (&b)
 __device__ __forceinline__ uint4 as_uint4(const uint32_t (&r)[4]) { return make_uint4(r[0], r[1], r[2], r[3]); }
 __device__ __forceinline__ void from_uint4(uint32_t (&r)[4], uint4 v) { r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
 
-// Blocks of 16 tokens belong to the two warps of a pair so that their
-// triangular products take the same time: 0 and 3 to one, 1 and 2 to the other.
+// The output warps of 16 columns take blocks of 16 tokens so that their triangular products take
+// the same time: 0 and 3 to one, 1 and 2 to the other.
 __device__ __forceinline__ int block_of(int half, int i) { return half ? 1 + i : 3 * i; }
 
-// The values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
-__device__ __forceinline__ void spoil(float (&d)[4][4], int half, int bad0, int bad1, float v) {
+// A block's values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
+__device__ __forceinline__ void spoil(float* d, int block, int bad0, int bad1, float v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int tok = block_of(half, i >> 1) * 16 + (i & 1) * 8 + 2 * (threadIdx.x & 3);
+  for (int i = 0; i < 2; ++i) {
+    const int tok = block * 16 + i * 8 + 2 * (threadIdx.x & 3);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i][j] = v;
+      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i * 4 + j] = v;
   }
 }
 
@@ -531,15 +574,15 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.full[i], 33);
-      mbar_init(&sm.empty[i], 8);
+      mbar_init(&sm.empty[i], 12);
     }
     for (int i = 0; i < kOutStages; ++i) {
       mbar_init(&sm.out_full[i], 1);
       mbar_init(&sm.out_empty[i], 4);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&sm.s_full[0][0] + i, 2);
-      mbar_init(&sm.d_full[0][0] + i, 2);
+      mbar_init(&sm.s_full[0][0] + i, 4);
+      mbar_init(&sm.d_full[0][0] + i, 4);
       mbar_init(&sm.out_done[0][0] + i, 2);
     }
     fence_mbar_init();
@@ -555,10 +598,13 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
   const float* s_from = first > 0 ? a.s_out : a.s_in;
   const int64_t s_at = (seq * a.heads + h) * DK * static_cast<int64_t>(a.dv) + c0;
 
-  if (w < 4) {
-    // ---- the recurrence: columns grp * 16 .. + 15, a half of dk per warp
-    constexpr int NT = DK / 16, KT = DK / 32;
-    const int grp = w >> 1, half = w & 1, d0 = half * (DK / 2);
+  if (w < 8) {
+    // ---- the recurrence: columns grp * 16 .. + 15; a warp holds a quarter of dk of S and forms R and d of
+    // 16 tokens.  The two column groups share the schedulers and do not wait for each other, so one's sums
+    // and barriers run under the other's products; the quarters run the other way in the second group,
+    // since block 3 has four times block 0's products in T R.
+    constexpr int NT = DK / 32, KT = DK / 64;
+    const int grp = w >> 2, qd = grp ? 3 - (w & 3) : w & 3, d0 = qd * (DK / 4);
     const float* src = s_from ? s_from + s_at + grp * 16 + g : nullptr;
     float S[NT][4];   // S^T: rows are columns g and g + 8, columns are dk
 #pragma unroll
@@ -573,218 +619,210 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
 #pragma unroll
       for (int i = 0; i < NT; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = CUDART_NAN_F;
     }
+    float acc[8][4], inv = 1.f;   // this quarter's part of S^T k 2^e, blocks qd, qd + 1, .. (mod 4); 2^-e
+    uint32_t s_max = warp_max(S);
+    // S as f16 terms, scaled by 2^e, times the keys of chunk n; the hi terms go to the warps of the outputs too.
+    auto times_keys = [&](uint32_t n, int e) {
+      const uint32_t kb = smem_u32(sm.stage[n % kStages].k), bf = n & 1;
+      const float s = exp2i(e);
+      inv = exp2i(-e);
+      uint32_t hi[KT][4], lo[KT][4];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) frag_split(S[2 * kt], S[2 * kt + 1], s, hi[kt], lo[kt]);
+      wait(&sm.full[n % kStages], (n / kStages) & 1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t x[4][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          ldsm4(x[b], kb + swz<DK * 2>(((qd + b) & 3) * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                       d0 / 8 + kt * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          mma_16816(acc[2 * b], hi[kt], x[b][0], x[b][1]);
+          mma_16816(acc[2 * b + 1], hi[kt], x[b][2], x[b][3]);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          mma_16816(acc[2 * b], lo[kt], x[b][0], x[b][1]);
+          mma_16816(acc[2 * b + 1], lo[kt], x[b][2], x[b][3]);
+        }
+      }
+      if (n >= 2) wait(&sm.out_done[bf][grp], ((n >> 1) + 1) & 1);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) sm.s_hi[bf][grp][qd][kt][lane] = as_uint4(hi[kt]);
+      if (lane == 0) sm.s_inv[bf][grp][qd] = inv;
+      if (qd == 0 && lane < 16) sm.bad[bf][grp][lane] = C;
+      warp_arrive(&sm.s_full[bf][grp]);
+    };
+    if (first < last) times_keys(0, scale_exp(s_max));
     for (int64_t ci = first; ci < last; ++ci) {
       const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kStages, buf = it & 1;
       Stage<DK>& sg = sm.stage[st];
-      // S as f16 terms; the hi terms also go to the warps of the outputs
-      uint32_t hi[KT][4], lo[KT][4];
-      float inv;
-      {
-        const int e = scale_exp(warp_max(S));
-        const float s = exp2i(e);
-        inv = exp2i(-e);
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) frag_split(S[2 * kt], S[2 * kt + 1], s, hi[kt], lo[kt]);
-      }
-      if (it >= 2) wait(&sm.out_done[buf][grp], ((it >> 1) + 1) & 1);
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) sm.s_hi[buf][grp][half][kt][lane] = as_uint4(hi[kt]);
-      if (lane == 0) sm.s_inv[buf][grp][half] = inv;
-      if (half == 0 && lane < 16) sm.bad[buf][grp][lane] = C;
-      warp_arrive(&sm.s_full[buf][grp]);
-      wait(&sm.full[st], (it / kStages) & 1);
-      // this half's part of S^T k: token blocks in the order own, own, other, other
       const uint32_t kb = smem_u32(sg.k);
-      float acc[8][4] = {};
+      // the quarters' parts meet, each in the warp of its token block
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
+      for (int b = 1; b < 4; ++b)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int blk = block_of(b < 2 ? half : half ^ 1, b & 1);
-          uint32_t x[4];
-          ldsm4(x, kb + swz<DK * 2>(blk * 16 + (lane & 7) + ((lane >> 4) << 3), d0 / 8 + kt * 2 + ((lane >> 3) & 1)));
-          mma_16816(acc[2 * b], hi[kt], x[0], x[1]);
-          mma_16816(acc[2 * b + 1], hi[kt], x[2], x[3]);
-          mma_16816(acc[2 * b], lo[kt], x[0], x[1]);
-          mma_16816(acc[2 * b + 1], lo[kt], x[2], x[3]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sm.x[grp][half][i][lane] =
-            make_float4(acc[4 + i][0] * inv, acc[4 + i][1] * inv, acc[4 + i][2] * inv, acc[4 + i][3] * inv);
-      pair_sync(grp);
-      // R of the own blocks
-      float R[4][4];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int tb = block_of(half, b) * 16;
+        for (int j = 0; j < 2; ++j)
+          sm.x[grp][qd][b - 1][j][lane] = make_float4(acc[2 * b + j][0] * inv, acc[2 * b + j][1] * inv,
+                                                      acc[2 * b + j][2] * inv, acc[2 * b + j][3] * inv);
+      quad_sync(grp);
+      float R[2][4];
+      {
         uint32_t v[4];   // (columns 0-7 | 8-15) x (tokens 0-7), then tokens 8-15, transposed
-        ldsm4t(v, smem_u32(sg.v) + swz<64>(tb + (lane & 7) + ((lane >> 4) << 3), grp * 2 + ((lane >> 3) & 1)));
+        ldsm4t(v, smem_u32(sg.v) + swz<64>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), grp * 2 + ((lane >> 3) & 1)));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float4 o = sm.x[grp][half ^ 1][2 * b + j][lane];
-          const float2 fa = *reinterpret_cast<const float2*>(&sg.f[kFA + tb + j * 8 + 2 * t]);
-          const float2 fb = *reinterpret_cast<const float2*>(&sg.f[kFB + tb + j * 8 + 2 * t]);
-          const int i = 2 * b + j;
+          const float4 o1 = sm.x[grp][(qd + 1) & 3][2][j][lane];
+          const float4 o2 = sm.x[grp][(qd + 2) & 3][1][j][lane];
+          const float4 o3 = sm.x[grp][(qd + 3) & 3][0][j][lane];
+          const float2 fa = *reinterpret_cast<const float2*>(&sg.f[kFA + qd * 16 + j * 8 + 2 * t]);
+          const float2 fb = *reinterpret_cast<const float2*>(&sg.f[kFB + qd * 16 + j * 8 + 2 * t]);
           const uint32_t v0 = v[2 * j], v1 = v[2 * j + 1];
-          R[i][0] = fmaf(fa.x, fmaf(acc[i][0], inv, o.x), fb.x * __uint_as_float(v0 << 16));
-          R[i][1] = fmaf(fa.y, fmaf(acc[i][1], inv, o.y), fb.y * __uint_as_float(v0 & 0xffff0000u));
-          R[i][2] = fmaf(fa.x, fmaf(acc[i][2], inv, o.z), fb.x * __uint_as_float(v1 << 16));
-          R[i][3] = fmaf(fa.y, fmaf(acc[i][3], inv, o.w), fb.y * __uint_as_float(v1 & 0xffff0000u));
+          R[j][0] = fmaf(fa.x, fmaf(acc[j][0], inv, o1.x) + (o2.x + o3.x), fb.x * __uint_as_float(v0 << 16));
+          R[j][1] = fmaf(fa.y, fmaf(acc[j][1], inv, o1.y) + (o2.y + o3.y), fb.y * __uint_as_float(v0 & 0xffff0000u));
+          R[j][2] = fmaf(fa.x, fmaf(acc[j][2], inv, o1.z) + (o2.z + o3.z), fb.x * __uint_as_float(v1 << 16));
+          R[j][3] = fmaf(fa.y, fmaf(acc[j][3], inv, o1.w) + (o2.w + o3.w), fb.y * __uint_as_float(v1 & 0xffff0000u));
         }
       }
-      uint32_t rh[2][4], rl[2][4];
-      float r_inv;
       {
         // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros:
         // it is taken out here and put back into d from that token on.
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(R[i][j]) & 0x7fffffffu);
-        m = __reduce_max_sync(0xffffffffu, m);
+        uint32_t m = warp_max_any(R);
         if (m >= 0x7f800000u) {
-          m = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 4; ++j)
               if ((__float_as_uint(R[i][j]) & 0x7fffffffu) >= 0x7f800000u) {
-                atomicMin(&sm.bad[buf][grp][g + (j >> 1) * 8], block_of(half, i >> 1) * 16 + (i & 1) * 8 + 2 * t + (j & 1));
+                atomicMin(&sm.bad[buf][grp][g + (j >> 1) * 8], qd * 16 + i * 8 + 2 * t + (j & 1));
                 R[i][j] = 0.f;
               }
-              m = max(m, __float_as_uint(R[i][j]) & 0x7fffffffu);
-            }
-          m = __reduce_max_sync(0xffffffffu, m);
+          m = warp_max_any(R);
         }
         const int e = scale_exp(m);
-        const float s = exp2i(e);
-        r_inv = exp2i(-e);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          frag_split(R[2 * b], R[2 * b + 1], s, rh[b], rl[b]);
-          sm.rx[grp][half][b][0][lane] = as_uint4(rh[b]);
-          sm.rx[grp][half][b][1][lane] = as_uint4(rl[b]);
-        }
-        if (lane == 0) sm.r_inv[grp][half] = r_inv;
-      }
-      pair_sync(grp);
-      // d = T R of the own blocks
-      float own[4][4] = {}, oth[4][4] = {};
-      const uint32_t th = smem_u32(sg.t_hi), tl = smem_u32(sg.t_lo);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {   // source block: own, own, other, other
-        const int bj = block_of(s < 2 ? half : half ^ 1, s & 1);
-        uint32_t xh[4], xl[4];
-        if (s < 2) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { xh[i] = rh[s & 1][i]; xl[i] = rl[s & 1][i]; }
-        } else {
-          from_uint4(xh, sm.rx[grp][half ^ 1][s & 1][0][lane]);
-          from_uint4(xl, sm.rx[grp][half ^ 1][s & 1][1][lane]);
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int bi = block_of(half, b);
-          if (bj > bi) continue;
-          uint32_t yh[4], yl[4];
-          const uint32_t at = swz<128>(bi * 16 + (lane & 7) + ((lane >> 4) << 3), bj * 2 + ((lane >> 3) & 1));
-          ldsm4(yh, th + at);
-          ldsm4(yl, tl + at);
-          float(*d)[4] = s < 2 ? own : oth;
-          mma_16816(d[2 * b], xh, yh[0], yh[1]);
-          mma_16816(d[2 * b + 1], xh, yh[2], yh[3]);
-          mma_16816(d[2 * b], xl, yh[0], yh[1]);
-          mma_16816(d[2 * b + 1], xl, yh[2], yh[3]);
-          mma_16816(d[2 * b], xh, yl[0], yl[1]);
-          mma_16816(d[2 * b + 1], xh, yl[2], yl[3]);
+        uint32_t rh[4], rl[4];
+        frag_split(R[0], R[1], exp2i(e), rh, rl);
+        sm.rx[grp][qd][0][lane] = as_uint4(rh);
+        sm.rx[grp][qd][1][lane] = as_uint4(rl);
+        if (lane == 0) {
+          sm.r_inv[grp][qd] = exp2i(-e);
+          sm.r_max[grp][qd] = m;
         }
       }
+      quad_sync(grp);
+      // d = T R of this block; a source block's R has its own scale
+      float d[2][4], d_scale, d_inv;
       {
-        const float t_inv = sg.f[kFEnd + 1];
-        const float so = r_inv * t_inv, sx = sm.r_inv[grp][half ^ 1] * t_inv;
+        float p[4][2][4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) {
+          if (j > qd) continue;
+          uint32_t xh[4], xl[4], yh[4], yl[4];
+          const uint32_t at = swz<128>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), j * 2 + ((lane >> 3) & 1));
+          ldsm4(yh, smem_u32(sg.t_hi) + at);
+          ldsm4(yl, smem_u32(sg.t_lo) + at);
+          from_uint4(xh, sm.rx[grp][j][0][lane]);
+          from_uint4(xl, sm.rx[grp][j][1][lane]);
+          mma_16816(p[j][0], xh, yh[0], yh[1]);
+          mma_16816(p[j][1], xh, yh[2], yh[3]);
+          mma_16816(p[j][0], xl, yh[0], yh[1]);
+          mma_16816(p[j][1], xl, yh[2], yh[3]);
+          mma_16816(p[j][0], xh, yl[0], yl[1]);
+          mma_16816(p[j][1], xh, yl[2], yl[3]);
+        }
+        const float4 ri = *reinterpret_cast<const float4*>(sm.r_inv[grp]);
+        const uint4 rm = *reinterpret_cast<const uint4*>(sm.r_max[grp]);
+        const float4 fe = *reinterpret_cast<const float4*>(&sg.f[kFEnd]);
+        // weighted d is at most R's largest times the bound dn_prep_kernel left
+        const float bound = __uint_as_float(max(max(rm.x, rm.y), max(rm.z, rm.w))) * fe.w;
+        const int e = bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
+        d_scale = exp2i(e);
+        d_inv = bound > 0.f ? exp2i(-e) : 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) own[i][j] = fmaf(oth[i][j], sx, own[i][j] * so);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            d[i][j] = fmaf(p[0][i][j], ri.x, fmaf(p[1][i][j], ri.y, fmaf(p[2][i][j], ri.z, p[3][i][j] * ri.w))) * fe.y;
       }
       const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
       const bool any_bad = __any_sync(0xffffffffu, bad0 < C || bad1 < C);
-      if (any_bad) spoil(own, half, bad0, bad1, 0.f);
-      // d in f16 for the outputs, weighted and in two terms for the state
+      uint32_t wh[4], wl[4];
       {
-        const int e = scale_exp(warp_max(own));
-        const float s = exp2i(e);
+        float dw[2][4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float(&p)[4] = own[2 * b];
-          const float(&q)[4] = own[2 * b + 1];
-          sm.d_hi[buf][grp][half][b][lane] = make_uint4(pack_h2(p[0] * s, p[1] * s), pack_h2(p[2] * s, p[3] * s),
-                                                        pack_h2(q[0] * s, q[1] * s), pack_h2(q[2] * s, q[3] * s));
+        for (int i = 0; i < 2; ++i) {
+          const float2 fw = *reinterpret_cast<const float2*>(&sg.f[kFW + qd * 16 + i * 8 + 2 * t]);
+          dw[i][0] = d[i][0] * fw.x;
+          dw[i][1] = d[i][1] * fw.y;
+          dw[i][2] = d[i][2] * fw.x;
+          dw[i][3] = d[i][3] * fw.y;
         }
-        if (lane == 0) sm.d_inv[buf][grp][half] = exp2i(-e);
+        if (any_bad) {
+          spoil(&d[0][0], qd, bad0, bad1, 0.f);
+          spoil(&dw[0][0], qd, bad0, bad1, CUDART_NAN_F);
+        }
+        frag_split(dw[0], dw[1], d_scale, wh, wl);
+        sm.dx[grp][qd][0][lane] = as_uint4(wh);
+        sm.dx[grp][qd][1][lane] = as_uint4(wl);
       }
-      warp_arrive(&sm.d_full[buf][grp]);
-      if (any_bad) spoil(own, half, bad0, bad1, CUDART_NAN_F);
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float2 fw = *reinterpret_cast<const float2*>(&sg.f[kFW + block_of(half, b) * 16 + j * 8 + 2 * t]);
-          own[2 * b + j][0] *= fw.x;
-          own[2 * b + j][1] *= fw.y;
-          own[2 * b + j][2] *= fw.x;
-          own[2 * b + j][3] *= fw.y;
-        }
-      float d_inv;
-      {
-        const int e = scale_exp(warp_max(own));
-        const float s = exp2i(e);
-        d_inv = exp2i(-e);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          frag_split(own[2 * b], own[2 * b + 1], s, rh[b], rl[b]);
-          sm.dx[grp][half][b][0][lane] = as_uint4(rh[b]);
-          sm.dx[grp][half][b][1][lane] = as_uint4(rl[b]);
-        }
-        if (lane == 0) sm.dx_inv[grp][half] = d_inv;
-      }
-      pair_sync(grp);
-      // S = e^G64 S + d k^T for this half of dk
+      quad_sync(grp);
+      // S = e^G64 S + d k^T for this quarter of dk
       const float eg = sg.f[kFEnd];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {   // the own tokens, then the other warp's
+      {
         float u[NT][4] = {};
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int blk = block_of(s ? half ^ 1 : half, b);
-          uint32_t xh[4], xl[4];
-          if (s == 0) {
+        for (int b = 0; b < 4; ++b) {
+          const int blk = (qd + b) & 3;
+          uint32_t xh[4], xl[4], y[NT / 2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { xh[i] = rh[b][i]; xl[i] = rl[b][i]; }
+          for (int np = 0; np < NT / 2; ++np)
+            ldsm4t(y[np], kb + swz<DK * 2>(blk * 16 + (lane & 15), d0 / 8 + np * 2 + (lane >> 4)));
+          if (b == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { xh[i] = wh[i]; xl[i] = wl[i]; }
           } else {
-            from_uint4(xh, sm.dx[grp][half ^ 1][b][0][lane]);
-            from_uint4(xl, sm.dx[grp][half ^ 1][b][1][lane]);
+            from_uint4(xh, sm.dx[grp][blk][0][lane]);
+            from_uint4(xl, sm.dx[grp][blk][1][lane]);
           }
 #pragma unroll
           for (int np = 0; np < NT / 2; ++np) {
-            uint32_t y[4];
-            ldsm4t(y, kb + swz<DK * 2>(blk * 16 + (lane & 15), d0 / 8 + np * 2 + (lane >> 4)));
-            mma_16816(u[2 * np], xh, y[0], y[1]);
-            mma_16816(u[2 * np + 1], xh, y[2], y[3]);
-            mma_16816(u[2 * np], xl, y[0], y[1]);
-            mma_16816(u[2 * np + 1], xl, y[2], y[3]);
+            mma_16816(u[2 * np], xh, y[np][0], y[np][1]);
+            mma_16816(u[2 * np + 1], xh, y[np][2], y[np][3]);
+          }
+#pragma unroll
+          for (int np = 0; np < NT / 2; ++np) {
+            mma_16816(u[2 * np], xl, y[np][0], y[np][1]);
+            mma_16816(u[2 * np + 1], xl, y[np][2], y[np][3]);
           }
         }
-        const float us = s ? sm.dx_inv[grp][half ^ 1] : d_inv;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) S[i][j] = fmaf(u[i][j], us, s ? S[i][j] : S[i][j] * eg);
+          for (int j = 0; j < 4; ++j) S[i][j] = fmaf(u[i][j], d_inv, S[i][j] * eg);
       }
-      warp_arrive(&sm.empty[st]);
+      if (ci + 1 < last) {
+        // S's next scale comes from a bound: 64 products of d and k, both below 2^15 as f16
+        const float bound = fmaf(__uint_as_float(s_max), eg, d_inv * 0x1p36f);
+        times_keys(it + 1, bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112);
+      }
+      // d in f16 for the outputs of this chunk
+      {
+        const int e = scale_exp(warp_max(d));
+        const float s = exp2i(e);
+        sm.d_hi[buf][grp][qd][lane] = make_uint4(pack_h2(d[0][0] * s, d[0][1] * s), pack_h2(d[0][2] * s, d[0][3] * s),
+                                                 pack_h2(d[1][0] * s, d[1][1] * s), pack_h2(d[1][2] * s, d[1][3] * s));
+        if (lane == 0) sm.d_inv[buf][grp][qd] = exp2i(-e);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sm.d_full[buf][grp]);
+        mbar_arrive(&sm.empty[st]);
+      }
+      s_max = warp_max(S);
     }
     float* dst = a.s_out + s_at + grp * 16 + g;
 #pragma unroll
@@ -795,10 +833,10 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
       dst[r + 8] = S[i][2];
       dst[r + a.dv + 8] = S[i][3];
     }
-  } else if (w < 8) {
+  } else if (w < 12) {
     // ---- the outputs: columns grp * 16 .. + 15, half of the token blocks per warp
-    constexpr int KT = DK / 32;
-    const int grp = (w - 4) >> 1, half = w & 1;
+    constexpr int KT = DK / 64;
+    const int grp = (w - 8) >> 1, half = w & 1;
     for (int64_t ci = first; ci < last; ++ci) {
       const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kStages, so = it % kOutStages, buf = it & 1;
       Stage<DK>& sg = sm.stage[st];
@@ -811,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
       wait(&sm.s_full[buf][grp], (it >> 1) & 1);
       const uint32_t qb = smem_u32(og.q), pb = smem_u32(og.p);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {   // halves of dk: each has its own scale
+      for (int hf = 0; hf < 4; ++hf) {   // quarters of dk: each has its own scale
         float acc[4][4] = {};
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
@@ -821,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
           for (int b = 0; b < 2; ++b) {
             uint32_t y[4];
             ldsm4(y, qb + swz<DK * 2>(block_of(half, b) * 16 + (lane & 7) + ((lane >> 4) << 3),
-                                      hf * (DK / 16) + kt * 2 + ((lane >> 3) & 1)));
+                                      hf * (DK / 32) + kt * 2 + ((lane >> 3) & 1)));
             mma_16816(acc[2 * b], x, y[0], y[1]);
             mma_16816(acc[2 * b + 1], x, y[2], y[3]);
           }
@@ -840,32 +878,31 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
       wait(&sm.d_full[buf][grp], (it >> 1) & 1);
       const float p_inv = sg.f[kFEnd + 2];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {   // the tokens of either warp of the recurrence
-        float acc[4][4] = {};
+      for (int bj = 0; bj < 4; ++bj) {   // source blocks: each has its own scale
+        const float s = sm.d_inv[buf][grp][bj] * p_inv;
+        uint32_t x[4];
+        from_uint4(x, sm.d_hi[buf][grp][bj][lane]);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int bj = block_of(hf, s);
-          uint32_t x[4];
-          from_uint4(x, sm.d_hi[buf][grp][hf][s][lane]);
+        for (int b = 0; b < 2; ++b) {
+          const int bi = block_of(half, b);
+          if (bj > bi) continue;
+          float acc[2][4] = {};
+          uint32_t y[4];
+          ldsm4(y, pb + swz<128>(bi * 16 + (lane & 7) + ((lane >> 4) << 3), bj * 2 + ((lane >> 3) & 1)));
+          mma_16816(acc[0], x, y[0], y[1]);
+          mma_16816(acc[1], x, y[2], y[3]);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int bi = block_of(half, b);
-            if (bj > bi) continue;
-            uint32_t y[4];
-            ldsm4(y, pb + swz<128>(bi * 16 + (lane & 7) + ((lane >> 4) << 3), bj * 2 + ((lane >> 3) & 1)));
-            mma_16816(acc[2 * b], x, y[0], y[1]);
-            mma_16816(acc[2 * b + 1], x, y[2], y[3]);
-          }
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[2 * b + i][j] = fmaf(acc[i][j], s, o[2 * b + i][j]);
         }
-        const float s = sm.d_inv[buf][grp][hf] * p_inv;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = fmaf(acc[i][j], s, o[i][j]);
       }
       {
         const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
-        if (__any_sync(0xffffffffu, bad0 < C || bad1 < C)) spoil(o, half, bad0, bad1, CUDART_NAN_F);
+        if (__any_sync(0xffffffffu, bad0 < C || bad1 < C)) {
+          spoil(&o[0][0], block_of(half, 0), bad0, bad1, CUDART_NAN_F);
+          spoil(&o[2][0], block_of(half, 1), bad0, bad1, CUDART_NAN_F);
+        }
       }
       __syncwarp();
       if (lane == 0) {
@@ -982,7 +1019,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
   auto even = [](const void* p, int64_t row, int64_t head, int64_t elems) {
     return aligned(p, 2 * elems) && row % elems == 0 && head % elems == 0;
   };
-  const bool kq_vec = even(a.q, a.q_row, a.q_head, 2) && even(a.k, a.k_row, a.k_head, 2);
+  const bool kq_vec = even(a.q, a.q_row, a.q_head, 8) && even(a.k, a.k_row, a.k_head, 8);
   const bool v_vec = even(a.v, a.v_row, a.v_head, 8);
   cudaError_t e = cudaFuncSetAttribute(dn_prep_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        sizeof(PrepSmem<DK>));
