@@ -10,14 +10,14 @@
 //
 // Two kernels.  dn_prep_kernel does everything that does not need the state,
 // a block per (chunk, key head): k and q as f16 rows, T, P and the decays of
-// each token.  dn_chunk_kernel then walks a sequence's chunks, a block per
-// (sequence, value head, 32 columns of S), with S in registers.
+// each token.  dn_walk_kernel then walks a sequence's chunks, a block per
+// (sequence, value head, 128 columns of S), its products on tcgen05.
 //
 // Precision.  S leaves as fp32, so its factors need more than f16's 11 bits:
 // every operand of an S or d product that is not exact is split into two f16
-// terms (22 bits) after a power-of-two scale taken from its largest element;
-// k and q rows are bf16 and exact in f16 after theirs.  The products that
-// only reach the bf16 output (P d and S^T q) take one term.
+// terms (22 bits) after a power-of-two scale of its column; k and q rows are
+// bf16 and exact in f16 after theirs.  The products that only reach the bf16
+// output (P d and S^T q) take one term.
 #include "deltanet_batch.cuh"
 #include "deltanet_chunk.cuh"
 
@@ -25,18 +25,18 @@ namespace qfn {
 namespace {
 
 constexpr int C = 64;            // tokens of a chunk
-constexpr int kCols = 32;        // state columns of a block
-constexpr int kStages = 3;       // chunks of what the recurrence reads
-constexpr int kOutStages = 2;    // chunks of what only the outputs read
+constexpr int kCols = 128;       // state columns of a block: the lanes of TMEM
+constexpr int kStages = 3;
 constexpr int kPrepThreads = 256;
-constexpr int kThreads = 13 * 32; // 8 warps of the recurrence, 4 of the outputs, 1 of the copies
+constexpr int kThreads = 14 * 32; // 8 warps of the recurrence, 4 of the outputs, the MMAs, the copies
 constexpr int kGS = 68;          // row pitch of the 64 x 64 fp32 matrices of dn_prep_kernel
 
 // Per chunk and value head: T hi, T lo (f16, 128-byte rows, swizzled), the
 // tokens' factors and the chunk's scales, then P (as T).
 constexpr int kMat = C * C * 2;
 enum { kFA = 0, kFB = C, kFQ = 2 * C, kFW = 3 * C, kFEnd = 4 * C };   // -beta e^G ck, beta, e^G cq, e^(G64 - G) ck
-constexpr int kFactors = 4 * C + 4;   // + e^G64, scale of T, scale of P, largest row sum of e^(G64 - G) ck |T|
+// + e^G64, scale of T, scale of P, largest row sums of e^(G64 - G) ck |T| and of |T|
+constexpr int kFactors = 4 * C + 8;
 constexpr int kRecBytes = 2 * kMat + kFactors * 4;
 constexpr int kHeadBytes = kRecBytes + kMat;
 
@@ -89,24 +89,14 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
+// Byte offset of 16-byte piece `ch` of row `row` in a matrix of 128-byte rows
+// in the 128-byte swizzle that tcgen05 reads.
+__device__ __forceinline__ uint32_t swz(int row, int ch) {
+  return static_cast<uint32_t>(row * 128 + ((ch ^ (row & 7)) << 4));
 }
 
-// Byte offset of 16-byte piece `ch` of row `row` in a matrix of ROW-byte rows
-// whose pieces are permuted so that eight rows' equal pieces lie in distinct banks.
-template <int ROW>
-__device__ __forceinline__ uint32_t swz(int row, int ch) {
-  return static_cast<uint32_t>(row * ROW + ((ROW == 64 ? ch ^ ((row >> 1) & 3) : ch ^ (row & 7)) << 4));
-}
+// A k or q tile: pieces of 64 elements of dk side by side, each [64 tokens][128 bytes], swizzled.
+__device__ __forceinline__ uint32_t tile_at(int row, int ch) { return (ch >> 3) * (C * 128) + swz(row, ch & 7); }
 
 // ------------------------------------------------------------------ what needs no state
 template <int DK>
@@ -122,7 +112,7 @@ struct PrepSmem {
   };
   float gk[C * kGS], gq[C * kGS];   // k_i . k_j, q_i . k_j of the scaled rows
   float g_hi[C], g_lo[C], ck[C], cq[C], beta[C], w[C];
-  uint32_t red[2][kPrepThreads / 32];
+  uint32_t red[3][kPrepThreads / 32];
   float p_scale;
 };
 
@@ -227,7 +217,7 @@ __device__ __forceinline__ void f16_row(const uint4 (&x)[DK / 64], unsigned char
   for (int i = 0; i < DK / 64; ++i) {
     const uint4 h = make_uint4(pack_h2(v[i * 8] * sc, v[i * 8 + 1] * sc), pack_h2(v[i * 8 + 2] * sc, v[i * 8 + 3] * sc),
                                pack_h2(v[i * 8 + 4] * sc, v[i * 8 + 5] * sc), pack_h2(v[i * 8 + 6] * sc, v[i * 8 + 7] * sc));
-    const uint32_t at = swz<DK * 2>(row, part * (DK / 64) + i);
+    const uint32_t at = tile_at(row, part * (DK / 64) + i);
     *reinterpret_cast<uint4*>(tile + at) = h;
     *reinterpret_cast<uint4*>(copy + at) = h;
   }
@@ -289,12 +279,12 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 #pragma unroll 2
     for (int kt = 0; kt < DK / 16; ++kt) {
       uint32_t x[4];
-      ldsm4(x, rows + swz<DK * 2>(m * 16 + (lane & 15), kt * 2 + (lane >> 4)));
+      ldsm4(x, rows + tile_at(m * 16 + (lane & 15), kt * 2 + (lane >> 4)));
 #pragma unroll
       for (int np = 0; np < 4; ++np) {
         if (np > m) continue;
         uint32_t b[4];
-        ldsm4(b, cols + swz<DK * 2>(np * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
+        ldsm4(b, cols + tile_at(np * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
         mma_16816(acc[2 * np], x, b[0], b[1]);
         mma_16816(acc[2 * np + 1], x, b[2], b[3]);
       }
@@ -394,7 +384,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         }
         *reinterpret_cast<float4*>(&sm.t[i * kGS + j0]) = make_float4(av[0], av[1], av[2], av[3]);
         *reinterpret_cast<float4*>(&sm.t[i * kGS + j0 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
-        *reinterpret_cast<uint4*>(dst + kRecBytes + swz<128>(i, w)) =
+        *reinterpret_cast<uint4*>(dst + kRecBytes + swz(i, w)) =
             make_uint4(pack_h2(pv[0], pv[1]), pack_h2(pv[2], pv[3]), pack_h2(pv[4], pv[5]), pack_h2(pv[6], pv[7]));
       }
     }
@@ -402,7 +392,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
     invert(sm);
     // T's scale, and a bound of the weighted d for the walk: the largest row sum of w |T| (eight lanes a row)
     float tv[2][8];
-    uint32_t tm = 0, wm = 0;
+    uint32_t tm = 0, wm = 0, top = 0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int i = s * 32 + (tid >> 3), jt = (tid & 7) * 8;
@@ -422,18 +412,22 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       wm = max(wm, finite_bits(sum * sm.w[i]));
+      top = max(top, finite_bits(sum));
     }
     tm = __reduce_max_sync(0xffffffffu, tm);
     wm = __reduce_max_sync(0xffffffffu, wm);
+    top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) {
       sm.red[0][w] = tm;
       sm.red[1][w] = wm;
+      sm.red[2][w] = top;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPrepThreads / 32; ++i) {
       tm = max(tm, sm.red[0][i]);
       wm = max(wm, sm.red[1][i]);
+      top = max(top, sm.red[2][i]);
     }
     const int et = scale_exp(tm);
     const float sc = exp2i(et);
@@ -442,13 +436,14 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) split2(tv[s][2 * j] * sc, tv[s][2 * j + 1] * sc, hi[j], lo[j]);
-      const uint32_t at = swz<128>(s * 32 + (tid >> 3), tid & 7);
+      const uint32_t at = swz(s * 32 + (tid >> 3), tid & 7);
       *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       *reinterpret_cast<uint4*>(dst + kMat + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     if (tid == 0) {
       factors[kFEnd + 1] = exp2i(-et);
       factors[kFEnd + 3] = __uint_as_float(wm) * 1.0001f;   // the sum's own rounding
+      factors[kFEnd + 4] = __uint_as_float(top) * 1.0001f;
     }
     // the next head's factors overwrite this one's only after every thread has passed the barrier above,
     // its A only after the next one
@@ -456,34 +451,38 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 }
 
 // ------------------------------------------------------------------ the walk over the chunks
+//
+// A lane of TMEM is a column of S, so every product is transposed: A holds S^T,
+// R^T or d^T as f16 terms in TMEM (K: dk or tokens), B the k, q, T or P tile
+// in shared memory (N: tokens or dk), and a thread's values are one column's:
+// scales are per column, and nothing of one column touches another's.  The
+// chain of a chunk is
+//   S k^T (MMA) -> R -> T R (MMA) -> d -> d k (MMA) -> S
+// with the outputs' products S q^T and d P^T issued behind them.
 template <int DK>
 struct Stage {
-  unsigned char k[C * DK * 2];
-  unsigned char t_hi[kMat], t_lo[kMat];
-  float f[kFactors];
+  unsigned char k[C * DK * 2], q[C * DK * 2];
+  unsigned char t_hi[kMat], t_lo[kMat], p[kMat];
   unsigned char v[C * kCols * 2];
 };
+
 template <int DK>
-struct OutStage {
-  unsigned char q[C * DK * 2], p[kMat];
+struct WalkSmem {
+  Stage<DK> stage[kStages];
+  float f[kStages][kFactors];
+  float s_max[2][kCols], r_max[2][kCols];        // [half of dk or of the tokens][column]
+  int r_bad[2][kCols];                           // first token whose R is not finite, or C
+  float o_s[2][kCols], o_d[2][kCols];            // [buffer][column] factors of S q^T and d P^T
+  int o_bad[2][kCols];
+  uint64_t full[kStages], empty[kStages];
+  uint64_t s_ready, r_ready, d_ready, ks_done, tr_done, u_done, o_done, o_free;
+  uint32_t tmem;
 };
 
-// Fragments travel as 16 bytes per lane.
-template <int DK>
-struct ChunkSmem {
-  Stage<DK> stage[kStages];
-  OutStage<DK> out_stage[kOutStages];
-  uint4 s_hi[2][2][4][DK / 64][32];   // [buffer][columns][quarter of dk][k tile][lane]
-  uint4 d_hi[2][2][4][32];            // [buffer][columns][token block][lane]
-  float4 x[2][4][3][2][32];           // partial S^T k [columns][quarter][block - quarter - 1][tile][lane]
-  uint4 rx[2][4][2][32];              // R [columns][token block][hi, lo][lane]
-  uint4 dx[2][4][2][32];              // weighted d, likewise
-  int bad[2][2][16];                  // [buffer][columns][column] first token whose R is not finite, or C
-  float s_inv[2][2][4], d_inv[2][2][4], r_inv[2][4];
-  uint32_t r_max[2][4];
-  uint64_t full[kStages], empty[kStages], out_full[kOutStages], out_empty[kOutStages];
-  uint64_t s_full[2][2], d_full[2][2], out_done[2][2];   // [buffer][columns]
-};
+// TMEM columns.  d's terms replace R's once T R is done; S k^T and T R lie in U's place,
+// both read before d k is written there.
+constexpr uint32_t kTShi = 0, kTSlo = 64, kTRhi = 128, kTRlo = 160, kTd = 192, kTU = 224, kTKS = 224, kTTR = 288,
+                   kTO1 = 352, kTO2 = 416, kTmemCols = 512;
 
 // The wait is bounded; a failure is recorded and the walk goes on with what is there.
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
@@ -496,463 +495,381 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// The four warps of 16 columns.
-__device__ __forceinline__ void quad_sync(int id) {
+__device__ __forceinline__ void columns_sync() {   // the 8 warps of the recurrence
   __syncwarp();
-  asm volatile("bar.sync %0, 128;" ::"r"(id + 1) : "memory");
+  asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
-// Largest finite magnitude of a warp's values as float bits.  Four chains of maxima: the recurrence's
-// warps run alone on their schedulers, so a chain's latency counts.
-template <int N>
-__device__ __forceinline__ uint32_t warp_max(const float (&v)[N][4]) {
-  float m[4] = {};
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
-  uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
-  if (b >= 0x7f800000u) {   // an infinity somewhere: the other columns keep their own scale
-    b = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b = max(b, finite_bits(v[i][j]));
-    b = __reduce_max_sync(0xffffffffu, b);
-  }
-  return b;
+// B operand whose N runs along the rows' bytes (k^T for d k): 64 elements of N per 128-byte row,
+// the next 64 C * 128 bytes on, the next 8 of K 1024 bytes on.
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(C * 128 >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+constexpr uint32_t kNMajorB = 1u << 16;
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-// The same with NaN counted: 0x7f800000 or more if any value is not finite.
-template <int N>
-__device__ __forceinline__ uint32_t warp_max_any(const float (&v)[N][4]) {
-  uint32_t m[4] = {};
+// Sixteen values of a column, scaled, as the f16 terms of 16 steps of K.
+__device__ __forceinline__ void store_terms(const float* v, float s, uint32_t hi_at, uint32_t lo_at) {
+  uint32_t hi[8], lo[8];
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m[j] = max(m[j], __float_as_uint(v[i][j]) & 0x7fffffffu);
-  return __reduce_max_sync(0xffffffffu, max(max(m[0], m[1]), max(m[2], m[3])));
+  for (int i = 0; i < 8; ++i) split2(v[2 * i] * s, v[2 * i + 1] * s, hi[i], lo[i]);
+  tmem_st_x8(hi_at, hi);
+  tmem_st_x8(lo_at, lo);
 }
 
-// Accumulators of two neighbouring 16 x 8 tiles as the hi and lo fragments of a 16 x 16 operand.
-__device__ __forceinline__ void frag_split(const float (&a)[4], const float (&b)[4], float s, uint32_t (&hi)[4],
-                                           uint32_t (&lo)[4]) {
-  split2(a[0] * s, a[1] * s, hi[0], lo[0]);
-  split2(a[2] * s, a[3] * s, hi[1], lo[1]);
-  split2(b[0] * s, b[1] * s, hi[2], lo[2]);
-  split2(b[2] * s, b[3] * s, hi[3], lo[3]);
-}
-
-__device__ __forceinline__ uint4 as_uint4(const uint32_t (&r)[4]) { return make_uint4(r[0], r[1], r[2], r[3]); }
-__device__ __forceinline__ void from_uint4(uint32_t (&r)[4], uint4 v) { r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
-
-// The output warps of 16 columns take blocks of 16 tokens so that their triangular products take
-// the same time: 0 and 3 to one, 1 and 2 to the other.
-__device__ __forceinline__ int block_of(int half, int i) { return half ? 1 + i : 3 * i; }
-
-// A block's values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
-__device__ __forceinline__ void spoil(float* d, int block, int bad0, int bad1, float v) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int tok = block * 16 + i * 8 + 2 * (threadIdx.x & 3);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i * 4 + j] = v;
-  }
+// Power-of-two scale for a bound; not finite: the smallest scale.
+__device__ __forceinline__ int bound_exp(float bound) {
+  return bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
 }
 
 template <int DK>
-__global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, const Plan plan, const Work work,
-                                                               int64_t slot0, int64_t slot1, bool vec) {
-  extern __shared__ __align__(1024) unsigned char raw[];
-  ChunkSmem<DK>& sm = *reinterpret_cast<ChunkSmem<DK>*>(raw);
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int cb = a.dv / kCols;
+__global__ void __launch_bounds__(kThreads, 1) dn_walk_kernel(const DnRows a, const Plan plan, const Work work,
+                                                              int64_t slot0, int64_t slot1, bool vec) {
+  extern __shared__ unsigned char raw[];
+  WalkSmem<DK>& sm = *reinterpret_cast<WalkSmem<DK>*>(raw + ((1024 - (smem_u32(raw) & 1023)) & 1023));
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int cb = (a.dv + kCols - 1) / kCols;
   const int c0 = static_cast<int>(blockIdx.x % cb) * kCols;
   const int h = static_cast<int>(blockIdx.x / cb % a.heads);
   const int64_t seq = blockIdx.x / cb / a.heads;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.full[i], 33);
-      mbar_init(&sm.empty[i], 12);
+      mbar_init(&sm.empty[i], 13);   // 8 + 4 warps, the last MMAs
     }
-    for (int i = 0; i < kOutStages; ++i) {
-      mbar_init(&sm.out_full[i], 1);
-      mbar_init(&sm.out_empty[i], 4);
-    }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&sm.s_full[0][0] + i, 4);
-      mbar_init(&sm.d_full[0][0] + i, 4);
-      mbar_init(&sm.out_done[0][0] + i, 2);
-    }
+    mbar_init(&sm.s_ready, 8);
+    mbar_init(&sm.r_ready, 8);
+    mbar_init(&sm.d_ready, 8);
+    mbar_init(&sm.ks_done, 1);
+    mbar_init(&sm.tr_done, 1);
+    mbar_init(&sm.u_done, 1);
+    mbar_init(&sm.o_done, 1);
+    mbar_init(&sm.o_free, 4);
     fence_mbar_init();
   }
   pdl_wait();
   const bool ok = !plan.cu || dn_plan_ok(plan.cu, plan.n_seqs, plan.tokens);
-  __syncthreads();
   // this launch's chunks of the sequence
   const int64_t begin = ok ? plan.begin(seq) : 0, base = ok ? plan.slot(seq) : slot0;
   const int64_t len = ok ? plan.end(seq) - begin : 0, chunks = (len + C - 1) / C;
   const int64_t first = max(slot0 - base, static_cast<int64_t>(0)), last = min(slot1 - base, chunks);
   if (base >= slot1 || (first > 0 && first >= last)) return;
+  const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
   const float* s_from = first > 0 ? a.s_out : a.s_in;
-  const int64_t s_at = (seq * a.heads + h) * DK * static_cast<int64_t>(a.dv) + c0;
+  if (w == 12) tmem_alloc(&sm.tmem, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = sm.tmem;
 
   if (w < 8) {
-    // ---- the recurrence: columns grp * 16 .. + 15; a warp holds a quarter of dk of S and forms R and d of
-    // 16 tokens.  The two column groups share the schedulers and do not wait for each other, so one's sums
-    // and barriers run under the other's products; the quarters run the other way in the second group,
-    // since block 3 has four times block 0's products in T R.
-    constexpr int NT = DK / 32, KT = DK / 64;
-    const int grp = w >> 2, qd = grp ? 3 - (w & 3) : w & 3, d0 = qd * (DK / 4);
-    const float* src = s_from ? s_from + s_at + grp * 16 + g : nullptr;
-    float S[NT][4];   // S^T: rows are columns g and g + 8, columns are dk
+    // ---- the recurrence: a thread has a column, half of dk and half of a chunk's tokens
+    constexpr int NS = DK / 2;
+    const int half = w >> 2, L = (w & 3) * 32 + lane, col = c0 + L;
+    const bool in = col < a.dv;
+    const uint32_t tl = tm + (static_cast<uint32_t>((w & 3) * 32) << 16);
+    const int64_t s_at = ((seq * a.heads + h) * DK + half * NS) * static_cast<int64_t>(a.dv) + col;
+    float S[NS], inv = 1.f, s_max = 0.f;   // S 2^e; 2^-e; the largest of this half
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int64_t r = static_cast<int64_t>(d0 + i * 8 + 2 * t) * a.dv;
-      S[i][0] = src ? src[r] : 0.f;
-      S[i][1] = src ? src[r + a.dv] : 0.f;
-      S[i][2] = src ? src[r + 8] : 0.f;
-      S[i][3] = src ? src[r + a.dv + 8] : 0.f;
+    for (int i = 0; i < NS; ++i) {
+      S[i] = in && s_from ? s_from[s_at + i * static_cast<int64_t>(a.dv)] : 0.f;
+      s_max = fmaxf(s_max, __uint_as_float(finite_bits(S[i])));
     }
     if (!ok) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = CUDART_NAN_F;
+      for (int i = 0; i < NS; ++i) S[i] = CUDART_NAN_F;
     }
-    float acc[8][4], inv = 1.f;   // this quarter's part of S^T k 2^e, blocks qd, qd + 1, .. (mod 4); 2^-e
-    uint32_t s_max = warp_max(S);
-    // S as f16 terms, scaled by 2^e, times the keys of chunk n; the hi terms go to the warps of the outputs too.
-    auto times_keys = [&](uint32_t n, int e) {
-      const uint32_t kb = smem_u32(sm.stage[n % kStages].k), bf = n & 1;
+    if (n > 0) {
+      sm.s_max[half][L] = s_max;
+      columns_sync();
+      const int e = scale_exp(__float_as_uint(fmaxf(s_max, sm.s_max[half ^ 1][L])));
       const float s = exp2i(e);
       inv = exp2i(-e);
-      uint32_t hi[KT][4], lo[KT][4];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) frag_split(S[2 * kt], S[2 * kt + 1], s, hi[kt], lo[kt]);
-      wait(&sm.full[n % kStages], (n / kStages) & 1);
+      for (int i = 0; i < NS; ++i) S[i] *= s;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+      for (int i = 0; i < NS; i += 16)
+        store_terms(&S[i], 1.f, tl + kTShi + (half * NS + i) / 2, tl + kTSlo + (half * NS + i) / 2);
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&sm.s_ready);
+    }
+    for (int it = 0; it < n; ++it) {
+      const uint32_t ph = it & 1, st = it % kStages;
+      const float* f = sm.f[st];
+      wait(&sm.full[st], (it / kStages) & 1);
+      // R = beta v - beta e^G S^T k of 32 tokens
+      float R[32];
+      {
+        uint32_t v[16];   // the column's values of v, two tokens a word
+        const uint16_t* vs = reinterpret_cast<const uint16_t*>(sm.stage[st].v) + half * 32 * kCols + L;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        uint32_t x[4][4];
+        for (int i = 0; i < 16; ++i) v[i] = vs[2 * i * kCols] | static_cast<uint32_t>(vs[(2 * i + 1) * kCols]) << 16;
+        wait(&sm.ks_done, ph);
+        tc_fence_after();
+        uint32_t ks[32];
+        tmem_ld_x32(tl + kTKS + half * 32, ks);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          ldsm4(x[b], kb + swz<DK * 2>(((qd + b) & 3) * 16 + (lane & 7) + ((lane >> 4) << 3),
-                                       d0 / 8 + kt * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          mma_16816(acc[2 * b], hi[kt], x[b][0], x[b][1]);
-          mma_16816(acc[2 * b + 1], hi[kt], x[b][2], x[b][3]);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          mma_16816(acc[2 * b], lo[kt], x[b][0], x[b][1]);
-          mma_16816(acc[2 * b + 1], lo[kt], x[b][2], x[b][3]);
+        for (int i = 0; i < 32; i += 4) {
+          const float4 fa = *reinterpret_cast<const float4*>(f + kFA + half * 32 + i);
+          const float4 fb = *reinterpret_cast<const float4*>(f + kFB + half * 32 + i);
+          R[i] = fmaf(fa.x, __uint_as_float(ks[i]) * inv, fb.x * __uint_as_float(v[i / 2] << 16));
+          R[i + 1] = fmaf(fa.y, __uint_as_float(ks[i + 1]) * inv, fb.y * __uint_as_float(v[i / 2] & 0xffff0000u));
+          R[i + 2] = fmaf(fa.z, __uint_as_float(ks[i + 2]) * inv, fb.z * __uint_as_float(v[i / 2 + 1] << 16));
+          R[i + 3] = fmaf(fa.w, __uint_as_float(ks[i + 3]) * inv, fb.w * __uint_as_float(v[i / 2 + 1] & 0xffff0000u));
         }
       }
-      if (n >= 2) wait(&sm.out_done[bf][grp], ((n >> 1) + 1) & 1);
+      float m4[4] = {};
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) sm.s_hi[bf][grp][qd][kt][lane] = as_uint4(hi[kt]);
-      if (lane == 0) sm.s_inv[bf][grp][qd] = inv;
-      if (qd == 0 && lane < 16) sm.bad[bf][grp][lane] = C;
-      warp_arrive(&sm.s_full[bf][grp]);
-    };
-    if (first < last) times_keys(0, scale_exp(s_max));
-    for (int64_t ci = first; ci < last; ++ci) {
-      const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kStages, buf = it & 1;
-      Stage<DK>& sg = sm.stage[st];
-      const uint32_t kb = smem_u32(sg.k);
-      // the quarters' parts meet, each in the warp of its token block
-#pragma unroll
-      for (int b = 1; b < 4; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          sm.x[grp][qd][b - 1][j][lane] = make_float4(acc[2 * b + j][0] * inv, acc[2 * b + j][1] * inv,
-                                                      acc[2 * b + j][2] * inv, acc[2 * b + j][3] * inv);
-      quad_sync(grp);
-      float R[2][4];
-      {
-        uint32_t v[4];   // (columns 0-7 | 8-15) x (tokens 0-7), then tokens 8-15, transposed
-        ldsm4t(v, smem_u32(sg.v) + swz<64>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), grp * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float4 o1 = sm.x[grp][(qd + 1) & 3][2][j][lane];
-          const float4 o2 = sm.x[grp][(qd + 2) & 3][1][j][lane];
-          const float4 o3 = sm.x[grp][(qd + 3) & 3][0][j][lane];
-          const float2 fa = *reinterpret_cast<const float2*>(&sg.f[kFA + qd * 16 + j * 8 + 2 * t]);
-          const float2 fb = *reinterpret_cast<const float2*>(&sg.f[kFB + qd * 16 + j * 8 + 2 * t]);
-          const uint32_t v0 = v[2 * j], v1 = v[2 * j + 1];
-          R[j][0] = fmaf(fa.x, fmaf(acc[j][0], inv, o1.x) + (o2.x + o3.x), fb.x * __uint_as_float(v0 << 16));
-          R[j][1] = fmaf(fa.y, fmaf(acc[j][1], inv, o1.y) + (o2.y + o3.y), fb.y * __uint_as_float(v0 & 0xffff0000u));
-          R[j][2] = fmaf(fa.x, fmaf(acc[j][2], inv, o1.z) + (o2.z + o3.z), fb.x * __uint_as_float(v1 << 16));
-          R[j][3] = fmaf(fa.y, fmaf(acc[j][3], inv, o1.w) + (o2.w + o3.w), fb.y * __uint_as_float(v1 & 0xffff0000u));
-        }
-      }
-      {
+      for (int i = 0; i < 32; ++i) m4[i & 3] = max_nan(m4[i & 3], fabsf(R[i]));
+      float m = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
+      int bad = C;
+      if (!(m < CUDART_INF_F)) {
         // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros:
         // it is taken out here and put back into d from that token on.
-        uint32_t m = warp_max_any(R);
-        if (m >= 0x7f800000u) {
+        m = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if ((__float_as_uint(R[i][j]) & 0x7fffffffu) >= 0x7f800000u) {
-                atomicMin(&sm.bad[buf][grp][g + (j >> 1) * 8], qd * 16 + i * 8 + 2 * t + (j & 1));
-                R[i][j] = 0.f;
-              }
-          m = warp_max_any(R);
-        }
-        const int e = scale_exp(m);
-        uint32_t rh[4], rl[4];
-        frag_split(R[0], R[1], exp2i(e), rh, rl);
-        sm.rx[grp][qd][0][lane] = as_uint4(rh);
-        sm.rx[grp][qd][1][lane] = as_uint4(rl);
-        if (lane == 0) {
-          sm.r_inv[grp][qd] = exp2i(-e);
-          sm.r_max[grp][qd] = m;
-        }
-      }
-      quad_sync(grp);
-      // d = T R of this block; a source block's R has its own scale
-      float d[2][4], d_scale, d_inv;
-      {
-        float p[4][2][4] = {};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j > qd) continue;
-          uint32_t xh[4], xl[4], yh[4], yl[4];
-          const uint32_t at = swz<128>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), j * 2 + ((lane >> 3) & 1));
-          ldsm4(yh, smem_u32(sg.t_hi) + at);
-          ldsm4(yl, smem_u32(sg.t_lo) + at);
-          from_uint4(xh, sm.rx[grp][j][0][lane]);
-          from_uint4(xl, sm.rx[grp][j][1][lane]);
-          mma_16816(p[j][0], xh, yh[0], yh[1]);
-          mma_16816(p[j][1], xh, yh[2], yh[3]);
-          mma_16816(p[j][0], xl, yh[0], yh[1]);
-          mma_16816(p[j][1], xl, yh[2], yh[3]);
-          mma_16816(p[j][0], xh, yl[0], yl[1]);
-          mma_16816(p[j][1], xh, yl[2], yl[3]);
-        }
-        const float4 ri = *reinterpret_cast<const float4*>(sm.r_inv[grp]);
-        const uint4 rm = *reinterpret_cast<const uint4*>(sm.r_max[grp]);
-        const float4 fe = *reinterpret_cast<const float4*>(&sg.f[kFEnd]);
-        // weighted d is at most R's largest times the bound dn_prep_kernel left
-        const float bound = __uint_as_float(max(max(rm.x, rm.y), max(rm.z, rm.w))) * fe.w;
-        const int e = bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
-        d_scale = exp2i(e);
-        d_inv = bound > 0.f ? exp2i(-e) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            d[i][j] = fmaf(p[0][i][j], ri.x, fmaf(p[1][i][j], ri.y, fmaf(p[2][i][j], ri.z, p[3][i][j] * ri.w))) * fe.y;
-      }
-      const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
-      const bool any_bad = __any_sync(0xffffffffu, bad0 < C || bad1 < C);
-      uint32_t wh[4], wl[4];
-      {
-        float dw[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 fw = *reinterpret_cast<const float2*>(&sg.f[kFW + qd * 16 + i * 8 + 2 * t]);
-          dw[i][0] = d[i][0] * fw.x;
-          dw[i][1] = d[i][1] * fw.y;
-          dw[i][2] = d[i][2] * fw.x;
-          dw[i][3] = d[i][3] * fw.y;
-        }
-        if (any_bad) {
-          spoil(&d[0][0], qd, bad0, bad1, 0.f);
-          spoil(&dw[0][0], qd, bad0, bad1, CUDART_NAN_F);
-        }
-        frag_split(dw[0], dw[1], d_scale, wh, wl);
-        sm.dx[grp][qd][0][lane] = as_uint4(wh);
-        sm.dx[grp][qd][1][lane] = as_uint4(wl);
-      }
-      quad_sync(grp);
-      // S = e^G64 S + d k^T for this quarter of dk
-      const float eg = sg.f[kFEnd];
-      {
-        float u[NT][4] = {};
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int blk = (qd + b) & 3;
-          uint32_t xh[4], xl[4], y[NT / 2][4];
-#pragma unroll
-          for (int np = 0; np < NT / 2; ++np)
-            ldsm4t(y[np], kb + swz<DK * 2>(blk * 16 + (lane & 15), d0 / 8 + np * 2 + (lane >> 4)));
-          if (b == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { xh[i] = wh[i]; xl[i] = wl[i]; }
-          } else {
-            from_uint4(xh, sm.dx[grp][blk][0][lane]);
-            from_uint4(xl, sm.dx[grp][blk][1][lane]);
+        for (int i = 31; i >= 0; --i) {
+          if (!(fabsf(R[i]) < CUDART_INF_F)) {
+            bad = half * 32 + i;
+            R[i] = 0.f;
           }
-#pragma unroll
-          for (int np = 0; np < NT / 2; ++np) {
-            mma_16816(u[2 * np], xh, y[np][0], y[np][1]);
-            mma_16816(u[2 * np + 1], xh, y[np][2], y[np][3]);
-          }
-#pragma unroll
-          for (int np = 0; np < NT / 2; ++np) {
-            mma_16816(u[2 * np], xl, y[np][0], y[np][1]);
-            mma_16816(u[2 * np + 1], xl, y[np][2], y[np][3]);
-          }
+          m = fmaxf(m, fabsf(R[i]));
         }
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) S[i][j] = fmaf(u[i][j], d_inv, S[i][j] * eg);
       }
-      if (ci + 1 < last) {
-        // S's next scale comes from a bound: 64 products of d and k, both below 2^15 as f16
-        const float bound = fmaf(__uint_as_float(s_max), eg, d_inv * 0x1p36f);
-        times_keys(it + 1, bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112);
-      }
-      // d in f16 for the outputs of this chunk
+      sm.r_max[half][L] = m;
+      sm.r_bad[half][L] = bad;
+      sm.s_max[half][L] = s_max;
+      columns_sync();
+      m = fmaxf(m, sm.r_max[half ^ 1][L]);
+      bad = min(bad, sm.r_bad[half ^ 1][L]);
+      const float s_all = fmaxf(s_max, sm.s_max[half ^ 1][L]);
+      const int re = scale_exp(__float_as_uint(m));
       {
-        const int e = scale_exp(warp_max(d));
-        const float s = exp2i(e);
-        sm.d_hi[buf][grp][qd][lane] = make_uint4(pack_h2(d[0][0] * s, d[0][1] * s), pack_h2(d[0][2] * s, d[0][3] * s),
-                                                 pack_h2(d[1][0] * s, d[1][1] * s), pack_h2(d[1][2] * s, d[1][3] * s));
-        if (lane == 0) sm.d_inv[buf][grp][qd] = exp2i(-e);
+        const float s = exp2i(re);
+#pragma unroll
+        for (int i = 0; i < 32; i += 16)
+          store_terms(&R[i], s, tl + kTRhi + half * 16 + i / 2, tl + kTRlo + half * 16 + i / 2);
       }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&sm.r_ready);
+      // d = T R.  Its scales come from bounds: R's largest times T's row sums, weighted and not.
+      const float4 fe = *reinterpret_cast<const float4*>(f + kFEnd);
+      const float w_bound = m * fe.w;
+      const int we = bound_exp(w_bound), de = bound_exp(m * f[kFEnd + 4]);
+      const float d_inv = w_bound > 0.f ? exp2i(-we) : 0.f;
+      {
+        const float c1 = exp2i(-re) * fe.y, c16 = c1 * exp2i(de), ws = exp2i(we);
+        wait(&sm.tr_done, ph);
+        tc_fence_after();
+        uint32_t d[32];
+        tmem_ld_x32(tl + kTTR + half * 32, d);
+#pragma unroll
+        for (int i = 0; i < 32; i += 16) {
+          uint32_t o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float x = __uint_as_float(d[i + 2 * j]) * c16, y = __uint_as_float(d[i + 2 * j + 1]) * c16;
+            if (half * 32 + i + 2 * j >= bad) x = 0.f;
+            if (half * 32 + i + 2 * j + 1 >= bad) y = 0.f;
+            o[j] = pack_h2(x, y);
+          }
+          tmem_st_x8(tl + kTd + half * 16 + i / 2, o);
+        }
+        const float cw = c1 * ws;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 fw = *reinterpret_cast<const float4*>(f + kFW + half * 32 + i);
+          R[i] = __uint_as_float(d[i]) * cw * fw.x;
+          R[i + 1] = __uint_as_float(d[i + 1]) * cw * fw.y;
+          R[i + 2] = __uint_as_float(d[i + 2]) * cw * fw.z;
+          R[i + 3] = __uint_as_float(d[i + 3]) * cw * fw.w;
+        }
+        if (bad < C) R[0] = CUDART_NAN_F;   // the state's column is lost with it
+#pragma unroll
+        for (int i = 0; i < 32; i += 16)
+          store_terms(&R[i], 1.f, tl + kTRhi + half * 16 + i / 2, tl + kTRlo + half * 16 + i / 2);
+      }
+      if (half == 0) {
+        sm.o_s[ph][L] = inv;
+        sm.o_d[ph][L] = exp2i(-de) * fe.z;
+        sm.o_bad[ph][L] = bad;
+      }
+      tmem_st_wait();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&sm.d_full[buf][grp]);
+        mbar_arrive(&sm.d_ready);
         mbar_arrive(&sm.empty[st]);
       }
-      s_max = warp_max(S);
-    }
-    float* dst = a.s_out + s_at + grp * 16 + g;
+      // S = e^G64 S + d k.  Its scale comes from a bound: 64 products of d and k, both below 2^15 as f16.
+      const int e = bound_exp(fmaf(s_all, fe.x, d_inv * 0x1p36f));
+      const float s = exp2i(e), keep = fe.x * inv * s, gain = d_inv * s;
+      inv = exp2i(-e);
+      wait(&sm.u_done, ph);
+      tc_fence_after();
+      float sm4[4] = {};
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int64_t r = static_cast<int64_t>(d0 + i * 8 + 2 * t) * a.dv;
-      dst[r] = S[i][0];
-      dst[r + a.dv] = S[i][1];
-      dst[r + 8] = S[i][2];
-      dst[r + a.dv + 8] = S[i][3];
+      for (int i = 0; i < NS; i += 16) {
+        uint32_t u[16];
+        tmem_ld_x16(tl + kTU + half * NS + i, u);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          S[i + j] = fmaf(__uint_as_float(u[j]), gain, S[i + j] * keep);
+          sm4[j & 3] = fmaxf(sm4[j & 3], fabsf(S[i + j]));
+        }
+        store_terms(&S[i], 1.f, tl + kTShi + (half * NS + i) / 2, tl + kTSlo + (half * NS + i) / 2);
+      }
+      s_max = fmaxf(fmaxf(sm4[0], sm4[1]), fmaxf(sm4[2], sm4[3])) * inv;
+      if (!(s_max < CUDART_INF_F)) s_max = 0.f;   // the column is lost; its scale no longer matters
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&sm.s_ready);
+    }
+    if (in) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) a.s_out[s_at + i * static_cast<int64_t>(a.dv)] = S[i] * inv;
     }
   } else if (w < 12) {
-    // ---- the outputs: columns grp * 16 .. + 15, half of the token blocks per warp
-    constexpr int KT = DK / 64;
-    const int grp = (w - 8) >> 1, half = w & 1;
-    for (int64_t ci = first; ci < last; ++ci) {
-      const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kStages, so = it % kOutStages, buf = it & 1;
-      Stage<DK>& sg = sm.stage[st];
-      OutStage<DK>& og = sm.out_stage[so];
-      const int64_t t0 = begin + ci * C;
+    // ---- the outputs: a thread has a column
+    const int L = (w & 3) * 32 + lane, col = c0 + L;
+    const uint32_t tl = tm + (static_cast<uint32_t>((w & 3) * 32) << 16);
+    for (int it = 0; it < n; ++it) {
+      const uint32_t ph = it & 1, st = it % kStages;
+      const float* f = sm.f[st];
+      const int64_t t0 = begin + (first + it) * C;
       const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
-      float o[4][4];
       wait(&sm.full[st], (it / kStages) & 1);
-      wait(&sm.out_full[so], (it / kOutStages) & 1);
-      wait(&sm.s_full[buf][grp], (it >> 1) & 1);
-      const uint32_t qb = smem_u32(og.q), pb = smem_u32(og.p);
+      wait(&sm.d_ready, ph);   // for o_s, o_d and o_bad
+      wait(&sm.o_done, ph);
+      tc_fence_after();
+      const float os = sm.o_s[ph][L], od = sm.o_d[ph][L];
+      const int bad = sm.o_bad[ph][L];
+      uint16_t* dst = a.out + (t0 * a.heads + h) * a.dv + col;
 #pragma unroll
-      for (int hf = 0; hf < 4; ++hf) {   // quarters of dk: each has its own scale
-        float acc[4][4] = {};
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t x[32], y[32];
+        tmem_ld_x32(tl + kTO1 + hf * 32, x);
+        tmem_ld_x32(tl + kTO2 + hf * 32, y);
+        if (hf) {
+          tc_fence_before();
+          warp_arrive(&sm.o_free);
+        }
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          uint32_t x[4];
-          from_uint4(x, sm.s_hi[buf][grp][hf][kt][lane]);
+        for (int i = 0; i < 32; i += 4) {
+          const float4 fq = *reinterpret_cast<const float4*>(f + kFQ + hf * 32 + i);
+          const float q4[4] = {fq.x, fq.y, fq.z, fq.w};
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            uint32_t y[4];
-            ldsm4(y, qb + swz<DK * 2>(block_of(half, b) * 16 + (lane & 7) + ((lane >> 4) << 3),
-                                      hf * (DK / 32) + kt * 2 + ((lane >> 3) & 1)));
-            mma_16816(acc[2 * b], x, y[0], y[1]);
-            mma_16816(acc[2 * b + 1], x, y[2], y[3]);
+          for (int j = 0; j < 4; ++j) {
+            const int tok = hf * 32 + i + j;
+            float o = fmaf(__uint_as_float(y[i + j]), od, __uint_as_float(x[i + j]) * os * q4[j]);
+            if (tok >= bad) o = CUDART_NAN_F;
+            if (tok < cnt && col < a.dv) dst[static_cast<int64_t>(tok) * a.heads * a.dv] = dn_bf16_bits(o);
           }
         }
-        const float s = sm.s_inv[buf][grp][hf];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = hf ? fmaf(acc[i][j], s, o[i][j]) : acc[i][j] * s;
       }
+      warp_arrive(&sm.empty[st]);
+    }
+  } else if (w == 12) {
+    // ---- the MMAs
+    constexpr uint32_t id = idesc_f16(128, C), id_u = idesc_f16(128, DK) | kNMajorB;
+    const uint32_t issue = elect_one();
+    auto tile = [](uint32_t addr, int kt) { return umma_desc_sw128(addr + (kt >> 2) * (C * 128) + (kt & 3) * 32, 1024); };
+    for (int it = 0; it < n; ++it) {
+      const uint32_t ph = it & 1, st = it % kStages;
+      const Stage<DK>& sg = sm.stage[st];
+      const uint32_t k = smem_u32(sg.k), q = smem_u32(sg.q), th = smem_u32(sg.t_hi), tlo = smem_u32(sg.t_lo),
+                     p = smem_u32(sg.p);
+      wait(&sm.full[st], (it / kStages) & 1);
+      wait(&sm.s_ready, ph);
+      tc_fence_after();
+      if (issue) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = *reinterpret_cast<const float2*>(&sg.f[kFQ + block_of(half, i >> 1) * 16 + (i & 1) * 8 + 2 * t]);
-        o[i][0] *= f.x; o[i][1] *= f.y; o[i][2] *= f.x; o[i][3] *= f.y;
-      }
-      wait(&sm.d_full[buf][grp], (it >> 1) & 1);
-      const float p_inv = sg.f[kFEnd + 2];
-#pragma unroll
-      for (int bj = 0; bj < 4; ++bj) {   // source blocks: each has its own scale
-        const float s = sm.d_inv[buf][grp][bj] * p_inv;
-        uint32_t x[4];
-        from_uint4(x, sm.d_hi[buf][grp][bj][lane]);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int bi = block_of(half, b);
-          if (bj > bi) continue;
-          float acc[2][4] = {};
-          uint32_t y[4];
-          ldsm4(y, pb + swz<128>(bi * 16 + (lane & 7) + ((lane >> 4) << 3), bj * 2 + ((lane >> 3) & 1)));
-          mma_16816(acc[0], x, y[0], y[1]);
-          mma_16816(acc[1], x, y[2], y[3]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[2 * b + i][j] = fmaf(acc[i][j], s, o[2 * b + i][j]);
+        for (int kt = 0; kt < DK / 16; ++kt) {
+          mma_f16_ta(tm + kTKS, tm + kTShi + kt * 8, tile(k, kt), id, kt > 0);
+          mma_f16_ta(tm + kTKS, tm + kTSlo + kt * 8, tile(k, kt), id, true);
         }
-      }
-      {
-        const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
-        if (__any_sync(0xffffffffu, bad0 < C || bad1 < C)) {
-          spoil(&o[0][0], block_of(half, 0), bad0, bad1, CUDART_NAN_F);
-          spoil(&o[2][0], block_of(half, 1), bad0, bad1, CUDART_NAN_F);
-        }
+        mma_commit(&sm.ks_done);
       }
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.out_done[buf][grp]);
-        mbar_arrive(&sm.empty[st]);
-        mbar_arrive(&sm.out_empty[so]);
+      if (it > 0) wait(&sm.o_free, ph ^ 1);
+      tc_fence_after();
+      if (issue) {
+#pragma unroll
+        for (int kt = 0; kt < DK / 16; ++kt) mma_f16_ta(tm + kTO1, tm + kTShi + kt * 8, tile(q, kt), id, kt > 0);
       }
+      __syncwarp();
+      wait(&sm.r_ready, ph);
+      tc_fence_after();
+      if (issue) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = block_of(half, i >> 1) * 16 + (i & 1) * 8 + g;   // after the transposition a row is a token
-        uint16_t* dst = a.out + ((t0 + tok) * a.heads + h) * a.dv + c0 + grp * 16 + 2 * t;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const __nv_bfloat162 b2 = __floats2bfloat162_rn(o[i][2 * r], o[i][2 * r + 1]);
-          const uint32_t y = transpose8x8(*reinterpret_cast<const uint32_t*>(&b2));
-          if (tok < cnt) *reinterpret_cast<uint32_t*>(dst + 8 * r) = y;
+        for (int kt = 0; kt < 4; ++kt) {
+          mma_f16_ta(tm + kTTR, tm + kTRhi + kt * 8, tile(th, kt), id, kt > 0);
+          mma_f16_ta(tm + kTTR, tm + kTRlo + kt * 8, tile(th, kt), id, true);
+          mma_f16_ta(tm + kTTR, tm + kTRhi + kt * 8, tile(tlo, kt), id, true);
         }
+        mma_commit(&sm.tr_done);
       }
+      __syncwarp();
+      wait(&sm.d_ready, ph);
+      tc_fence_after();
+      if (issue) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const uint64_t b = desc_n_major(k + kt * 2048);
+          mma_f16_ta(tm + kTU, tm + kTRhi + kt * 8, b, id_u, kt > 0);
+          mma_f16_ta(tm + kTU, tm + kTRlo + kt * 8, b, id_u, true);
+        }
+        mma_commit(&sm.u_done);
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) mma_f16_ta(tm + kTO2, tm + kTd + kt * 8, tile(p, kt), id, kt > 0);
+        mma_commit(&sm.o_done);
+        mma_commit(&sm.empty[st]);
+      }
+      __syncwarp();
     }
   } else {
     // ---- the copies
     asm volatile("fence.proxy.async.global;" ::: "memory");   // the other kernel's stores, before bulk copies of them
     const int key_heads = a.heads / a.ratio;
-    for (int64_t ci = first; ci < last; ++ci) {
-      const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kStages, so = it % kOutStages;
+    for (int it = 0; it < n; ++it) {
+      const uint32_t st = it % kStages;
       Stage<DK>& sg = sm.stage[st];
-      OutStage<DK>& og = sm.out_stage[so];
-      const int64_t t0 = begin + ci * C, slot = base + ci - slot0;
+      const int64_t ci = first + it, t0 = begin + ci * C, slot = base + ci - slot0;
+      const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
       const unsigned char* kq = work.kq + (slot * key_heads + h / a.ratio) * (2 * C * DK * 2);
       const unsigned char* head = work.heads + (slot * a.heads + h) * static_cast<int64_t>(kHeadBytes);
-      const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
       if (it >= kStages) wait(&sm.empty[st], (it / kStages + 1) & 1);
       if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.full[st], C * DK * 2 + kRecBytes);
-        bulk_g2s(sg.k, kq, C * DK * 2, &sm.full[st]);
-        bulk_g2s(sg.t_hi, head, kRecBytes, &sm.full[st]);
+        mbar_arrive_expect_tx(&sm.full[st], 2 * C * DK * 2 + kHeadBytes);
+        bulk_g2s(sg.k, kq, 2 * C * DK * 2, &sm.full[st]);
+        bulk_g2s(sg.t_hi, head, 2 * kMat, &sm.full[st]);
+        bulk_g2s(sm.f[st], head + 2 * kMat, kFactors * 4, &sm.full[st]);
+        bulk_g2s(sg.p, head + kRecBytes, kMat, &sm.full[st]);
       }
       __syncwarp();
       const uint16_t* v = a.v + t0 * a.v_row + h * a.v_head + c0;
-#pragma unroll
-      for (int i = 0; i < C * kCols * 2 / 16 / 32; ++i) {
-        const int r = i * 8 + (lane >> 2), ch = lane & 3;
-        const uint32_t dst = smem_u32(sg.v) + swz<64>(r, ch);
-        const uint16_t* src = v + (r < cnt ? r * a.v_row + ch * 8 : 0);
+      const int ch = lane & 15, cols = min(a.dv - c0, kCols);
+      const bool in = ch * 8 < cols;
+#pragma unroll 8
+      for (int i = 0; i < C / 2; ++i) {
+        const int r = i * 2 + (lane >> 4);
+        const uint32_t dst = smem_u32(sg.v) + r * (kCols * 2) + ch * 16;
+        const bool live = in && r < cnt;
+        const uint16_t* src = v + (live ? r * a.v_row + ch * 8 : 0);
         if (vec) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < cnt ? 16 : 0)
-                       : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
         } else {
           uint32_t x[4] = {0, 0, 0, 0};
-          if (r < cnt)
+          if (live)
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
@@ -963,17 +880,15 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
         asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&sm.full[st])) : "memory");
       else
         mbar_arrive(&sm.full[st]);
-      if (it >= kOutStages) wait(&sm.out_empty[so], (it / kOutStages + 1) & 1);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.out_full[so], C * DK * 2 + kMat);
-        bulk_g2s(og.q, kq + C * DK * 2, C * DK * 2, &sm.out_full[so]);
-        bulk_g2s(og.p, head + kRecBytes, kMat, &sm.out_full[so]);
-      }
-      __syncwarp();
     }
     // nothing of this warp may still be on its way when the block ends
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (w == 12) tmem_dealloc(tm, kTmemCols);
 }
 
 }  // namespace
@@ -982,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
 namespace {
 
 // Chunks are taken in segments whose workspace stays within this, so that
-// what dn_prep_kernel writes is still in L2 when dn_chunk_kernel reads it.
+// what dn_prep_kernel writes is still in L2 when dn_walk_kernel reads it.
 constexpr int64_t kSegmentBytes = int64_t{128} << 20;
 
 int64_t slot_bytes(int n_heads, int n_key_heads, int dk) {
@@ -1013,7 +928,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
   constexpr const char* what = "qfn_deltanet_chunk";
   const int key_heads = a.heads / a.ratio;
   const int64_t slots = tokens / C + n_seqs, seg = segment_slots(slots, a.heads, key_heads, DK);
-  const int64_t blocks = n_seqs * a.heads * (a.dv / kCols);
+  const int64_t blocks = n_seqs * a.heads * ((a.dv + kCols - 1) / kCols);
   QFN_REQUIRE(blocks <= 0x7fffffff && seg * key_heads <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many sequences",
               what);
   auto even = [](const void* p, int64_t row, int64_t head, int64_t elems) {
@@ -1024,7 +939,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
   cudaError_t e = cudaFuncSetAttribute(dn_prep_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        sizeof(PrepSmem<DK>));
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(dn_chunk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ChunkSmem<DK>));
+    e = cudaFuncSetAttribute(dn_walk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(WalkSmem<DK>) + 1024);
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
   const Plan plan{cu, n_seqs, tokens};
   unsigned char* ws = static_cast<unsigned char*>(workspace);
@@ -1034,7 +949,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
     e = launch(dn_prep_kernel<DK>, (s1 - s0) * key_heads, kPrepThreads, sizeof(PrepSmem<DK>), as_stream(stream), a, plan,
                work, s0, kq_vec);
     if (e == cudaSuccess)
-      e = launch(dn_chunk_kernel<DK>, blocks, kThreads, sizeof(ChunkSmem<DK>), as_stream(stream), a, plan, work, s0, s1,
+      e = launch(dn_walk_kernel<DK>, blocks, kThreads, sizeof(WalkSmem<DK>) + 1024, as_stream(stream), a, plan, work, s0, s1,
                  v_vec);
   }
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
