@@ -10,14 +10,14 @@
 //
 // Two kernels.  dn_prep_kernel does everything that does not need the state,
 // a block per (chunk, key head): k and q as f16 rows, T, P and the decays of
-// each token.  dn_walk_kernel then walks a sequence's chunks, a block per
-// (sequence, value head, 128 columns of S), its products on tcgen05.
+// each token.  dn_chunk_kernel then walks a sequence's chunks, a block per
+// (sequence, value head, 32 columns of S), with S in registers.
 //
 // Precision.  S leaves as fp32, so its factors need more than f16's 11 bits:
 // every operand of an S or d product that is not exact is split into two f16
-// terms (22 bits) after a power-of-two scale of its column; k and q rows are
-// bf16 and exact in f16 after theirs.  The products that only reach the bf16
-// output (P d and S^T q) take one term.
+// terms (22 bits) after a power-of-two scale taken from its largest element;
+// k and q rows are bf16 and exact in f16 after theirs.  The products that
+// only reach the bf16 output (P d and S^T q) take one term.
 #include "deltanet_batch.cuh"
 #include "deltanet_chunk.cuh"
 
@@ -25,17 +25,18 @@ namespace qfn {
 namespace {
 
 constexpr int C = 64;            // tokens of a chunk
-constexpr int kCols = 128;       // state columns of a block: the lanes of TMEM
-constexpr int kStages = 3;
+constexpr int kCols = 32;        // state columns of a block
+constexpr int kStages = 3;       // chunks of what the recurrence reads
+constexpr int kOutStages = 2;    // chunks of what only the outputs read
 constexpr int kPrepThreads = 256;
-constexpr int kThreads = 14 * 32; // 8 warps of the recurrence, 4 of the outputs, the MMAs, the copies
+constexpr int kThreads = 12 * 32; // 8 warps of the recurrence, 4 of the outputs and the copies
 constexpr int kGS = 68;          // row pitch of the 64 x 64 fp32 matrices of dn_prep_kernel
 
 // Per chunk and value head: T hi, T lo (f16, 128-byte rows, swizzled), the
 // tokens' factors and the chunk's scales, then P (as T).
 constexpr int kMat = C * C * 2;
 enum { kFA = 0, kFB = C, kFQ = 2 * C, kFW = 3 * C, kFEnd = 4 * C };   // -beta e^G ck, beta, e^G cq, e^(G64 - G) ck
-// + e^G64, scale of T, scale of P, largest row sums of e^(G64 - G) ck |T| and of |T|
+// + e^G64, scale of T, scale of P, largest row sums of e^(G64 - G) ck |T| and of |T|, largest |beta| e^G
 constexpr int kFactors = 4 * C + 8;
 constexpr int kRecBytes = 2 * kMat + kFactors * 4;
 constexpr int kHeadBytes = kRecBytes + kMat;
@@ -83,20 +84,48 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = pack_h2(a - f.x, b - f.y);
 }
 
+// max(m, |a|, |b|), NaN dropped or kept
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
+  return m;
+}
+__device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
+  asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// D = A B: the first product of an accumulator.
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
 }
-// Byte offset of 16-byte piece `ch` of row `row` in a matrix of 128-byte rows
-// in the 128-byte swizzle that tcgen05 reads.
-__device__ __forceinline__ uint32_t swz(int row, int ch) {
-  return static_cast<uint32_t>(row * 128 + ((ch ^ (row & 7)) << 4));
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
-// A k or q tile: pieces of 64 elements of dk side by side, each [64 tokens][128 bytes], swizzled.
-__device__ __forceinline__ uint32_t tile_at(int row, int ch) { return (ch >> 3) * (C * 128) + swz(row, ch & 7); }
+// Byte offset of 16-byte piece `ch` of row `row` in a matrix of ROW-byte rows
+// whose pieces are permuted so that eight rows' equal pieces lie in distinct banks.
+template <int ROW>
+__device__ __forceinline__ uint32_t swz(int row, int ch) {
+  return static_cast<uint32_t>(row * ROW + ((ROW == 64 ? ch ^ ((row >> 1) & 3) : ch ^ (row & 7)) << 4));
+}
 
 // ------------------------------------------------------------------ what needs no state
 template <int DK>
@@ -217,7 +246,7 @@ __device__ __forceinline__ void f16_row(const uint4 (&x)[DK / 64], unsigned char
   for (int i = 0; i < DK / 64; ++i) {
     const uint4 h = make_uint4(pack_h2(v[i * 8] * sc, v[i * 8 + 1] * sc), pack_h2(v[i * 8 + 2] * sc, v[i * 8 + 3] * sc),
                                pack_h2(v[i * 8 + 4] * sc, v[i * 8 + 5] * sc), pack_h2(v[i * 8 + 6] * sc, v[i * 8 + 7] * sc));
-    const uint32_t at = tile_at(row, part * (DK / 64) + i);
+    const uint32_t at = swz<DK * 2>(row, part * (DK / 64) + i);
     *reinterpret_cast<uint4*>(tile + at) = h;
     *reinterpret_cast<uint4*>(copy + at) = h;
   }
@@ -279,12 +308,12 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 #pragma unroll 2
     for (int kt = 0; kt < DK / 16; ++kt) {
       uint32_t x[4];
-      ldsm4(x, rows + tile_at(m * 16 + (lane & 15), kt * 2 + (lane >> 4)));
+      ldsm4(x, rows + swz<DK * 2>(m * 16 + (lane & 15), kt * 2 + (lane >> 4)));
 #pragma unroll
       for (int np = 0; np < 4; ++np) {
         if (np > m) continue;
         uint32_t b[4];
-        ldsm4(b, cols + tile_at(np * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
+        ldsm4(b, cols + swz<DK * 2>(np * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
         mma_16816(acc[2 * np], x, b[0], b[1]);
         mma_16816(acc[2 * np + 1], x, b[2], b[3]);
       }
@@ -324,6 +353,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         if (lane >= o) run += up;
       }
       rise = warp_sum(rise);
+      float bmax = 0.f;
       const double G[2] = {run - s[1], run};
       const double last = __shfl_sync(0xffffffffu, run, 31);
 #pragma unroll
@@ -335,12 +365,15 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         sm.beta[r] = bt[i];
         const float eg = expf(hi), wt = expf(static_cast<float>(last - G[i])) * sm.ck[r];
         sm.w[r] = wt;
+        bmax = fmaxf(bmax, fabsf(bt[i]) * eg);
         factors[kFA + r] = -bt[i] * eg * sm.ck[r];
         factors[kFB + r] = bt[i];
         factors[kFQ + r] = eg * sm.cq[r];
         factors[kFW + r] = wt;
       }
+      bmax = __uint_as_float(__reduce_max_sync(0xffffffffu, finite_bits(bmax)));
       if (lane == 0) {
+        factors[kFEnd + 5] = bmax;
         // |q_i . k_j| <= 1 / q_scale after the norms, and no decay is above the sum of the rises
         const float bound = expf(rise) / a.q_scale * 1.01f;
         const int e = bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
@@ -384,7 +417,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         }
         *reinterpret_cast<float4*>(&sm.t[i * kGS + j0]) = make_float4(av[0], av[1], av[2], av[3]);
         *reinterpret_cast<float4*>(&sm.t[i * kGS + j0 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
-        *reinterpret_cast<uint4*>(dst + kRecBytes + swz(i, w)) =
+        *reinterpret_cast<uint4*>(dst + kRecBytes + swz<128>(i, w)) =
             make_uint4(pack_h2(pv[0], pv[1]), pack_h2(pv[2], pv[3]), pack_h2(pv[4], pv[5]), pack_h2(pv[6], pv[7]));
       }
     }
@@ -436,7 +469,7 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) split2(tv[s][2 * j] * sc, tv[s][2 * j + 1] * sc, hi[j], lo[j]);
-      const uint32_t at = swz(s * 32 + (tid >> 3), tid & 7);
+      const uint32_t at = swz<128>(s * 32 + (tid >> 3), tid & 7);
       *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       *reinterpret_cast<uint4*>(dst + kMat + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
@@ -451,38 +484,34 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 }
 
 // ------------------------------------------------------------------ the walk over the chunks
-//
-// A lane of TMEM is a column of S, so every product is transposed: A holds S^T,
-// R^T or d^T as f16 terms in TMEM (K: dk or tokens), B the k, q, T or P tile
-// in shared memory (N: tokens or dk), and a thread's values are one column's:
-// scales are per column, and nothing of one column touches another's.  The
-// chain of a chunk is
-//   S k^T (MMA) -> R -> T R (MMA) -> d -> d k (MMA) -> S
-// with the outputs' products S q^T and d P^T issued behind them.
 template <int DK>
 struct Stage {
-  unsigned char k[C * DK * 2], q[C * DK * 2];
-  unsigned char t_hi[kMat], t_lo[kMat], p[kMat];
+  unsigned char k[C * DK * 2];
+  unsigned char t_hi[kMat], t_lo[kMat];
+  float f[kFactors];
   unsigned char v[C * kCols * 2];
 };
-
 template <int DK>
-struct WalkSmem {
-  Stage<DK> stage[kStages];
-  float f[kStages][kFactors];
-  float s_max[2][kCols], r_max[2][kCols];        // [half of dk or of the tokens][column]
-  int r_bad[2][kCols];                           // first token whose R is not finite, or C
-  float o_s[2][kCols], o_d[2][kCols];            // [buffer][column] factors of S q^T and d P^T
-  int o_bad[2][kCols];
-  uint64_t full[kStages], empty[kStages];
-  uint64_t s_ready, r_ready, d_ready, ks_done, tr_done, u_done, o_done, o_free;
-  uint32_t tmem;
+struct OutStage {
+  unsigned char q[C * DK * 2], p[kMat];
 };
 
-// TMEM columns.  d's terms replace R's once T R is done; S k^T and T R lie in U's place,
-// both read before d k is written there.
-constexpr uint32_t kTShi = 0, kTSlo = 64, kTRhi = 128, kTRlo = 160, kTd = 192, kTU = 224, kTKS = 224, kTTR = 288,
-                   kTO1 = 352, kTO2 = 416, kTmemCols = 512;
+// Fragments travel as 16 bytes per lane.
+template <int DK>
+struct ChunkSmem {
+  Stage<DK> stage[kStages];
+  OutStage<DK> out_stage[kOutStages];
+  uint4 s_hi[2][2][4][DK / 64][32];   // [buffer][columns][quarter of dk][k tile][lane]
+  uint4 d_hi[2][2][4][32];            // [buffer][columns][token block][lane]
+  float4 x[2][4][3][2][32];           // partial S^T k [columns][quarter][block - quarter - 1][tile][lane]
+  uint4 rx[2][4][2][32];              // R [columns][token block][hi, lo][lane]
+  uint4 dx[2][4][2][32];              // weighted d, likewise
+  int bad[2][2][16];                  // [buffer][columns][column] first token whose R is not finite, or C
+  float s_inv[2][2], d_inv[2][2];     // [buffer][columns]
+  float s_max[2][4], v_max[2][4];     // [columns][quarter]
+  uint64_t full[kStages], empty[kStages], out_full[kOutStages], out_empty[kOutStages];
+  uint64_t s_full[2][2], d_full[2][2], out_done[2][2];   // [buffer][columns]
+};
 
 // The wait is bounded; a failure is recorded and the walk goes on with what is there.
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
@@ -495,33 +524,31 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-__device__ __forceinline__ void columns_sync() {   // the 8 warps of the recurrence
+// The four warps of 16 columns.
+__device__ __forceinline__ void quad_sync(int id) {
   __syncwarp();
-  asm volatile("bar.sync 1, 256;" ::: "memory");
+  asm volatile("bar.sync %0, 128;" ::"r"(id + 1) : "memory");
 }
 
-// B operand whose N runs along the rows' bytes (k^T for d k): 64 elements of N per 128-byte row,
-// the next 64 C * 128 bytes on, the next 8 of K 1024 bytes on.
-__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(C * 128 >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-constexpr uint32_t kNMajorB = 1u << 16;
-
-// max that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// Sixteen values of a column, scaled, as the f16 terms of 16 steps of K.
-__device__ __forceinline__ void store_terms(const float* v, float s, uint32_t hi_at, uint32_t lo_at) {
-  uint32_t hi[8], lo[8];
+// Largest finite magnitude of a warp's values, the same in every lane.
+template <int N>
+__device__ __forceinline__ float warp_max(const float (&v)[N][4]) {
+  float m0 = 0.f, m1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) split2(v[2 * i] * s, v[2 * i + 1] * s, hi[i], lo[i]);
-  tmem_st_x8(hi_at, hi);
-  tmem_st_x8(lo_at, lo);
+  for (int i = 0; i < N; ++i) {
+    m0 = max_abs(m0, v[i][0], v[i][1]);
+    m1 = max_abs(m1, v[i][2], v[i][3]);
+  }
+  uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(m0, m1)));
+  if (b >= 0x7f800000u) {   // an infinity somewhere: the other columns keep their own scale
+    b = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b = max(b, finite_bits(v[i][j]));
+    b = __reduce_max_sync(0xffffffffu, b);
+  }
+  return __uint_as_float(b);
 }
 
 // Power-of-two scale for a bound; not finite: the smallest scale.
@@ -529,347 +556,400 @@ __device__ __forceinline__ int bound_exp(float bound) {
   return bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
 }
 
+// Accumulators of two neighbouring 16 x 8 tiles as the hi and lo fragments of a 16 x 16 operand.
+__device__ __forceinline__ void frag_split(const float (&a)[4], const float (&b)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  split2(a[0], a[1], hi[0], lo[0]);
+  split2(a[2], a[3], hi[1], lo[1]);
+  split2(b[0], b[1], hi[2], lo[2]);
+  split2(b[2], b[3], hi[3], lo[3]);
+}
+
+__device__ __forceinline__ uint4 as_uint4(const uint32_t (&r)[4]) { return make_uint4(r[0], r[1], r[2], r[3]); }
+__device__ __forceinline__ void from_uint4(uint32_t (&r)[4], uint4 v) { r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w; }
+
+// The output warps of 16 columns take blocks of 16 tokens so that their triangular products take
+// the same time: 0 and 3 to one, 1 and 2 to the other.
+__device__ __forceinline__ int block_of(int half, int i) { return half ? 1 + i : 3 * i; }
+
+// A block's values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
+__device__ __forceinline__ void spoil(float* d, int block, int bad0, int bad1, float v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int tok = block * 16 + i * 8 + 2 * (threadIdx.x & 3);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i * 4 + j] = v;
+  }
+}
+
 template <int DK>
-__global__ void __launch_bounds__(kThreads, 1) dn_walk_kernel(const DnRows a, const Plan plan, const Work work,
-                                                              int64_t slot0, int64_t slot1, bool vec) {
-  extern __shared__ unsigned char raw[];
-  WalkSmem<DK>& sm = *reinterpret_cast<WalkSmem<DK>*>(raw + ((1024 - (smem_u32(raw) & 1023)) & 1023));
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const int cb = (a.dv + kCols - 1) / kCols;
+__global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, const Plan plan, const Work work,
+                                                               int64_t slot0, int64_t slot1, bool vec) {
+  extern __shared__ __align__(1024) unsigned char raw[];
+  ChunkSmem<DK>& sm = *reinterpret_cast<ChunkSmem<DK>*>(raw);
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int cb = a.dv / kCols;
   const int c0 = static_cast<int>(blockIdx.x % cb) * kCols;
   const int h = static_cast<int>(blockIdx.x / cb % a.heads);
   const int64_t seq = blockIdx.x / cb / a.heads;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sm.full[i], 33);
-      mbar_init(&sm.empty[i], 13);   // 8 + 4 warps, the last MMAs
+      mbar_init(&sm.full[i], 129);   // the bulk copies' bytes, 128 lanes' copies of v
+      mbar_init(&sm.empty[i], 12);
     }
-    mbar_init(&sm.s_ready, 8);
-    mbar_init(&sm.r_ready, 8);
-    mbar_init(&sm.d_ready, 8);
-    mbar_init(&sm.ks_done, 1);
-    mbar_init(&sm.tr_done, 1);
-    mbar_init(&sm.u_done, 1);
-    mbar_init(&sm.o_done, 1);
-    mbar_init(&sm.o_free, 4);
+    for (int i = 0; i < kOutStages; ++i) {
+      mbar_init(&sm.out_full[i], 1);
+      mbar_init(&sm.out_empty[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sm.s_full[0][0] + i, 4);
+      mbar_init(&sm.d_full[0][0] + i, 4);
+      mbar_init(&sm.out_done[0][0] + i, 2);
+    }
     fence_mbar_init();
   }
   pdl_wait();
   const bool ok = !plan.cu || dn_plan_ok(plan.cu, plan.n_seqs, plan.tokens);
+  __syncthreads();
   // this launch's chunks of the sequence
   const int64_t begin = ok ? plan.begin(seq) : 0, base = ok ? plan.slot(seq) : slot0;
   const int64_t len = ok ? plan.end(seq) - begin : 0, chunks = (len + C - 1) / C;
   const int64_t first = max(slot0 - base, static_cast<int64_t>(0)), last = min(slot1 - base, chunks);
   if (base >= slot1 || (first > 0 && first >= last)) return;
-  const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
   const float* s_from = first > 0 ? a.s_out : a.s_in;
-  if (w == 12) tmem_alloc(&sm.tmem, kTmemCols);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tm = sm.tmem;
+  const int64_t s_at = (seq * a.heads + h) * DK * static_cast<int64_t>(a.dv) + c0;
 
   if (w < 8) {
-    // ---- the recurrence: a thread has a column, half of dk and half of a chunk's tokens
-    constexpr int NS = DK / 2;
-    const int half = w >> 2, L = (w & 3) * 32 + lane, col = c0 + L;
-    const bool in = col < a.dv;
-    const uint32_t tl = tm + (static_cast<uint32_t>((w & 3) * 32) << 16);
-    const int64_t s_at = ((seq * a.heads + h) * DK + half * NS) * static_cast<int64_t>(a.dv) + col;
-    float S[NS], inv = 1.f, s_max = 0.f;   // S 2^e; 2^-e; the largest of this half
+    // ---- the recurrence: columns grp * 16 .. + 15; a warp holds a quarter of dk of S and forms R and d of
+    // 16 tokens.  The two column groups share the schedulers and do not wait for each other, so one's sums
+    // and barriers run under the other's products; the quarters run the other way in the second group,
+    // since block 3 has four times block 0's products in T R.
+    constexpr int NT = DK / 32, KT = DK / 64;
+    const int grp = w >> 2, qd = grp ? 3 - (w & 3) : w & 3, d0 = qd * (DK / 4);
+    const float* src = s_from ? s_from + s_at + grp * 16 + g : nullptr;
+    float S[NT][4];   // S^T 2^e: rows are columns g and g + 8, columns are dk
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      S[i] = in && s_from ? s_from[s_at + i * static_cast<int64_t>(a.dv)] : 0.f;
-      s_max = fmaxf(s_max, __uint_as_float(finite_bits(S[i])));
+    for (int i = 0; i < NT; ++i) {
+      const int64_t r = static_cast<int64_t>(d0 + i * 8 + 2 * t) * a.dv;
+      S[i][0] = src ? src[r] : 0.f;
+      S[i][1] = src ? src[r + a.dv] : 0.f;
+      S[i][2] = src ? src[r + 8] : 0.f;
+      S[i][3] = src ? src[r + a.dv + 8] : 0.f;
     }
     if (!ok) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) S[i] = CUDART_NAN_F;
+      for (int i = 0; i < NT; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = CUDART_NAN_F;
     }
-    if (n > 0) {
-      sm.s_max[half][L] = s_max;
-      columns_sync();
-      const int e = scale_exp(__float_as_uint(fmaxf(s_max, sm.s_max[half ^ 1][L])));
+    float acc[8][4], vb[2][4];   // this quarter's part of S^T k 2^e, blocks qd, qd + 1, .. (mod 4); beta v of the block
+    float inv = 1.f;             // 2^-e
+    uint32_t kx[KT][4][4];       // k's fragments of the chunk that comes next
+    auto load_keys = [&](uint32_t n) {
+      wait(&sm.full[n % kStages], (n / kStages) & 1);
+      const uint32_t kb = smem_u32(sm.stage[n % kStages].k);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          ldsm4(kx[kt][b], kb + swz<DK * 2>(((qd + b) & 3) * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                            d0 / 8 + kt * 2 + ((lane >> 3) & 1)));
+    };
+    // S as f16 terms times the keys of chunk n; the hi terms go to the warps of the outputs too.  What chunk
+    // n's R needs besides comes behind the products.
+    auto times_keys = [&](uint32_t n) {
+      const uint32_t bf = n & 1;
+      const Stage<DK>& sn = sm.stage[n % kStages];
+      uint32_t hi[KT][4], lo[KT][4];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) frag_split(S[2 * kt], S[2 * kt + 1], hi[kt], lo[kt]);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (kt == 0) {
+            mma_first(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
+            mma_first(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
+          } else {
+            mma_16816(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
+            mma_16816(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          mma_16816(acc[2 * b], lo[kt], kx[kt][b][0], kx[kt][b][1]);
+          mma_16816(acc[2 * b + 1], lo[kt], kx[kt][b][2], kx[kt][b][3]);
+        }
+      }
+      if (n >= 2) wait(&sm.out_done[bf][grp], ((n >> 1) + 1) & 1);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) sm.s_hi[bf][grp][qd][kt][lane] = as_uint4(hi[kt]);
+      if (qd == 0) {
+        if (lane == 0) sm.s_inv[bf][grp] = inv;
+        if (lane < 16) sm.bad[bf][grp][lane] = C;
+      }
+      warp_arrive(&sm.s_full[bf][grp]);
+      uint32_t v[4];   // (columns 0-7 | 8-15) x (tokens 0-7), then tokens 8-15, transposed
+      ldsm4t(v, smem_u32(sn.v) + swz<64>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), grp * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 fb = *reinterpret_cast<const float2*>(&sn.f[kFB + qd * 16 + j * 8 + 2 * t]);
+        vb[j][0] = fb.x * __uint_as_float(v[2 * j] << 16);
+        vb[j][1] = fb.y * __uint_as_float(v[2 * j] & 0xffff0000u);
+        vb[j][2] = fb.x * __uint_as_float(v[2 * j + 1] << 16);
+        vb[j][3] = fb.y * __uint_as_float(v[2 * j + 1] & 0xffff0000u);
+      }
+      const float s_max = warp_max(S) * inv, v_max = warp_max(vb);
+      if (lane == 0) {
+        sm.s_max[grp][qd] = s_max;
+        sm.v_max[grp][qd] = v_max;
+      }
+    };
+    auto largest = [](const float (&v)[4]) {
+      const float4 x = *reinterpret_cast<const float4*>(v);
+      return fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+    };
+    if (first < last) {
+      const float m = warp_max(S);
+      if (lane == 0) sm.s_max[grp][qd] = m;
+      quad_sync(grp);
+      const int e = scale_exp(__float_as_uint(largest(sm.s_max[grp])));
+      quad_sync(grp);   // s_max is written again below
       const float s = exp2i(e);
       inv = exp2i(-e);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) S[i] *= s;
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int i = 0; i < NS; i += 16)
-        store_terms(&S[i], 1.f, tl + kTShi + (half * NS + i) / 2, tl + kTSlo + (half * NS + i) / 2);
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&sm.s_ready);
+        for (int j = 0; j < 4; ++j) S[i][j] *= s;
+      load_keys(0);
+      times_keys(0);
     }
-    for (int it = 0; it < n; ++it) {
-      const uint32_t ph = it & 1, st = it % kStages;
-      const float* f = sm.f[st];
-      wait(&sm.full[st], (it / kStages) & 1);
-      // R = beta v - beta e^G S^T k of 32 tokens
-      float R[32];
-      {
-        uint32_t v[16];   // the column's values of v, two tokens a word
-        const uint16_t* vs = reinterpret_cast<const uint16_t*>(sm.stage[st].v) + half * 32 * kCols + L;
+    for (int64_t ci = first; ci < last; ++ci) {
+      const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kStages, buf = it & 1;
+      Stage<DK>& sg = sm.stage[st];
+      const uint32_t kb = smem_u32(sg.k);
+      const bool more = ci + 1 < last;
+      const float4 fe = *reinterpret_cast<const float4*>(&sg.f[kFEnd]);
+      const float2 fm = *reinterpret_cast<const float2*>(&sg.f[kFEnd + 4]);
+      // the quarters' parts meet, each in the warp of its token block
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = vs[2 * i * kCols] | static_cast<uint32_t>(vs[(2 * i + 1) * kCols]) << 16;
-        wait(&sm.ks_done, ph);
-        tc_fence_after();
-        uint32_t ks[32];
-        tmem_ld_x32(tl + kTKS + half * 32, ks);
+      for (int b = 1; b < 4; ++b)
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 fa = *reinterpret_cast<const float4*>(f + kFA + half * 32 + i);
-          const float4 fb = *reinterpret_cast<const float4*>(f + kFB + half * 32 + i);
-          R[i] = fmaf(fa.x, __uint_as_float(ks[i]) * inv, fb.x * __uint_as_float(v[i / 2] << 16));
-          R[i + 1] = fmaf(fa.y, __uint_as_float(ks[i + 1]) * inv, fb.y * __uint_as_float(v[i / 2] & 0xffff0000u));
-          R[i + 2] = fmaf(fa.z, __uint_as_float(ks[i + 2]) * inv, fb.z * __uint_as_float(v[i / 2 + 1] << 16));
-          R[i + 3] = fmaf(fa.w, __uint_as_float(ks[i + 3]) * inv, fb.w * __uint_as_float(v[i / 2 + 1] & 0xffff0000u));
-        }
+        for (int j = 0; j < 2; ++j)
+          sm.x[grp][qd][b - 1][j][lane] = make_float4(acc[2 * b + j][0], acc[2 * b + j][1], acc[2 * b + j][2], acc[2 * b + j][3]);
+      quad_sync(grp);
+      float R[2][4];
+      const float s_all = largest(sm.s_max[grp]);
+      // |k| <= 1: S^T k is at most sqrt(dk) times S's largest
+      const float r_bound = fmaf(fm.y * (DK == 128 ? 11.4f : 8.1f), s_all, largest(sm.v_max[grp]));
+      const int re = bound_exp(r_bound);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 o1 = sm.x[grp][(qd + 1) & 3][2][j][lane];
+        const float4 o2 = sm.x[grp][(qd + 2) & 3][1][j][lane];
+        const float4 o3 = sm.x[grp][(qd + 3) & 3][0][j][lane];
+        const float2 fa = *reinterpret_cast<const float2*>(&sg.f[kFA + qd * 16 + j * 8 + 2 * t]);
+        const float ax = fa.x * inv, ay = fa.y * inv;
+        R[j][0] = fmaf(ax, (acc[j][0] + o1.x) + (o2.x + o3.x), vb[j][0]);
+        R[j][1] = fmaf(ay, (acc[j][1] + o1.y) + (o2.y + o3.y), vb[j][1]);
+        R[j][2] = fmaf(ax, (acc[j][2] + o1.z) + (o2.z + o3.z), vb[j][2]);
+        R[j][3] = fmaf(ay, (acc[j][3] + o1.w) + (o2.w + o3.w), vb[j][3]);
       }
-      float m4[4] = {};
-#pragma unroll
-      for (int i = 0; i < 32; ++i) m4[i & 3] = max_nan(m4[i & 3], fabsf(R[i]));
-      float m = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
-      int bad = C;
-      if (!(m < CUDART_INF_F)) {
+      const float r_nan = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(0.f, R[0][0], R[0][1]), R[0][2], R[0][3]), R[1][0],
+                                                  R[1][1]), R[1][2], R[1][3]);
+      if (__any_sync(0xffffffffu, !(r_nan < CUDART_INF_F))) {
         // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros:
         // it is taken out here and put back into d from that token on.
-        m = 0.f;
 #pragma unroll
-        for (int i = 31; i >= 0; --i) {
-          if (!(fabsf(R[i]) < CUDART_INF_F)) {
-            bad = half * 32 + i;
-            R[i] = 0.f;
-          }
-          m = fmaxf(m, fabsf(R[i]));
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!(fabsf(R[i][j]) < CUDART_INF_F)) {
+              atomicMin(&sm.bad[buf][grp][g + (j >> 1) * 8], qd * 16 + i * 8 + 2 * t + (j & 1));
+              R[i][j] = 0.f;
+            }
       }
-      sm.r_max[half][L] = m;
-      sm.r_bad[half][L] = bad;
-      sm.s_max[half][L] = s_max;
-      columns_sync();
-      m = fmaxf(m, sm.r_max[half ^ 1][L]);
-      bad = min(bad, sm.r_bad[half ^ 1][L]);
-      const float s_all = fmaxf(s_max, sm.s_max[half ^ 1][L]);
-      const int re = scale_exp(__float_as_uint(m));
+      uint32_t rh[4], rl[4];
       {
         const float s = exp2i(re);
 #pragma unroll
-        for (int i = 0; i < 32; i += 16)
-          store_terms(&R[i], s, tl + kTRhi + half * 16 + i / 2, tl + kTRlo + half * 16 + i / 2);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) R[i][j] *= s;
+        frag_split(R[0], R[1], rh, rl);
+        sm.rx[grp][qd][0][lane] = as_uint4(rh);
+        sm.rx[grp][qd][1][lane] = as_uint4(rl);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&sm.r_ready);
-      // d = T R.  Its scales come from bounds: R's largest times T's row sums, weighted and not.
-      const float4 fe = *reinterpret_cast<const float4*>(f + kFEnd);
-      const float w_bound = m * fe.w;
-      const int we = bound_exp(w_bound), de = bound_exp(m * f[kFEnd + 4]);
+      // T's rows of this block; beyond the diagonal they are zero, and all four warps go the same way
+      uint32_t yh[4][4], yl[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = swz<128>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), ((qd + j) & 3) * 2 + ((lane >> 3) & 1));
+        ldsm4(yh[j], smem_u32(sg.t_hi) + at);
+        ldsm4(yl[j], smem_u32(sg.t_lo) + at);
+      }
+      quad_sync(grp);
+      // d = T R of this block: source blocks qd, qd + 1, .. (mod 4), in two sets of accumulators
+      float p[2][2][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t xh[4], xl[4];
+        if (j == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { xh[i] = rh[i]; xl[i] = rl[i]; }
+        } else {
+          from_uint4(xh, sm.rx[grp][(qd + j) & 3][0][lane]);
+          from_uint4(xl, sm.rx[grp][(qd + j) & 3][1][lane]);
+        }
+        float(&d0_)[4] = p[j & 1][0];
+        float(&d1_)[4] = p[j & 1][1];
+        if (j < 2) {
+          mma_first(d0_, xh, yh[j][0], yh[j][1]);
+          mma_first(d1_, xh, yh[j][2], yh[j][3]);
+        } else {
+          mma_16816(d0_, xh, yh[j][0], yh[j][1]);
+          mma_16816(d1_, xh, yh[j][2], yh[j][3]);
+        }
+        mma_16816(d0_, xl, yh[j][0], yh[j][1]);
+        mma_16816(d1_, xl, yh[j][2], yh[j][3]);
+        mma_16816(d0_, xh, yl[j][0], yl[j][1]);
+        mma_16816(d1_, xh, yl[j][2], yl[j][3]);
+      }
+      // k^T's fragments for the state's update
+      uint32_t kt_[4][NT / 2][4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int np = 0; np < NT / 2; ++np)
+          ldsm4t(kt_[b][np], kb + swz<DK * 2>(((qd + b) & 3) * 16 + (lane & 15), d0 / 8 + np * 2 + (lane >> 4)));
+      // d's scales come from bounds: R's times T's row sums, weighted (for the state, in two terms) and not
+      // (for the outputs, in one)
+      const float w_bound = r_bound * fe.w;
+      const int we = bound_exp(w_bound), de = bound_exp(r_bound * fm.x);
       const float d_inv = w_bound > 0.f ? exp2i(-we) : 0.f;
+      const float c = exp2i(-re) * fe.y, c16 = c * exp2i(de), cw = c * exp2i(we);
+      const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
+      const bool any_bad = __any_sync(0xffffffffu, bad0 < C || bad1 < C);
+      uint32_t wh[4], wl[4], d16[4];
       {
-        const float c1 = exp2i(-re) * fe.y, c16 = c1 * exp2i(de), ws = exp2i(we);
-        wait(&sm.tr_done, ph);
-        tc_fence_after();
-        uint32_t d[32];
-        tmem_ld_x32(tl + kTTR + half * 32, d);
+        float d[2][4];
 #pragma unroll
-        for (int i = 0; i < 32; i += 16) {
-          uint32_t o[8];
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float x = __uint_as_float(d[i + 2 * j]) * c16, y = __uint_as_float(d[i + 2 * j + 1]) * c16;
-            if (half * 32 + i + 2 * j >= bad) x = 0.f;
-            if (half * 32 + i + 2 * j + 1 >= bad) y = 0.f;
-            o[j] = pack_h2(x, y);
-          }
-          tmem_st_x8(tl + kTd + half * 16 + i / 2, o);
+          for (int j = 0; j < 4; ++j) d[i][j] = p[0][i][j] + p[1][i][j];
+        if (any_bad) spoil(&d[0][0], qd, bad0, bad1, 0.f);
+        d16[0] = pack_h2(d[0][0] * c16, d[0][1] * c16);
+        d16[1] = pack_h2(d[0][2] * c16, d[0][3] * c16);
+        d16[2] = pack_h2(d[1][0] * c16, d[1][1] * c16);
+        d16[3] = pack_h2(d[1][2] * c16, d[1][3] * c16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 fw = *reinterpret_cast<const float2*>(&sg.f[kFW + qd * 16 + i * 8 + 2 * t]);
+          const float wx = fw.x * cw, wy = fw.y * cw;
+          d[i][0] *= wx;
+          d[i][1] *= wy;
+          d[i][2] *= wx;
+          d[i][3] *= wy;
         }
-        const float cw = c1 * ws;
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 fw = *reinterpret_cast<const float4*>(f + kFW + half * 32 + i);
-          R[i] = __uint_as_float(d[i]) * cw * fw.x;
-          R[i + 1] = __uint_as_float(d[i + 1]) * cw * fw.y;
-          R[i + 2] = __uint_as_float(d[i + 2]) * cw * fw.z;
-          R[i + 3] = __uint_as_float(d[i + 3]) * cw * fw.w;
-        }
-        if (bad < C) R[0] = CUDART_NAN_F;   // the state's column is lost with it
-#pragma unroll
-        for (int i = 0; i < 32; i += 16)
-          store_terms(&R[i], 1.f, tl + kTRhi + half * 16 + i / 2, tl + kTRlo + half * 16 + i / 2);
+        if (any_bad) spoil(&d[0][0], qd, bad0, bad1, CUDART_NAN_F);
+        frag_split(d[0], d[1], wh, wl);
+        sm.dx[grp][qd][0][lane] = as_uint4(wh);
+        sm.dx[grp][qd][1][lane] = as_uint4(wl);
       }
-      if (half == 0) {
-        sm.o_s[ph][L] = inv;
-        sm.o_d[ph][L] = exp2i(-de) * fe.z;
-        sm.o_bad[ph][L] = bad;
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.d_ready);
-        mbar_arrive(&sm.empty[st]);
-      }
-      // S = e^G64 S + d k.  Its scale comes from a bound: 64 products of d and k, both below 2^15 as f16.
+      quad_sync(grp);
+      // S = e^G64 S + d k^T for this quarter of dk.  Its scale comes from a bound: 64 products of d and
+      // k, both below 2^15 as f16.
       const int e = bound_exp(fmaf(s_all, fe.x, d_inv * 0x1p36f));
       const float s = exp2i(e), keep = fe.x * inv * s, gain = d_inv * s;
       inv = exp2i(-e);
-      wait(&sm.u_done, ph);
-      tc_fence_after();
-      float sm4[4] = {};
+      {
+        float u[NT][4];
 #pragma unroll
-      for (int i = 0; i < NS; i += 16) {
-        uint32_t u[16];
-        tmem_ld_x16(tl + kTU + half * NS + i, u);
+        for (int b = 0; b < 4; ++b) {
+          uint32_t xh[4], xl[4];
+          if (b == 0) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          S[i + j] = fmaf(__uint_as_float(u[j]), gain, S[i + j] * keep);
-          sm4[j & 3] = fmaxf(sm4[j & 3], fabsf(S[i + j]));
-        }
-        store_terms(&S[i], 1.f, tl + kTShi + (half * NS + i) / 2, tl + kTSlo + (half * NS + i) / 2);
-      }
-      s_max = fmaxf(fmaxf(sm4[0], sm4[1]), fmaxf(sm4[2], sm4[3])) * inv;
-      if (!(s_max < CUDART_INF_F)) s_max = 0.f;   // the column is lost; its scale no longer matters
-      tmem_st_wait();
-      tc_fence_before();
-      warp_arrive(&sm.s_ready);
-    }
-    if (in) {
+            for (int i = 0; i < 4; ++i) { xh[i] = wh[i]; xl[i] = wl[i]; }
+          } else {
+            from_uint4(xh, sm.dx[grp][(qd + b) & 3][0][lane]);
+            from_uint4(xl, sm.dx[grp][(qd + b) & 3][1][lane]);
+          }
 #pragma unroll
-      for (int i = 0; i < NS; ++i) a.s_out[s_at + i * static_cast<int64_t>(a.dv)] = S[i] * inv;
-    }
-  } else if (w < 12) {
-    // ---- the outputs: a thread has a column
-    const int L = (w & 3) * 32 + lane, col = c0 + L;
-    const uint32_t tl = tm + (static_cast<uint32_t>((w & 3) * 32) << 16);
-    for (int it = 0; it < n; ++it) {
-      const uint32_t ph = it & 1, st = it % kStages;
-      const float* f = sm.f[st];
-      const int64_t t0 = begin + (first + it) * C;
-      const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
-      wait(&sm.full[st], (it / kStages) & 1);
-      wait(&sm.d_ready, ph);   // for o_s, o_d and o_bad
-      wait(&sm.o_done, ph);
-      tc_fence_after();
-      const float os = sm.o_s[ph][L], od = sm.o_d[ph][L];
-      const int bad = sm.o_bad[ph][L];
-      uint16_t* dst = a.out + (t0 * a.heads + h) * a.dv + col;
+          for (int np = 0; np < NT / 2; ++np) {
+            const uint32_t(&y)[4] = kt_[b][np];
+            if (b == 0) {
+              mma_first(u[2 * np], xh, y[0], y[1]);
+              mma_first(u[2 * np + 1], xh, y[2], y[3]);
+            } else {
+              mma_16816(u[2 * np], xh, y[0], y[1]);
+              mma_16816(u[2 * np + 1], xh, y[2], y[3]);
+            }
+          }
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t x[32], y[32];
-        tmem_ld_x32(tl + kTO1 + hf * 32, x);
-        tmem_ld_x32(tl + kTO2 + hf * 32, y);
-        if (hf) {
-          tc_fence_before();
-          warp_arrive(&sm.o_free);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 fq = *reinterpret_cast<const float4*>(f + kFQ + hf * 32 + i);
-          const float q4[4] = {fq.x, fq.y, fq.z, fq.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int tok = hf * 32 + i + j;
-            float o = fmaf(__uint_as_float(y[i + j]), od, __uint_as_float(x[i + j]) * os * q4[j]);
-            if (tok >= bad) o = CUDART_NAN_F;
-            if (tok < cnt && col < a.dv) dst[static_cast<int64_t>(tok) * a.heads * a.dv] = dn_bf16_bits(o);
+          for (int np = 0; np < NT / 2; ++np) {
+            mma_16816(u[2 * np], xl, kt_[b][np][0], kt_[b][np][1]);
+            mma_16816(u[2 * np + 1], xl, kt_[b][np][2], kt_[b][np][3]);
           }
         }
+        if (more) load_keys(it + 1);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) S[i][j] = fmaf(u[i][j], gain, S[i][j] * keep);
       }
-      warp_arrive(&sm.empty[st]);
+      // d for the outputs of this chunk
+      sm.d_hi[buf][grp][qd][lane] = make_uint4(d16[0], d16[1], d16[2], d16[3]);
+      if (qd == 0 && lane == 0) sm.d_inv[buf][grp] = exp2i(-de);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sm.d_full[buf][grp]);
+        mbar_arrive(&sm.empty[st]);
+      }
+      if (more) times_keys(it + 1);
     }
-  } else if (w == 12) {
-    // ---- the MMAs
-    constexpr uint32_t id = idesc_f16(128, C), id_u = idesc_f16(128, DK) | kNMajorB;
-    const uint32_t issue = elect_one();
-    auto tile = [](uint32_t addr, int kt) { return umma_desc_sw128(addr + (kt >> 2) * (C * 128) + (kt & 3) * 32, 1024); };
-    for (int it = 0; it < n; ++it) {
-      const uint32_t ph = it & 1, st = it % kStages;
-      const Stage<DK>& sg = sm.stage[st];
-      const uint32_t k = smem_u32(sg.k), q = smem_u32(sg.q), th = smem_u32(sg.t_hi), tlo = smem_u32(sg.t_lo),
-                     p = smem_u32(sg.p);
-      wait(&sm.full[st], (it / kStages) & 1);
-      wait(&sm.s_ready, ph);
-      tc_fence_after();
-      if (issue) {
+    float* dst = a.s_out + s_at + grp * 16 + g;
 #pragma unroll
-        for (int kt = 0; kt < DK / 16; ++kt) {
-          mma_f16_ta(tm + kTKS, tm + kTShi + kt * 8, tile(k, kt), id, kt > 0);
-          mma_f16_ta(tm + kTKS, tm + kTSlo + kt * 8, tile(k, kt), id, true);
-        }
-        mma_commit(&sm.ks_done);
-      }
-      __syncwarp();
-      if (it > 0) wait(&sm.o_free, ph ^ 1);
-      tc_fence_after();
-      if (issue) {
-#pragma unroll
-        for (int kt = 0; kt < DK / 16; ++kt) mma_f16_ta(tm + kTO1, tm + kTShi + kt * 8, tile(q, kt), id, kt > 0);
-      }
-      __syncwarp();
-      wait(&sm.r_ready, ph);
-      tc_fence_after();
-      if (issue) {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          mma_f16_ta(tm + kTTR, tm + kTRhi + kt * 8, tile(th, kt), id, kt > 0);
-          mma_f16_ta(tm + kTTR, tm + kTRlo + kt * 8, tile(th, kt), id, true);
-          mma_f16_ta(tm + kTTR, tm + kTRhi + kt * 8, tile(tlo, kt), id, true);
-        }
-        mma_commit(&sm.tr_done);
-      }
-      __syncwarp();
-      wait(&sm.d_ready, ph);
-      tc_fence_after();
-      if (issue) {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          const uint64_t b = desc_n_major(k + kt * 2048);
-          mma_f16_ta(tm + kTU, tm + kTRhi + kt * 8, b, id_u, kt > 0);
-          mma_f16_ta(tm + kTU, tm + kTRlo + kt * 8, b, id_u, true);
-        }
-        mma_commit(&sm.u_done);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) mma_f16_ta(tm + kTO2, tm + kTd + kt * 8, tile(p, kt), id, kt > 0);
-        mma_commit(&sm.o_done);
-        mma_commit(&sm.empty[st]);
-      }
-      __syncwarp();
+    for (int i = 0; i < NT; ++i) {
+      const int64_t r = static_cast<int64_t>(d0 + i * 8 + 2 * t) * a.dv;
+      dst[r] = S[i][0] * inv;
+      dst[r + a.dv] = S[i][1] * inv;
+      dst[r + 8] = S[i][2] * inv;
+      dst[r + a.dv + 8] = S[i][3] * inv;
     }
   } else {
-    // ---- the copies
+    // ---- the outputs: columns grp * 16 .. + 15, half of the token blocks per warp; and the copies
+    constexpr int KT = DK / 64;
+    const int grp = (w - 8) >> 1, half = w & 1, hl = tid - 8 * 32, key_heads = a.heads / a.ratio;
+    const uint32_t n = static_cast<uint32_t>(max(last - first, static_cast<int64_t>(0)));
     asm volatile("fence.proxy.async.global;" ::: "memory");   // the other kernel's stores, before bulk copies of them
-    const int key_heads = a.heads / a.ratio;
-    for (int it = 0; it < n; ++it) {
-      const uint32_t st = it % kStages;
-      Stage<DK>& sg = sm.stage[st];
-      const int64_t ci = first + it, t0 = begin + ci * C, slot = base + ci - slot0;
+    auto head_at = [&](uint32_t it) {
+      return work.heads + ((base + first + it - slot0) * a.heads + h) * static_cast<int64_t>(kHeadBytes);
+    };
+    auto keys_at = [&](uint32_t it) {
+      return work.kq + ((base + first + it - slot0) * key_heads + h / a.ratio) * (2 * C * DK * 2);
+    };
+    // chunk `it` of what the recurrence reads, its stage being free
+    auto copy_in = [&](uint32_t it) {
+      Stage<DK>& sg = sm.stage[it % kStages];
+      uint64_t* bar = &sm.full[it % kStages];
+      const int64_t t0 = begin + (first + it) * C;
       const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
-      const unsigned char* kq = work.kq + (slot * key_heads + h / a.ratio) * (2 * C * DK * 2);
-      const unsigned char* head = work.heads + (slot * a.heads + h) * static_cast<int64_t>(kHeadBytes);
-      if (it >= kStages) wait(&sm.empty[st], (it / kStages + 1) & 1);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sm.full[st], 2 * C * DK * 2 + kHeadBytes);
-        bulk_g2s(sg.k, kq, 2 * C * DK * 2, &sm.full[st]);
-        bulk_g2s(sg.t_hi, head, 2 * kMat, &sm.full[st]);
-        bulk_g2s(sm.f[st], head + 2 * kMat, kFactors * 4, &sm.full[st]);
-        bulk_g2s(sg.p, head + kRecBytes, kMat, &sm.full[st]);
+      if (hl == 0) {
+        mbar_arrive_expect_tx(bar, C * DK * 2 + kRecBytes);
+        bulk_g2s(sg.k, keys_at(it), C * DK * 2, bar);
+        bulk_g2s(sg.t_hi, head_at(it), kRecBytes, bar);
       }
       __syncwarp();
       const uint16_t* v = a.v + t0 * a.v_row + h * a.v_head + c0;
-      const int ch = lane & 15, cols = min(a.dv - c0, kCols);
-      const bool in = ch * 8 < cols;
-#pragma unroll 8
-      for (int i = 0; i < C / 2; ++i) {
-        const int r = i * 2 + (lane >> 4);
-        const uint32_t dst = smem_u32(sg.v) + r * (kCols * 2) + ch * 16;
-        const bool live = in && r < cnt;
-        const uint16_t* src = v + (live ? r * a.v_row + ch * 8 : 0);
+#pragma unroll
+      for (int i = 0; i < C * kCols * 2 / 16 / 128; ++i) {
+        const int r = i * 32 + (hl >> 2), ch = hl & 3;
+        const uint32_t dst = smem_u32(sg.v) + swz<64>(r, ch);
+        const uint16_t* src = v + (r < cnt ? r * a.v_row + ch * 8 : 0);
         if (vec) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < cnt ? 16 : 0)
+                       : "memory");
         } else {
           uint32_t x[4] = {0, 0, 0, 0};
-          if (live)
+          if (r < cnt)
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
@@ -877,18 +957,120 @@ __global__ void __launch_bounds__(kThreads, 1) dn_walk_kernel(const DnRows a, co
         }
       }
       if (vec)
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&sm.full[st])) : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
       else
-        mbar_arrive(&sm.full[st]);
+        mbar_arrive(bar);
+    };
+    // chunk `it` of what only the outputs read
+    auto copy_out_operands = [&](uint32_t it) {
+      OutStage<DK>& og = sm.out_stage[it % kOutStages];
+      uint64_t* bar = &sm.out_full[it % kOutStages];
+      if (hl == 0) {
+        mbar_arrive_expect_tx(bar, C * DK * 2 + kMat);
+        bulk_g2s(og.q, keys_at(it) + C * DK * 2, C * DK * 2, bar);
+        bulk_g2s(og.p, head_at(it) + kRecBytes, kMat, bar);
+      }
+      __syncwarp();
+    };
+    for (uint32_t i = 0; i < n && i < kStages; ++i) copy_in(i);
+    for (uint32_t i = 0; i < n && i < kOutStages; ++i) copy_out_operands(i);
+    for (uint32_t it = 0; it < n; ++it) {
+      const uint32_t st = it % kStages, so = it % kOutStages, buf = it & 1;
+      Stage<DK>& sg = sm.stage[st];
+      OutStage<DK>& og = sm.out_stage[so];
+      const int64_t t0 = begin + (first + it) * C;
+      const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
+      wait(&sm.full[st], (it / kStages) & 1);
+      wait(&sm.out_full[so], (it / kOutStages) & 1);
+      wait(&sm.s_full[buf][grp], (it >> 1) & 1);
+      const uint32_t qb = smem_u32(og.q), pb = smem_u32(og.p);
+      float acc[4][4], o[4][4];
+#pragma unroll
+      for (int kt = 0; kt < DK / 16; ++kt) {
+        uint32_t x[4];
+        from_uint4(x, sm.s_hi[buf][grp][kt / KT][kt % KT][lane]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t y[4];
+          ldsm4(y, qb + swz<DK * 2>(block_of(half, b) * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
+          if (kt == 0) {
+            mma_first(acc[2 * b], x, y[0], y[1]);
+            mma_first(acc[2 * b + 1], x, y[2], y[3]);
+          } else {
+            mma_16816(acc[2 * b], x, y[0], y[1]);
+            mma_16816(acc[2 * b + 1], x, y[2], y[3]);
+          }
+        }
+      }
+      const float si = sm.s_inv[buf][grp];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = *reinterpret_cast<const float2*>(&sg.f[kFQ + block_of(half, i >> 1) * 16 + (i & 1) * 8 + 2 * t]);
+        const float fx = f.x * si, fy = f.y * si;
+        o[i][0] = acc[i][0] * fx;
+        o[i][1] = acc[i][1] * fy;
+        o[i][2] = acc[i][2] * fx;
+        o[i][3] = acc[i][3] * fy;
+      }
+      wait(&sm.d_full[buf][grp], (it >> 1) & 1);
+      const float ps = sm.d_inv[buf][grp] * sg.f[kFEnd + 2];
+#pragma unroll
+      for (int bj = 0; bj < 4; ++bj) {   // P is zero beyond the diagonal
+        uint32_t x[4];
+        from_uint4(x, sm.d_hi[buf][grp][bj][lane]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t y[4];
+          ldsm4(y, pb + swz<128>(block_of(half, b) * 16 + (lane & 7) + ((lane >> 4) << 3), bj * 2 + ((lane >> 3) & 1)));
+          if (bj == 0) {
+            mma_first(acc[2 * b], x, y[0], y[1]);
+            mma_first(acc[2 * b + 1], x, y[2], y[3]);
+          } else {
+            mma_16816(acc[2 * b], x, y[0], y[1]);
+            mma_16816(acc[2 * b + 1], x, y[2], y[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = fmaf(acc[i][j], ps, o[i][j]);
+      {
+        const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
+        if (__any_sync(0xffffffffu, bad0 < C || bad1 < C)) {
+          spoil(&o[0][0], block_of(half, 0), bad0, bad1, CUDART_NAN_F);
+          spoil(&o[2][0], block_of(half, 1), bad0, bad1, CUDART_NAN_F);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sm.out_done[buf][grp]);
+        mbar_arrive(&sm.empty[st]);
+        mbar_arrive(&sm.out_empty[so]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = block_of(half, i >> 1) * 16 + (i & 1) * 8 + g;   // after the transposition a row is a token
+        uint16_t* dst = a.out + ((t0 + tok) * a.heads + h) * a.dv + c0 + grp * 16 + 2 * t;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const __nv_bfloat162 b2 = __floats2bfloat162_rn(o[i][2 * r], o[i][2 * r + 1]);
+          const uint32_t y = transpose8x8(*reinterpret_cast<const uint32_t*>(&b2));
+          if (tok < cnt) *reinterpret_cast<uint32_t*>(dst + 8 * r) = y;
+        }
+      }
+      if (it + kOutStages < n) {
+        wait(&sm.out_empty[so], (it / kOutStages) & 1);
+        copy_out_operands(it + kOutStages);
+      }
+      if (it + kStages < n) {
+        wait(&sm.empty[st], (it / kStages) & 1);
+        copy_in(it + kStages);
+      }
     }
-    // nothing of this warp may still be on its way when the block ends
+    // nothing of these warps may still be on its way when the block ends
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (w == 12) tmem_dealloc(tm, kTmemCols);
 }
 
 }  // namespace
@@ -897,7 +1079,7 @@ __global__ void __launch_bounds__(kThreads, 1) dn_walk_kernel(const DnRows a, co
 namespace {
 
 // Chunks are taken in segments whose workspace stays within this, so that
-// what dn_prep_kernel writes is still in L2 when dn_walk_kernel reads it.
+// what dn_prep_kernel writes is still in L2 when dn_chunk_kernel reads it.
 constexpr int64_t kSegmentBytes = int64_t{128} << 20;
 
 int64_t slot_bytes(int n_heads, int n_key_heads, int dk) {
@@ -928,7 +1110,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
   constexpr const char* what = "qfn_deltanet_chunk";
   const int key_heads = a.heads / a.ratio;
   const int64_t slots = tokens / C + n_seqs, seg = segment_slots(slots, a.heads, key_heads, DK);
-  const int64_t blocks = n_seqs * a.heads * ((a.dv + kCols - 1) / kCols);
+  const int64_t blocks = n_seqs * a.heads * (a.dv / kCols);
   QFN_REQUIRE(blocks <= 0x7fffffff && seg * key_heads <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many sequences",
               what);
   auto even = [](const void* p, int64_t row, int64_t head, int64_t elems) {
@@ -939,7 +1121,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
   cudaError_t e = cudaFuncSetAttribute(dn_prep_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        sizeof(PrepSmem<DK>));
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(dn_walk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(WalkSmem<DK>) + 1024);
+    e = cudaFuncSetAttribute(dn_chunk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(ChunkSmem<DK>));
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
   const Plan plan{cu, n_seqs, tokens};
   unsigned char* ws = static_cast<unsigned char*>(workspace);
@@ -949,7 +1131,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, void
     e = launch(dn_prep_kernel<DK>, (s1 - s0) * key_heads, kPrepThreads, sizeof(PrepSmem<DK>), as_stream(stream), a, plan,
                work, s0, kq_vec);
     if (e == cudaSuccess)
-      e = launch(dn_walk_kernel<DK>, blocks, kThreads, sizeof(WalkSmem<DK>) + 1024, as_stream(stream), a, plan, work, s0, s1,
+      e = launch(dn_chunk_kernel<DK>, blocks, kThreads, sizeof(ChunkSmem<DK>), as_stream(stream), a, plan, work, s0, s1,
                  v_vec);
   }
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
