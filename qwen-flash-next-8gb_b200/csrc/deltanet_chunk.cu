@@ -94,9 +94,15 @@ __device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
   return m;
 }
 
-// D = A B: the first product of an accumulator.
+// D += A B and, for the first product of an accumulator, D = A B.  Not volatile: the compiler may
+// move the products between the loads.
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
@@ -116,7 +122,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
@@ -314,8 +320,8 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         if (np > m) continue;
         uint32_t b[4];
         ldsm4(b, cols + swz<DK * 2>(np * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
-        mma_16816(acc[2 * np], x, b[0], b[1]);
-        mma_16816(acc[2 * np + 1], x, b[2], b[3]);
+        mma_add(acc[2 * np], x, b[0], b[1]);
+        mma_add(acc[2 * np + 1], x, b[2], b[3]);
       }
     }
     float* dst = w < 4 ? sm.gk : sm.gq;
@@ -669,14 +675,14 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
             mma_first(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
             mma_first(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
           } else {
-            mma_16816(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
-            mma_16816(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
+            mma_add(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
+            mma_add(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
           }
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          mma_16816(acc[2 * b], lo[kt], kx[kt][b][0], kx[kt][b][1]);
-          mma_16816(acc[2 * b + 1], lo[kt], kx[kt][b][2], kx[kt][b][3]);
+          mma_add(acc[2 * b], lo[kt], kx[kt][b][0], kx[kt][b][1]);
+          mma_add(acc[2 * b + 1], lo[kt], kx[kt][b][2], kx[kt][b][3]);
         }
       }
       if (n >= 2) wait(&sm.out_done[bf][grp], ((n >> 1) + 1) & 1);
@@ -805,13 +811,13 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
           mma_first(d0_, xh, yh[j][0], yh[j][1]);
           mma_first(d1_, xh, yh[j][2], yh[j][3]);
         } else {
-          mma_16816(d0_, xh, yh[j][0], yh[j][1]);
-          mma_16816(d1_, xh, yh[j][2], yh[j][3]);
+          mma_add(d0_, xh, yh[j][0], yh[j][1]);
+          mma_add(d1_, xh, yh[j][2], yh[j][3]);
         }
-        mma_16816(d0_, xl, yh[j][0], yh[j][1]);
-        mma_16816(d1_, xl, yh[j][2], yh[j][3]);
-        mma_16816(d0_, xh, yl[j][0], yl[j][1]);
-        mma_16816(d1_, xh, yl[j][2], yl[j][3]);
+        mma_add(d0_, xl, yh[j][0], yh[j][1]);
+        mma_add(d1_, xl, yh[j][2], yh[j][3]);
+        mma_add(d0_, xh, yl[j][0], yl[j][1]);
+        mma_add(d1_, xh, yl[j][2], yl[j][3]);
       }
       // k^T's fragments for the state's update
       uint32_t kt_[4][NT / 2][4];
@@ -879,14 +885,14 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
               mma_first(u[2 * np], xh, y[0], y[1]);
               mma_first(u[2 * np + 1], xh, y[2], y[3]);
             } else {
-              mma_16816(u[2 * np], xh, y[0], y[1]);
-              mma_16816(u[2 * np + 1], xh, y[2], y[3]);
+              mma_add(u[2 * np], xh, y[0], y[1]);
+              mma_add(u[2 * np + 1], xh, y[2], y[3]);
             }
           }
 #pragma unroll
           for (int np = 0; np < NT / 2; ++np) {
-            mma_16816(u[2 * np], xl, kt_[b][np][0], kt_[b][np][1]);
-            mma_16816(u[2 * np + 1], xl, kt_[b][np][2], kt_[b][np][3]);
+            mma_add(u[2 * np], xl, kt_[b][np][0], kt_[b][np][1]);
+            mma_add(u[2 * np + 1], xl, kt_[b][np][2], kt_[b][np][3]);
           }
         }
         if (more) load_keys(it + 1);
@@ -997,8 +1003,8 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
             mma_first(acc[2 * b], x, y[0], y[1]);
             mma_first(acc[2 * b + 1], x, y[2], y[3]);
           } else {
-            mma_16816(acc[2 * b], x, y[0], y[1]);
-            mma_16816(acc[2 * b + 1], x, y[2], y[3]);
+            mma_add(acc[2 * b], x, y[0], y[1]);
+            mma_add(acc[2 * b + 1], x, y[2], y[3]);
           }
         }
       }
@@ -1026,8 +1032,8 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
             mma_first(acc[2 * b], x, y[0], y[1]);
             mma_first(acc[2 * b + 1], x, y[2], y[3]);
           } else {
-            mma_16816(acc[2 * b], x, y[0], y[1]);
-            mma_16816(acc[2 * b + 1], x, y[2], y[3]);
+            mma_add(acc[2 * b], x, y[0], y[1]);
+            mma_add(acc[2 * b + 1], x, y[2], y[3]);
           }
         }
       }

@@ -65,7 +65,15 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t i, const floa
   }
 }
 
-__device__ __forceinline__ float sigmoidf(float x) { return 1.f / (1.f + expf(-x)); }
+// 1 / (1 + e^-x) from the special-function unit's exp2 and reciprocal: each within 2 steps of fp32,
+// and the rounding of x log2(e) moves the exponential by |x| 2^-23 at most.  (With expf and a true
+// division the gated norm was bound by its instructions: 106 us for 16384 x 32 rows of 128, 79 with these.)
+__device__ __forceinline__ float sigmoidf(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 
 // ------------------------------------------------------------------ gated norm
 struct GatedNorm {
@@ -77,32 +85,46 @@ struct GatedNorm {
   float eps;
 };
 
-// LANES lanes of a warp share one row of dim <= 8 LANES; a warp carries
-// 32 / LANES rows.
-template <int LANES>
+// LANES lanes of a warp share one row of dim <= 8 LANES; a thread takes its
+// piece of ROWS rows, one block's worth apart, and requests all of them first.
+template <int LANES, int ROWS>
 __global__ void __launch_bounds__(256) gated_norm_kernel(const GatedNorm a) {
+  constexpr int kPer = 256 / LANES;   // rows of a block at a time
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kPer * ROWS) + threadIdx.x / LANES;   // n < 2^31
   const int c = static_cast<int>(threadIdx.x % LANES) * 8;
-  const bool in = i < a.n && c < a.dim;
-  const int64_t row = i / a.heads;
-  const int h = static_cast<int>(i % a.heads);
-  float x[8] = {}, z[8], w[8], ss = 0.f;
-  if (in) {
-    load8(a.x, QFN_DTYPE_BF16, row * a.x_row + h * a.x_head + c, x);
-    load8(a.z, QFN_DTYPE_BF16, row * a.z_row + h * a.z_head + c, z);
-    load8(a.w, a.w_dtype, c, w);
+  const bool col = c < a.dim;
+  uint4 xr[ROWS], zr[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const int64_t i = i0 + k * kPer;
+    const uint32_t row = static_cast<uint32_t>(i) / static_cast<uint32_t>(a.heads),
+                   h = static_cast<uint32_t>(i) - row * static_cast<uint32_t>(a.heads);
+    xr[k] = zr[k] = make_uint4(0, 0, 0, 0);
+    if (col && i < a.n) {
+      xr[k] = *reinterpret_cast<const uint4*>(a.x + row * a.x_row + h * a.x_head + c);
+      zr[k] = *reinterpret_cast<const uint4*>(a.z + row * a.z_row + h * a.z_head + c);
+    }
   }
+  float w[8] = {};
+  if (col) load8(a.w, a.w_dtype, c, w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+  for (int k = 0; k < ROWS; ++k) {
+    const int64_t i = i0 + k * kPer;
+    float x[8], z[8], ss = 0.f;
+    unpack8(xr[k], x);
+    unpack8(zr[k], z);
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (!in) return;
-  const float r = rsqrtf(ss / static_cast<float>(a.dim) + a.eps);
+    for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j] * (z[j] * sigmoidf(z[j]));
-  store8(a.y, QFN_DTYPE_BF16, i * a.dim + c, x);
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!col || i >= a.n) continue;
+    const float r = rsqrtf(ss / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j] * (z[j] * sigmoidf(z[j]));
+    store8(a.y, QFN_DTYPE_BF16, i * a.dim + c, x);
+  }
 }
 
 // Any dim and alignment: a warp per row, read twice (the second time from L1).
@@ -148,7 +170,97 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return warp_sum(t);
 }
 
-// CTA = one row; a thread holds PARTS pieces of WIDTH neighbouring elements
+// Rows of one 8-element piece a thread (dim <= 8 x 512).  A CTA takes row after
+// row, gridDim.x apart, and requests the next row's block, residual and gate
+// while this one's sums are formed, so that two barriers a row leave no gap
+// in the stream of loads.  F32 flags: the operands' types.
+constexpr int kPieceThreads = 512;
+
+template <bool F32>
+struct Piece {
+  uint4 u[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    const uint4* q = F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i)
+                         : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    u[0] = q[0];
+    if (F32) u[F32 ? 1 : 0] = q[F32 ? 1 : 0];
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if (F32) {
+      const uint4 b = u[F32 ? 1 : 0];
+      const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    } else {
+      unpack8(u[0], v);
+    }
+  }
+};
+
+template <bool BF, bool RF, bool GF>
+__global__ void __launch_bounds__(kPieceThreads, 2) norm_residual_piece_kernel(const NormResidual a, int64_t rows) {
+  __shared__ float red[2][2][32];   // [row parity]: a slow warp may still read the last row's sums
+  pdl_wait();
+  pdl_launch_dependents();
+  const int c = threadIdx.x * 8;
+  const bool in = c < a.dim, per_element = a.gate_kind == 2;
+  Piece<BF> bp;
+  Piece<RF> rp;
+  Piece<GF> gp;
+  auto request = [&](int64_t row) {
+    if (row >= rows || !in) return;
+    bp.load(a.block, row * a.block_row + c);
+    rp.load(a.residual, row * a.residual_row + c);
+    if (per_element) gp.load(a.gate, row * a.gate_row + c);
+  };
+  request(blockIdx.x);
+  int parity = 0;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, parity ^= 1) {
+    float b[8] = {}, v[8] = {}, ss = 0.f;
+    if (in) bp.get(b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fmaf(b[j], b[j], ss);
+    if (in && per_element) {   // the gated block; the norm's factor comes later
+      gp.get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] *= a.sigmoid ? sigmoidf(v[j]) : v[j];
+    }
+    if (in) rp.get(v);
+    request(row + gridDim.x);
+    float m = a.scale;
+    if (a.gate_kind == 1) {
+      const float g = load1(a.gate, a.gate_dtype, row * a.gate_row);
+      m *= a.sigmoid ? sigmoidf(g) : g;
+    }
+    if (a.w_post) {
+      m *= rsqrtf(block_sum(ss, red[parity][0]) / static_cast<float>(a.dim) + a.eps);
+      if (in) {
+        float w[8];
+        load8(a.w_post, a.post_dtype, c, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] *= w[j];
+      }
+    }
+    float s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = fmaf(b[j], m, v[j]);
+      s2 = fmaf(v[j], v[j], s2);
+    }
+    if (in) store8(a.r_out, RF ? QFN_DTYPE_F32 : QFN_DTYPE_BF16, row * a.dim + c, v);
+    if (!a.w_next) continue;
+    const float rn = rsqrtf(block_sum(s2, red[parity][1]) / static_cast<float>(a.dim) + a.eps);
+    if (in) {
+      float w[8];
+      load8(a.w_next, a.next_dtype, c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] *= v[j] * rn;
+      store8(a.n_out, QFN_DTYPE_BF16, row * a.dim + c, w);
+    }
+  }
+}
+
+// Other rows: CTA = one row; a thread holds PARTS pieces of WIDTH neighbouring elements
 // (8, or 1 where alignment or dim rule 16-byte pieces out), blockDim.x pieces apart.
 template <int WIDTH, int PARTS>
 __global__ void __launch_bounds__(1024) norm_residual_kernel(const NormResidual a) {
@@ -220,8 +332,8 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(const NormResidual 
 
 namespace {
 
-template <typename Kernel, typename Args>
-int launch(const char* what, Kernel kernel, int64_t blocks, int threads, qfn_stream_t stream, const Args& args) {
+template <typename Kernel, typename... Args>
+int launch(const char* what, Kernel kernel, int64_t blocks, int threads, qfn_stream_t stream, const Args&... args) {
   QFN_REQUIRE(blocks <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many rows", what);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -232,7 +344,7 @@ int launch(const char* what, Kernel kernel, int64_t blocks, int threads, qfn_str
   cfg.stream = as_stream(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   return check_launch(what);
 }
@@ -264,12 +376,18 @@ extern "C" int qfn_gated_norm(const uint16_t* x, int64_t x_row, int64_t x_head, 
   const int rc = current_device(&dev);
   if (rc) return rc;
   const GatedNorm a{x, z, w, y, x_row, x_head, z_row, z_head, rows * heads, w_dtype, heads, dim, eps};
-  const bool v = dim % 8 == 0 && dim <= 256 && wide(x, QFN_DTYPE_BF16, x_row, x_head) &&
+  const bool v = dim % 8 == 0 && dim <= 256 && a.n < (int64_t{1} << 31) && wide(x, QFN_DTYPE_BF16, x_row, x_head) &&
                  wide(z, QFN_DTYPE_BF16, z_row, z_head) && wide(w, w_dtype, 0, 0) && aligned(y, 16);
   if (!v) return launch(what, gated_norm_any_kernel, (a.n + 7) / 8, 256, stream, a);
-  if (dim <= 64) return launch(what, gated_norm_kernel<8>, (a.n + 31) / 32, 256, stream, a);
-  if (dim <= 128) return launch(what, gated_norm_kernel<16>, (a.n + 15) / 16, 256, stream, a);
-  return launch(what, gated_norm_kernel<32>, (a.n + 7) / 8, 256, stream, a);
+  // four rows a thread keep more bytes on their way; below a wave of blocks of them, one row a thread
+  const int lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
+  const int rows_of = a.n >= int64_t{4} * (256 / lanes) * dev->sm_count ? 4 : 1;
+  auto kernel = rows_of == 4 ? (lanes == 8 ? gated_norm_kernel<8, 4> : lanes == 16 ? gated_norm_kernel<16, 4>
+                                                                                : gated_norm_kernel<32, 4>)
+                             : (lanes == 8 ? gated_norm_kernel<8, 1> : lanes == 16 ? gated_norm_kernel<16, 1>
+                                                                                : gated_norm_kernel<32, 1>);
+  const int64_t per = static_cast<int64_t>(256 / lanes) * rows_of;
+  return launch(what, kernel, (a.n + per - 1) / per, 256, stream, a);
 }
 
 extern "C" int qfn_norm_residual(const void* block, int block_dtype, int64_t block_row, const void* residual,
@@ -298,6 +416,17 @@ extern "C" int qfn_norm_residual(const void* block, int block_dtype, int64_t blo
                  (gate_kind != 2 || wide(gate, gate_dtype, gate_row, 0)) && wide(w_next, next_dtype, 0, 0) &&
                  aligned(residual_out, 16) && aligned(normed, 16);
   const int pieces = v ? dim / 8 : dim;
+  if (v && pieces <= kPieceThreads) {
+    const int threads = (pieces + 31) / 32 * 32;
+    const bool bf = block_dtype == QFN_DTYPE_F32, rf = residual_dtype == QFN_DTYPE_F32, gf = gate_dtype == QFN_DTYPE_F32;
+    auto kernel = bf ? (rf ? (gf ? norm_residual_piece_kernel<true, true, true> : norm_residual_piece_kernel<true, true, false>)
+                           : (gf ? norm_residual_piece_kernel<true, false, true> : norm_residual_piece_kernel<true, false, false>))
+                     : (rf ? (gf ? norm_residual_piece_kernel<false, true, true> : norm_residual_piece_kernel<false, true, false>)
+                           : (gf ? norm_residual_piece_kernel<false, false, true> : norm_residual_piece_kernel<false, false, false>));
+    // as many CTAs as are resident at 64 registers a thread
+    const int64_t resident = static_cast<int64_t>(dev->sm_count) * (1024 / threads);
+    return launch(what, kernel, rows < resident ? rows : resident, threads, stream, a, rows);
+  }
   const int parts = (pieces + 1023) / 1024;   // pieces of a thread
   const int per = (pieces + parts - 1) / parts;
   const int threads = (per + 31) / 32 * 32;
