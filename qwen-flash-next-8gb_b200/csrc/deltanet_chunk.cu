@@ -27,6 +27,7 @@ namespace {
 constexpr int C = 64;            // tokens of a chunk
 constexpr int kCols = 32;        // state columns of a block
 constexpr int kStages = 3;       // chunks of what the recurrence reads
+constexpr int kSorted = 64;        // sequences up to which the longest are walked first
 constexpr int kOutStages = 2;    // chunks of what only the outputs read
 constexpr int kPrepThreads = 256;
 constexpr int kThreads = 12 * 32; // 8 warps of the recurrence, 4 of the outputs and the copies
@@ -516,6 +517,7 @@ struct ChunkSmem {
   float s_inv[2][2], d_inv[2][2];     // [buffer][columns]
   float s_max[2][4], v_max[2][4];     // [columns][quarter]
   uint64_t full[kStages], empty[kStages], out_full[kOutStages], out_empty[kOutStages];
+  int length[kSorted], seq;
   uint64_t s_full[2][2], d_full[2][2], out_done[2][2];   // [buffer][columns]
 };
 
@@ -597,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
   const int cb = a.dv / kCols;
   const int c0 = static_cast<int>(blockIdx.x % cb) * kCols;
   const int h = static_cast<int>(blockIdx.x / cb % a.heads);
-  const int64_t seq = blockIdx.x / cb / a.heads;
+  int64_t seq = blockIdx.x / cb / a.heads;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.full[i], 129);   // the bulk copies' bytes, 128 lanes' copies of v
@@ -616,6 +618,20 @@ __global__ void __launch_bounds__(kThreads, 1) dn_chunk_kernel(const DnRows a, c
   }
   pdl_wait();
   const bool ok = !plan.cu || dn_plan_ok(plan.cu, plan.n_seqs, plan.tokens);
+  // Blocks start in order and a sequence's walk cannot be split, so the longest go first: block n takes the
+  // sequence with n longer ones (equal ones in their order).  Worth its n_seqs^2 reads for few sequences only.
+  if (ok && plan.cu && plan.n_seqs <= kSorted) {
+    const int n = static_cast<int>(plan.n_seqs);
+    if (tid < n) sm.length[tid] = plan.cu[tid + 1] - plan.cu[tid];
+    __syncthreads();
+    if (tid < n) {
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += sm.length[i] > sm.length[tid] || (sm.length[i] == sm.length[tid] && i < tid);
+      if (rank == seq) sm.seq = tid;
+    }
+    __syncthreads();
+    seq = sm.seq;
+  }
   __syncthreads();
   // this launch's chunks of the sequence
   const int64_t begin = ok ? plan.begin(seq) : 0, base = ok ? plan.slot(seq) : slot0;
