@@ -305,7 +305,7 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
   DeviceInfo* dev;
   rc = current_device(&dev);
   if (rc) return rc;
-  if (chunked) return dn_chunk(a, cu_seqlens, n_seqs, tokens, dk, workspace, stream);
+  if (chunked) return dn_chunk(a, cu_seqlens, n_seqs, tokens, dk, dev->sm_count, workspace, stream);
   const int64_t blocks = n_seqs * n_heads * (dv / kDbCols);
   auto kernel = dk == 64 ? deltanet_recurrence_kernel<64>
                          : dk == 128 ? deltanet_recurrence_kernel<128> : deltanet_recurrence_kernel<256>;

@@ -1,0 +1,389 @@
+// The walk for many sequences (deltanet_chunk.cu): a block takes 128 columns of
+// a head's S, a warp 16 of them on its own.
+#pragma once
+
+#include "deltanet_chunk_parts.cuh"
+
+namespace qfn {
+namespace {
+
+constexpr int kWarpCols = 128;
+constexpr int kWarpStages = 3;
+constexpr int kWarpThreads = kWarpCols / 16 * 32;
+
+template <int DK>
+struct WarpStage {
+  unsigned char k[C * DK * 2], q[C * DK * 2];
+  unsigned char t_hi[kMat], t_lo[kMat];
+  float f[kFactors];
+  unsigned char p[kMat];
+  unsigned char v[C * kWarpCols * 2];
+};
+
+template <int DK>
+struct WarpSmem {
+  WarpStage<DK> stage[kWarpStages];
+  uint64_t full[kWarpStages], empty[kWarpStages];
+  int length[kSorted], seq;
+};
+
+// Values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
+__device__ __forceinline__ void spoil(float (&d)[8][4], int bad0, int bad1, float v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int tok = i * 8 + 2 * (threadIdx.x & 3);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i][j] = v;
+  }
+}
+
+// A warp walks 16 columns of S on its own, every product transposed so that the columns are the 16 rows
+// of the A operand: the accumulators of one product, split into f16 terms, are then the A fragments of
+// the next, and S, R and d never leave the registers.  The k, q, T and P tiles are B operands that all
+// warps of the block read from shared memory.
+template <int DK>
+__global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnRows a, const Plan plan, const Work work,
+                                                                       int64_t slot0, int64_t slot1, bool vec) {
+  constexpr int kStages = kWarpStages, kVRow = kWarpCols * 2;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  WarpSmem<DK>& sm = *reinterpret_cast<WarpSmem<DK>*>(raw);
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int cb = (a.dv + kWarpCols - 1) / kWarpCols;
+  const int c0 = static_cast<int>(blockIdx.x % cb) * kWarpCols;
+  const int h = static_cast<int>(blockIdx.x / cb % a.heads);
+  const int warps = min(kWarpCols / 16, (a.dv - c0) / 16);   // those with columns
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], 1 + warps * 32);   // the bulk copies' bytes, the lanes' copies of v
+      mbar_init(&sm.empty[i], warps);
+    }
+    fence_mbar_init();
+  }
+  pdl_wait();
+  const Part part = choose(plan, blockIdx.x / cb / a.heads, slot0, slot1, sm.length, &sm.seq);
+  if (part.none(slot1)) return;
+  const int64_t seq = part.seq, begin = part.begin, len = part.len, base = part.base, first = part.first, last = part.last;
+  const bool ok = part.ok;
+  const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
+
+  if (w < warps) {
+    constexpr int NT = DK / 8, KT = DK / 16;
+    const float* s_from = first > 0 ? a.s_out : a.s_in;
+    const int64_t s_at = (seq * a.heads + h) * DK * static_cast<int64_t>(a.dv) + c0 + w * 16 + g;
+    float S[NT][4];   // S^T 2^e: rows are columns g and g + 8, columns are dk
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const float* src = s_from + s_at + static_cast<int64_t>(i * 8 + 2 * t) * a.dv;
+      S[i][0] = s_from ? src[0] : 0.f;
+      S[i][1] = s_from ? src[a.dv] : 0.f;
+      S[i][2] = s_from ? src[8] : 0.f;
+      S[i][3] = s_from ? src[a.dv + 8] : 0.f;
+      if (!ok) S[i][0] = S[i][1] = S[i][2] = S[i][3] = CUDART_NAN_F;
+    }
+    float s_max = warp_max(S), inv;   // the largest of S; 2^-e
+    {
+      const int e = scale_exp(__float_as_uint(s_max));
+      const float s = exp2i(e);
+      inv = exp2i(-e);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[i][j] *= s;
+    }
+    const int64_t pitch = static_cast<int64_t>(a.heads) * a.dv;
+    // where this lane's pieces of a tile's fragments lie: rows of N, and rows of K (transposed)
+    const int n_row = (lane & 7) + ((lane >> 4) << 3), n_ch = (lane >> 3) & 1, k_row = lane & 15, k_ch = lane >> 4;
+    // Chunk `it` to its stage, this warp being done with the chunk before it there: its own columns of v; the
+    // tiles that all warps read by the first, once all are done with it.
+    auto copy = [&](int it) {
+      const int st = it % kStages;
+      WarpStage<DK>& sg = sm.stage[st];
+      const int64_t t0 = begin + (first + it) * C, slot = base + first + it - slot0;
+      const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
+      const uint16_t* v = a.v + t0 * a.v_row + h * a.v_head + c0 + w * 16;
+#pragma unroll
+      for (int i = 0; i < C * 2 / 32; ++i) {
+        const int r = i * 16 + (lane >> 1), ch = lane & 1;
+        const uint32_t dst = smem_u32(sg.v) + swz<kVRow>(r, w * 2 + ch);
+        const uint16_t* src = v + (r < cnt ? r * a.v_row + ch * 8 : 0);
+        if (vec) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(r < cnt ? 16 : 0)
+                       : "memory");
+        } else {
+          uint32_t u[4] = {0, 0, 0, 0};
+          if (r < cnt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3])
+                       : "memory");
+        }
+      }
+      if (vec)
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&sm.full[st])) : "memory");
+      else
+        mbar_arrive(&sm.full[st]);
+      if (w == 0) {
+        if (it >= kStages) wait(&sm.empty[st], (it / kStages + 1) & 1);
+        if (lane == 0) {
+          const int key_heads = a.heads / a.ratio;
+          const unsigned char* head = work.heads + (slot * a.heads + h) * static_cast<int64_t>(kHeadBytes);
+          mbar_arrive_expect_tx(&sm.full[st], 2 * C * DK * 2 + kHeadBytes);
+          bulk_g2s(sg.k, work.kq + (slot * key_heads + h / a.ratio) * (2 * C * DK * 2), 2 * C * DK * 2, &sm.full[st]);
+          bulk_g2s(sg.t_hi, head, kHeadBytes, &sm.full[st]);
+        }
+        __syncwarp();
+      }
+    };
+    asm volatile("fence.proxy.async.global;" ::: "memory");   // the other kernel's stores, before bulk copies of them
+#pragma unroll 1
+    for (int it = 0; it < n && it < kStages - 1; ++it) copy(it);
+#pragma unroll 1
+    for (int it = 0; it < n; ++it) {
+      const int st = it % kStages;
+      const WarpStage<DK>& sg = sm.stage[st];
+      const uint32_t kb = smem_u32(sg.k), qb = smem_u32(sg.q);
+      if (it + kStages - 1 < n) copy(it + kStages - 1);
+      const float* f = sg.f;
+      wait(&sm.full[st], (it / kStages) & 1);
+      // S^T k and, from S's hi terms alone, S^T q: token tiles of 8
+      float x[8][4], o[8][4];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t hi[4], lo[4];
+        frag_split(S[2 * kt], S[2 * kt + 1], hi, lo);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t y[4], z[4];
+          const uint32_t at = swz<DK * 2>(b * 16 + n_row, kt * 2 + n_ch);
+          ldsm4(y, kb + at);
+          ldsm4(z, qb + at);
+          if (kt == 0) {
+            mma_first(x[2 * b], hi, y[0], y[1]);
+            mma_first(x[2 * b + 1], hi, y[2], y[3]);
+            mma_first(o[2 * b], hi, z[0], z[1]);
+            mma_first(o[2 * b + 1], hi, z[2], z[3]);
+          } else {
+            mma_add(x[2 * b], hi, y[0], y[1]);
+            mma_add(x[2 * b + 1], hi, y[2], y[3]);
+            mma_add(o[2 * b], hi, z[0], z[1]);
+            mma_add(o[2 * b + 1], hi, z[2], z[3]);
+          }
+          mma_add(x[2 * b], lo, y[0], y[1]);
+          mma_add(x[2 * b + 1], lo, y[2], y[3]);
+        }
+      }
+      // R = beta v - beta e^G S^T k
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t v[4];   // (columns 0-7 | 8-15) x (tokens 0-7), then tokens 8-15, transposed
+        ldsm4t(v, smem_u32(sg.v) + swz<kVRow>(b * 16 + n_row, w * 2 + n_ch));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = 2 * b + j;
+          const float2 fa = *reinterpret_cast<const float2*>(f + kFA + i * 8 + 2 * t);
+          const float2 fb = *reinterpret_cast<const float2*>(f + kFB + i * 8 + 2 * t);
+          const float ax = fa.x * inv, ay = fa.y * inv;
+          x[i][0] = fmaf(ax, x[i][0], fb.x * __uint_as_float(v[2 * j] << 16));
+          x[i][1] = fmaf(ay, x[i][1], fb.y * __uint_as_float(v[2 * j] & 0xffff0000u));
+          x[i][2] = fmaf(ax, x[i][2], fb.x * __uint_as_float(v[2 * j + 1] << 16));
+          x[i][3] = fmaf(ay, x[i][3], fb.y * __uint_as_float(v[2 * j + 1] & 0xffff0000u));
+        }
+      }
+      float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        m0 = max_abs_nan(m0, x[i][0], x[i][1]);
+        m1 = max_abs_nan(m1, x[i][2], x[i][3]);
+      }
+      uint32_t rm = __reduce_max_sync(0xffffffffu, __float_as_uint(max_abs_nan(m0, m1, 0.f)) & 0x7fffffffu);
+      int bad0 = C, bad1 = C;
+      const bool any_bad = rm >= 0x7f800000u;
+      if (any_bad) {
+        // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros:
+        // it is taken out here and put back into d from that token on.
+        rm = 0;
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+#pragma unroll
+          for (int j = 3; j >= 0; --j) {
+            if (!(fabsf(x[i][j]) < CUDART_INF_F)) {
+              (j < 2 ? bad0 : bad1) = min(j < 2 ? bad0 : bad1, i * 8 + 2 * t + (j & 1));
+              x[i][j] = 0.f;
+            }
+            rm = max(rm, finite_bits(x[i][j]));
+          }
+        rm = __reduce_max_sync(0xffffffffu, rm);
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+          bad0 = min(bad0, __shfl_xor_sync(0xffffffffu, bad0, off));
+          bad1 = min(bad1, __shfl_xor_sync(0xffffffffu, bad1, off));
+        }
+      }
+      const float r_max = __uint_as_float(rm);
+      const int re = scale_exp(rm);
+      uint32_t rh[4][4], rl[4][4];
+      {
+        const float s = exp2i(re);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i][j] *= s;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) frag_split(x[2 * b], x[2 * b + 1], rh[b], rl[b]);
+      }
+      // d = T R, blocks on and below the diagonal
+      const uint32_t th = smem_u32(sg.t_hi), tl = smem_u32(sg.t_lo);
+#pragma unroll
+      for (int bj = 0; bj < 4; ++bj) {
+#pragma unroll
+        for (int bi = bj; bi < 4; ++bi) {
+          uint32_t y[4], z[4];
+          const uint32_t at = swz<128>(bi * 16 + n_row, bj * 2 + n_ch);
+          ldsm4(y, th + at);
+          ldsm4(z, tl + at);
+          if (bj == 0) {
+            mma_first(x[2 * bi], rh[bj], y[0], y[1]);
+            mma_first(x[2 * bi + 1], rh[bj], y[2], y[3]);
+          } else {
+            mma_add(x[2 * bi], rh[bj], y[0], y[1]);
+            mma_add(x[2 * bi + 1], rh[bj], y[2], y[3]);
+          }
+          mma_add(x[2 * bi], rl[bj], y[0], y[1]);
+          mma_add(x[2 * bi + 1], rl[bj], y[2], y[3]);
+          mma_add(x[2 * bi], rh[bj], z[0], z[1]);
+          mma_add(x[2 * bi + 1], rh[bj], z[2], z[3]);
+        }
+      }
+      // d's scales come from bounds: R's largest times T's row sums, weighted (for the state, in two terms) and
+      // not (for the outputs, in one)
+      const float4 fe = *reinterpret_cast<const float4*>(f + kFEnd);
+      const float w_bound = r_max * fe.w;
+      const int we = bound_exp(w_bound), de = bound_exp(r_max * f[kFEnd + 4]);
+      const float d_inv = w_bound > 0.f ? exp2i(-we) : 0.f;
+      const float c = exp2i(-re) * fe.y, c16 = c * exp2i(de), cw = c * exp2i(we);
+      if (any_bad) spoil(x, bad0, bad1, 0.f);
+      uint32_t d16[4][4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        d16[b][0] = pack_h2(x[2 * b][0] * c16, x[2 * b][1] * c16);
+        d16[b][1] = pack_h2(x[2 * b][2] * c16, x[2 * b][3] * c16);
+        d16[b][2] = pack_h2(x[2 * b + 1][0] * c16, x[2 * b + 1][1] * c16);
+        d16[b][3] = pack_h2(x[2 * b + 1][2] * c16, x[2 * b + 1][3] * c16);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 fw = *reinterpret_cast<const float2*>(f + kFW + i * 8 + 2 * t);
+        const float wx = fw.x * cw, wy = fw.y * cw;
+        x[i][0] *= wx;
+        x[i][1] *= wy;
+        x[i][2] *= wx;
+        x[i][3] *= wy;
+      }
+      if (any_bad) spoil(x, bad0, bad1, CUDART_NAN_F);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) frag_split(x[2 * b], x[2 * b + 1], rh[b], rl[b]);
+      // o = e^G S^T q + P d
+      {
+        const float os = inv, ps = exp2i(-de) * fe.z;
+        const uint32_t pb = smem_u32(sg.p);
+#pragma unroll
+        for (int bi = 0; bi < 4; ++bi) {
+          float e[2][4];
+#pragma unroll
+          for (int bj = 0; bj <= bi; ++bj) {
+            uint32_t y[4];
+            ldsm4(y, pb + swz<128>(bi * 16 + n_row, bj * 2 + n_ch));
+            if (bj == 0) {
+              mma_first(e[0], d16[bj], y[0], y[1]);
+              mma_first(e[1], d16[bj], y[2], y[3]);
+            } else {
+              mma_add(e[0], d16[bj], y[0], y[1]);
+              mma_add(e[1], d16[bj], y[2], y[3]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int i = 2 * bi + j;
+            const float2 fq = *reinterpret_cast<const float2*>(f + kFQ + i * 8 + 2 * t);
+            const float qx = fq.x * os, qy = fq.y * os;
+            o[i][0] = fmaf(e[j][0], ps, o[i][0] * qx);
+            o[i][1] = fmaf(e[j][1], ps, o[i][1] * qy);
+            o[i][2] = fmaf(e[j][2], ps, o[i][2] * qx);
+            o[i][3] = fmaf(e[j][3], ps, o[i][3] * qy);
+          }
+        }
+        if (any_bad) spoil(o, bad0, bad1, CUDART_NAN_F);
+        const int64_t t0 = begin + (first + it) * C;
+        const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
+        uint16_t* dst = a.out + (t0 + g) * pitch + static_cast<int64_t>(h) * a.dv + c0 + w * 16 + 2 * t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {   // after the transposition a row is a token
+          const __nv_bfloat162 b0 = __floats2bfloat162_rn(o[i][0], o[i][1]), b1 = __floats2bfloat162_rn(o[i][2], o[i][3]);
+          const uint32_t y0 = transpose8x8(*reinterpret_cast<const uint32_t*>(&b0));
+          const uint32_t y1 = transpose8x8(*reinterpret_cast<const uint32_t*>(&b1));
+          if (i * 8 + g < cnt) {
+            *reinterpret_cast<uint32_t*>(dst) = y0;
+            *reinterpret_cast<uint32_t*>(dst + 8) = y1;
+          }
+          dst += 8 * pitch;
+        }
+      }
+      // S = e^G64 S + d k.  Its scale comes from a bound: 64 products of d and k, both below 2^15 as f16.
+      const int e = bound_exp(fmaf(s_max, fe.x, d_inv * 0x1p36f));
+      const float s = exp2i(e), keep = fe.x * inv * s, gain = d_inv * s;
+      inv = exp2i(-e);
+      m0 = m1 = 0.f;
+#pragma unroll
+      for (int np = 0; np < NT / 4; ++np) {   // 32 of dk at a time
+        float u[4][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t y[4], z[4];
+          ldsm4t(y, kb + swz<DK * 2>(b * 16 + k_row, np * 4 + k_ch));
+          ldsm4t(z, kb + swz<DK * 2>(b * 16 + k_row, np * 4 + 2 + k_ch));
+          if (b == 0) {
+            mma_first(u[0], rh[b], y[0], y[1]);
+            mma_first(u[1], rh[b], y[2], y[3]);
+            mma_first(u[2], rh[b], z[0], z[1]);
+            mma_first(u[3], rh[b], z[2], z[3]);
+          } else {
+            mma_add(u[0], rh[b], y[0], y[1]);
+            mma_add(u[1], rh[b], y[2], y[3]);
+            mma_add(u[2], rh[b], z[0], z[1]);
+            mma_add(u[3], rh[b], z[2], z[3]);
+          }
+          mma_add(u[0], rl[b], y[0], y[1]);
+          mma_add(u[1], rl[b], y[2], y[3]);
+          mma_add(u[2], rl[b], z[0], z[1]);
+          mma_add(u[3], rl[b], z[2], z[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) S[np * 4 + i][j] = fmaf(u[i][j], gain, S[np * 4 + i][j] * keep);
+          m0 = max_abs(m0, S[np * 4 + i][0], S[np * 4 + i][1]);
+          m1 = max_abs(m1, S[np * 4 + i][2], S[np * 4 + i][3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[st]);
+      s_max = fmaxf(m0, m1);
+      uint32_t sb = __reduce_max_sync(0xffffffffu, __float_as_uint(s_max));
+      s_max = sb < 0x7f800000u ? __uint_as_float(sb) * inv : warp_max(S) * inv;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      float* dst = a.s_out + s_at + static_cast<int64_t>(i * 8 + 2 * t) * a.dv;
+      dst[0] = S[i][0] * inv;
+      dst[a.dv] = S[i][1] * inv;
+      dst[8] = S[i][2] * inv;
+      dst[a.dv + 8] = S[i][3] * inv;
+    }
+    // nothing of this warp may still be on its way when the block ends
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+}
+
+}  // namespace
+}  // namespace qfn

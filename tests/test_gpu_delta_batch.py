@@ -122,6 +122,70 @@ def test_chunk_more_than_one_segment():
     run_ragged([100, 6000, 0, 40], 32, 32, 128, 32, seed=8, carried=True)
 
 
+@pytest.mark.parametrize("lens,H,Hk,dk,dv", [
+    ([70, 1, 0, 64, 129, 65, 200, 33, 16, 128, 5, 63], 8, 4, 128, 128),
+    ([90] * 20, 8, 8, 64, 96),
+    ([90] * 50, 4, 2, 128, 64),
+    ([65, 0, 100] * 10, 8, 2, 64, 160),
+    ([20] * 70 + [100], 3, 1, 128, 128)], ids=lambda x: str(x)[:20])
+def test_chunk_many_states(lens, H, Hk, dk, dv):
+    """Enough states for the walk of many sequences (blocks of 128 columns, the last of them partly filled)."""
+    run_ragged(lens, H, Hk, dk, dv, seed=len(lens) + dv, carried=True)
+
+
+def test_chunk_few_and_many_states_agree():
+    """The two walks on the same sequences: one alone, and as one of many."""
+    H, Hk, dk, dv, T, N = 4, 2, 128, 128, 200, 40
+    q, k, v, g, beta = inputs(T, H, Hk, dk, dv, seed=12, strided=False)
+    S0 = states(1, H, dk, dv, 3)
+    one, S_one = deltanet.chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], S0)
+    rep = [t.repeat(N, *[1] * (t.dim() - 1)).unflatten(0, (N, T)) for t in (q, k, v, g, beta)]
+    many, S_many = deltanet.chunk_gated_delta_rule(*rep, S0.repeat(N, 1, 1, 1))
+    assert (many == many[:1]).all() and (S_many == S_many[:1]).all()
+    ref = oracle(q, k, v, g, beta, S0[0])
+    check(one[0], S_one[0], ref, T)
+    check(many[N - 1], S_many[N - 1], ref, T)
+
+
+@pytest.mark.parametrize("case", ["reset", "strong", "none", "zero-keys", "beta0", "same-keys", "large", "small"])
+def test_chunk_extremes_many_states(case):
+    """The cases of test_chunk_extremes in the walk of many sequences."""
+    H, Hk, dk, dv, T, N = 4, 1, 128, 128, 150, 40
+    q, k, v, g, beta = inputs(T, H, Hk, dk, dv, seed=22, strided=False)
+    S0 = states(1, H, dk, dv, 8)
+    q, k, v, g, beta, S0 = extreme(case, q, k, v, g, beta, S0)
+    rep = [t.repeat(N, *[1] * (t.dim() - 1)).unflatten(0, (N, T)) for t in (q, k, v, g, beta)]
+    out, S = deltanet.chunk_gated_delta_rule(*rep, S0.repeat(N, 1, 1, 1))
+    check(out[N - 1], S[N - 1], oracle(q, k, v, g, beta, S0[0]), T)
+
+
+def test_chunk_nan_stays_in_its_column_many_states():
+    H, dk, dv, T, N = 4, 64, 128, 150, 40
+    q, k, v, g, beta = inputs(T, H, 1, dk, dv, seed=4, strided=False)
+    v[T // 2, 1, 40] = float("nan")
+    v[T // 2, 1, 9] = float("inf")
+    rep = [t.repeat(N, *[1] * (t.dim() - 1)).unflatten(0, (N, T)) for t in (q, k, v, g, beta)]
+    out, S = deltanet.chunk_gated_delta_rule(*rep)
+    keep = torch.ones(H, dv, dtype=torch.bool, device=DEV)
+    keep[1, [9, 40]] = False
+    assert not out[0, T // 2:].isfinite()[:, ~keep].any() and out[0, :T // 2].isfinite().all()
+    assert not S[0].isfinite()[1][:, [9, 40]].any()
+    vv = torch.where(v.isfinite(), v, 0)
+    r_out, r_S, mag, top = oracle(q, k, vv, g, beta, None)
+    zero = lambda t, m: torch.where(m, t.double(), 0.0)
+    check(zero(out[3], keep), zero(S[3], keep[:, None]), (zero(r_out, keep), zero(r_S, keep[:, None]), mag, top), T)
+
+
+def test_chunk_bad_bounds_many_states():
+    T, N, H, dk, dv = 400, 40, 4, 64, 128
+    q, k, v, g, beta = inputs(T, H, 1, dk, dv, seed=2)
+    out = torch.full((1, T, H, dv), 7.0, dtype=torch.bfloat16, device=DEV)
+    cu = torch.arange(N + 1, dtype=torch.int32, device=DEV) * 10
+    cu[17] = 400
+    _, S = deltanet.chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], out=out, cu_seqlens=cu)
+    assert (out == 7).all() and S.isnan().all()
+
+
 def test_chunk_many_short_sequences():
     gen = torch.Generator().manual_seed(9)
     lens = torch.randint(0, 9, (150,), generator=gen).tolist()
@@ -217,14 +281,8 @@ def test_chunk_nothing_to_do():
     assert S.shape == (1, H, dk, dv) and (S == 0).all()
 
 
-@pytest.mark.parametrize("T", [9, 150])
-@pytest.mark.parametrize("case", ["reset", "strong", "none", "zero-keys", "beta0", "same-keys", "large", "small"])
-def test_chunk_extremes(case, T):
-    """A decay of zero in mid-sequence, strong and no decay, keys and betas of zero, one key
-    repeated, values far from one."""
-    H, Hk, dk, dv = 2, 1, 128, 32
-    q, k, v, g, beta = inputs(T, H, Hk, dk, dv, seed=21, strided=False)
-    S0 = states(1, H, dk, dv, 8)
+def extreme(case, q, k, v, g, beta, S0):
+    T = q.shape[0]
     if case == "reset":
         g[T // 2] = -float("inf")
         g[T // 2 + 2] = -1e30
@@ -246,6 +304,18 @@ def test_chunk_extremes(case, T):
     elif case == "small":
         v, S0 = v * 2.0 ** -60, S0 * 2.0 ** -60
         k, q = k * 2.0 ** -8, q * 2.0 ** 50
+    return q, k, v, g, beta, S0
+
+
+@pytest.mark.parametrize("T", [9, 150])
+@pytest.mark.parametrize("case", ["reset", "strong", "none", "zero-keys", "beta0", "same-keys", "large", "small"])
+def test_chunk_extremes(case, T):
+    """A decay of zero in mid-sequence, strong and no decay, keys and betas of zero, one key
+    repeated, values far from one."""
+    H, Hk, dk, dv = 2, 1, 128, 32
+    q, k, v, g, beta = inputs(T, H, Hk, dk, dv, seed=21, strided=False)
+    S0 = states(1, H, dk, dv, 8)
+    q, k, v, g, beta, S0 = extreme(case, q, k, v, g, beta, S0)
     out, S = deltanet.chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], S0,
                                              torch.tensor([0, T], dtype=torch.int32, device=DEV))
     check(out[0], S[0], oracle(q, k, v, g, beta, S0[0]), T)
@@ -272,9 +342,18 @@ def test_chunk_nan_stays_in_its_sequence_and_column(T):
 
 def test_chunk_repeats_bit_for_bit_on_another_stream_and_in_a_graph():
     lens, H, Hk, dk, dv = [70, 3, 129], 4, 2, 128, 64
+    stream_and_graph(lens, H, Hk, dk, dv, (lens, [1, 200, 1], [0, 0, 202]))
+
+
+def test_chunk_many_states_on_another_stream_and_in_a_graph():
+    lens = [30] * 40
+    stream_and_graph(lens, 4, 2, 64, 128, (lens, [1200] + [0] * 39, [29] * 39 + [69]))
+
+
+def stream_and_graph(lens, H, Hk, dk, dv, replays):
     cu = offsets(lens)
     q, k, v, g, beta = (t[None] for t in inputs(sum(lens), H, Hk, dk, dv, seed=6))
-    S0 = states(3, H, dk, dv, 2)
+    S0 = states(len(lens), H, dk, dv, 2)
     out, S = deltanet.chunk_gated_delta_rule(q, k, v, g, beta, S0, cu)
     torch.cuda.synchronize()
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
@@ -291,7 +370,7 @@ def test_chunk_repeats_bit_for_bit_on_another_stream_and_in_a_graph():
         o1, s1 = deltanet.chunk_gated_delta_rule(q, k, v, g, beta, S0, cu)
         o2, s2 = deltanet.chunk_gated_delta_rule(q, k, v, g, beta, s1, cu)
     # other lengths at replay: the bounds are read on the device
-    for lens2 in (lens, [1, 200, 1], [0, 0, 202]):
+    for lens2 in replays:
         cu.copy_(offsets(lens2))
         graph.replay()
         e1, f1 = deltanet.chunk_gated_delta_rule(q, k, v, g, beta, S0, cu)
