@@ -107,6 +107,17 @@ def ops():
     return _ops
 
 
+_overloads = {}
+
+
+def op(name):
+    """One operator of ops() as its overload, which skips the search for one at every call."""
+    f = _overloads.get(name)
+    if f is None:
+        f = _overloads[name] = getattr(ops(), name).default
+    return f
+
+
 def check(rc, what):
     if rc != 0:
         L = lib()

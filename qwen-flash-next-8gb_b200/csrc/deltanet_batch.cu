@@ -105,7 +105,7 @@ __device__ __forceinline__ void dn_store_state(const float4 (&s)[DK / 16], float
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane & 7, row0 = w * 4 + (lane >> 3);
 #pragma unroll
   for (int p = 0; p < DK / 16; ++p)
-    *reinterpret_cast<float4*>(S + static_cast<int64_t>(p * 16 + row0) * dv + c4 * 4) = s[p];
+    __stcs(reinterpret_cast<float4*>(S + static_cast<int64_t>(p * 16 + row0) * dv + c4 * 4), s[p]);
 }
 
 template <int DK>
@@ -113,7 +113,7 @@ __device__ __forceinline__ void dn_load_state(float4 (&s)[DK / 16], const float*
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane & 7, row0 = w * 4 + (lane >> 3);
 #pragma unroll
   for (int p = 0; p < DK / 16; ++p)
-    s[p] = S ? *reinterpret_cast<const float4*>(S + static_cast<int64_t>(p * 16 + row0) * dv + c4 * 4)
+    s[p] = S ? __ldcs(reinterpret_cast<const float4*>(S + static_cast<int64_t>(p * 16 + row0) * dv + c4 * 4))
              : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 

@@ -387,15 +387,16 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 // ------------------------------------------------------------------ host
 namespace {
 
-// Chunks are taken in segments whose workspace stays within this, so that
-// what dn_prep_kernel writes is still in L2 when a walk reads it.
-constexpr int64_t kSegmentBytes = int64_t{128} << 20;
+// Chunks are taken in segments of slots, which bounds the workspace.  One sequence: what dn_prep_kernel writes
+// should still be in L2 when a walk reads it.  Several: a segment holds whole sequences but for its ends, so it
+// has to be long enough for all SMs to have some to walk.
+constexpr int64_t kSegmentBytes = int64_t{128} << 20, kBatchSegmentBytes = int64_t{1} << 30;
 
 int64_t slot_bytes(int n_heads, int n_key_heads, int dk) {
   return static_cast<int64_t>(n_key_heads) * 2 * C * dk * 2 + static_cast<int64_t>(n_heads) * kHeadBytes;
 }
-int64_t segment_slots(int64_t slots, int n_heads, int n_key_heads, int dk) {
-  const int64_t fit = kSegmentBytes / slot_bytes(n_heads, n_key_heads, dk);
+int64_t segment_slots(int64_t n_seqs, int64_t slots, int n_heads, int n_key_heads, int dk) {
+  const int64_t fit = (n_seqs == 1 ? kSegmentBytes : kBatchSegmentBytes) / slot_bytes(n_heads, n_key_heads, dk);
   return slots < fit ? slots : fit > 1 ? fit : 1;
 }
 
@@ -426,7 +427,7 @@ template <int DK>
 int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, int sms, void* workspace, qfn_stream_t stream) {
   constexpr const char* what = "qfn_deltanet_chunk";
   const int key_heads = a.heads / a.ratio;
-  const int64_t slots = tokens / C + n_seqs, seg = segment_slots(slots, a.heads, key_heads, DK);
+  const int64_t slots = tokens / C + n_seqs, seg = segment_slots(n_seqs, slots, a.heads, key_heads, DK);
   const bool quad = quad_walk(n_seqs * a.heads, a.dv, sms);
   const int cols = quad ? kQuadCols : kWarpCols;
   const int64_t blocks = n_seqs * a.heads * ((a.dv + cols - 1) / cols);
@@ -465,7 +466,7 @@ bool dn_chunk_takes(int64_t tokens, int dk) { return dk <= 128 && tokens > kRecu
 
 size_t dn_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk) {
   const int64_t slots = tokens / C + n_seqs;
-  return static_cast<size_t>(segment_slots(slots, n_heads, n_key_heads, dk) * slot_bytes(n_heads, n_key_heads, dk));
+  return static_cast<size_t>(segment_slots(n_seqs, slots, n_heads, n_key_heads, dk) * slot_bytes(n_heads, n_key_heads, dk));
 }
 
 int dn_chunk(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, int dk, int sms, void* workspace,

@@ -19,7 +19,7 @@ All three are forward only.
 """
 import torch
 
-from _lib import check, lib, on_device, ops, require_cuda, stream_of
+from _lib import check, lib, on_device, op, require_cuda, stream_of
 
 
 def recurrent_gated_delta_rule(query, key, value, g, beta, initial_state):
@@ -82,7 +82,7 @@ def chunk_gated_delta_rule(query, key, value, g, beta, initial_state=None, cu_se
             raise ValueError(f"out must be a contiguous [{B}, {T}, {value.shape[2]}, {value.shape[3]}], "
                              f"got {tuple(out.shape)}")
         out = out.view(B * T, *out.shape[2:])
-    o, S = ops().deltanet_chunk(query.flatten(0, 1), key.flatten(0, 1), value.flatten(0, 1), g.flatten(0, 1),
+    o, S = op("deltanet_chunk")(query.flatten(0, 1), key.flatten(0, 1), value.flatten(0, 1), g.flatten(0, 1),
                                 beta.flatten(0, 1), B, cu_seqlens, initial_state, final_state, out)
     return o.view(B, T, *o.shape[1:]), S
 
@@ -100,5 +100,5 @@ def step_gated_delta_rule(query, key, value, g, beta, state, state_index=None, o
     (None: state itself, in place); slots that no row names are left as they were."""
     if out_state is None:
         out_state = state
-    o = ops().deltanet_step(query, key, value, g, beta, state, state_index, out_state, out)
+    o = op("deltanet_step")(query, key, value, g, beta, state, state_index, out_state, out)
     return o, out_state

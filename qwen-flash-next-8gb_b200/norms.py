@@ -5,7 +5,7 @@ qfn_norm_residual).
 RMSNorm here is x * rsqrt(mean(x^2) + eps) * weight, computed in fp32; every
 output is rounded once.  Both are forward only.
 """
-from _lib import ops
+from _lib import op
 
 
 def gated_rms_norm(x, z, weight, eps=1e-6):
@@ -18,10 +18,10 @@ def gated_rms_norm(x, z, weight, eps=1e-6):
         raise ValueError(f"x and z must have the same shape of two or more dimensions, got {tuple(x.shape)}, "
                          f"{tuple(z.shape)}")
     if x.dim() == 2:
-        return ops().gated_norm(x[:, None], z[:, None], weight, eps)[:, 0]
+        return op("gated_norm")(x[:, None], z[:, None], weight, eps)[:, 0]
     if x.dim() == 3:
-        return ops().gated_norm(x, z, weight, eps)
-    return ops().gated_norm(x.flatten(0, -3), z.flatten(0, -3), weight, eps).view(x.shape)
+        return op("gated_norm")(x, z, weight, eps)
+    return op("gated_norm")(x.flatten(0, -3), z.flatten(0, -3), weight, eps).view(x.shape)
 
 
 def norm_residual(block, residual, post_weight=None, gate=None, scale=1.0, next_weight=None, eps=1e-6,
@@ -37,5 +37,5 @@ def norm_residual(block, residual, post_weight=None, gate=None, scale=1.0, next_
     type, n bf16.  n is formed from r before its rounding.  out: where r goes, residual itself included."""
     if gate is not None and gate.dim() == 1:
         gate = gate[:, None]
-    r, n = ops().norm_residual(block, residual, post_weight, gate, sigmoid, scale, next_weight, eps, out)
+    r, n = op("norm_residual")(block, residual, post_weight, gate, sigmoid, scale, next_weight, eps, out)
     return r, (None if next_weight is None else n)
