@@ -277,7 +277,15 @@ int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t
  *   Bounds that do not rise: no row is written and every final state is NaN.
  *   state_in: f32[n_seqs][n_heads][dk][dv] or NULL (zeros); state_out: the
  *   same shape, state_in itself or an array that does not overlap it; both
- *   16-byte aligned.  dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.
+ *   16-byte aligned; out 4-byte aligned.  dk in {64, 128, 256}; dv % 32 == 0,
+ *   dv <= 4096.  q, k and v are read in 16-byte pieces where their bases and
+ *   strides allow it, else element by element.
+ *   dk <= 128 and more than 8 tokens run 64 tokens at a time on the tensor
+ *   cores (two launches for each segment of the workspace); others token by
+ *   token.  Both hold S and every sum in fp32; g is the log of the decay, and
+ *   -inf clears the state.  Results do not depend on the other sequences'
+ *   contents; they differ in their last bits between calls of few and of many
+ *   states, which run different kernels.
  *   workspace: device scratch of qfn_deltanet_chunk_workspace(...) bytes,
  *   256-byte aligned (may be NULL where that is 0).  Calls that can overlap
  *   on the device need workspaces of their own.

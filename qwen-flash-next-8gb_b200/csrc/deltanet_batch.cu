@@ -285,8 +285,7 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
   int rc = dn_rows_check(what, q, k, v, g, beta, strides, state_in, state_out, out, tokens, n_seqs, n_heads,
                          n_key_heads, dk, dv, &a);
   if (rc) return rc;
-  QFN_REQUIRE(n_seqs >= 0 && tokens >= 0 && (n_seqs > 0 || tokens == 0) &&
-                  (cu_seqlens || n_seqs == 0 || tokens % n_seqs == 0),
+  QFN_REQUIRE(n_seqs >= 0 && tokens >= 0 && (cu_seqlens || (n_seqs == 0 ? tokens == 0 : tokens % n_seqs == 0)),
               QFN_ERR_INVALID_ARG, "%s: tokens=%lld, n_seqs=%lld (equal lengths without cu_seqlens)", what,
               static_cast<long long>(tokens), static_cast<long long>(n_seqs));
   QFN_REQUIRE(!states_clash(state_in, state_out, n_seqs * n_heads * dk * dv), QFN_ERR_INVALID_ARG,
@@ -305,7 +304,7 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
   DeviceInfo* dev;
   rc = current_device(&dev);
   if (rc) return rc;
-  if (chunked) return dn_chunk(a, cu_seqlens, n_seqs, tokens, dk, dev->sm_count, workspace, stream);
+  if (chunked) return dn_chunk(a, cu_seqlens, n_seqs, tokens, dk, *dev, workspace, stream);
   const int64_t blocks = n_seqs * n_heads * (dv / kDbCols);
   auto kernel = dk == 64 ? deltanet_recurrence_kernel<64>
                          : dk == 128 ? deltanet_recurrence_kernel<128> : deltanet_recurrence_kernel<256>;

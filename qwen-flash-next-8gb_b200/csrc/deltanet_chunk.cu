@@ -18,6 +18,8 @@
 // terms (22 bits) after a power-of-two scale taken from its largest element;
 // k and q rows are bf16 and exact in f16 after theirs.  The products that
 // only reach the bf16 output (P d and S^T q) take one term.
+#include <atomic>
+
 #include "deltanet_chunk.cuh"
 #include "deltanet_chunk_parts.cuh"
 #include "deltanet_walk_quad.cuh"
@@ -424,11 +426,12 @@ bool quad_walk(int64_t states, int dv, int sms) {
 }
 
 template <int DK>
-int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, int sms, void* workspace, qfn_stream_t stream) {
+int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, const DeviceInfo& dev, void* workspace,
+        qfn_stream_t stream) {
   constexpr const char* what = "qfn_deltanet_chunk";
   const int key_heads = a.heads / a.ratio;
   const int64_t slots = tokens / C + n_seqs, seg = segment_slots(n_seqs, slots, a.heads, key_heads, DK);
-  const bool quad = quad_walk(n_seqs * a.heads, a.dv, sms);
+  const bool quad = quad_walk(n_seqs * a.heads, a.dv, dev.sm_count);
   const int cols = quad ? kQuadCols : kWarpCols;
   const int64_t blocks = n_seqs * a.heads * ((a.dv + cols - 1) / cols);
   QFN_REQUIRE(blocks <= 0x7fffffff && seg * key_heads <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many sequences",
@@ -440,11 +443,18 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, int 
   const bool v_vec = even(a.v, a.v_row, a.v_head);
   auto walk = quad ? dn_walk_quad_kernel<DK> : dn_walk_warp_kernel<DK>;
   const size_t walk_smem = quad ? sizeof(QuadSmem<DK>) : sizeof(WarpSmem<DK>);
-  cudaError_t e = cudaFuncSetAttribute(dn_prep_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       sizeof(PrepSmem<DK>));
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(walk, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(walk_smem));
-  if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  // the kernels' shared memory, once for each device
+  static std::atomic<uint64_t> prepared{0};
+  const uint64_t bit = uint64_t{1} << dev.device;
+  cudaError_t e = cudaSuccess;
+  if (!(prepared.load(std::memory_order_acquire) & bit)) {
+    const cudaFuncAttribute smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    e = cudaFuncSetAttribute(dn_prep_kernel<DK>, smem, sizeof(PrepSmem<DK>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(dn_walk_quad_kernel<DK>, smem, sizeof(QuadSmem<DK>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(dn_walk_warp_kernel<DK>, smem, sizeof(WarpSmem<DK>));
+    if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+    prepared.fetch_or(bit, std::memory_order_release);
+  }
   const Plan plan{cu, n_seqs, tokens};
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const Work work{ws, ws + seg * key_heads * (2 * C * DK * 2)};
@@ -469,10 +479,10 @@ size_t dn_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key
   return static_cast<size_t>(segment_slots(n_seqs, slots, n_heads, n_key_heads, dk) * slot_bytes(n_heads, n_key_heads, dk));
 }
 
-int dn_chunk(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, int dk, int sms, void* workspace,
-             qfn_stream_t stream) {
-  return dk == 64 ? run<64>(a, cu, n_seqs, tokens, sms, workspace, stream)
-                  : run<128>(a, cu, n_seqs, tokens, sms, workspace, stream);
+int dn_chunk(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, int dk, const DeviceInfo& dev,
+             void* workspace, qfn_stream_t stream) {
+  return dk == 64 ? run<64>(a, cu, n_seqs, tokens, dev, workspace, stream)
+                  : run<128>(a, cu, n_seqs, tokens, dev, workspace, stream);
 }
 
 int dn_chunk_status(unsigned int* v, bool clear) {

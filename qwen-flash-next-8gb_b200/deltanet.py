@@ -69,22 +69,7 @@ def chunk_gated_delta_rule(query, key, value, g, beta, initial_state=None, cu_se
     initial_state [N, H, dk, dv] fp32 (None: zeros).  final_state and out may be
     given to be written; final_state may be initial_state itself.  Views with any
     row and head strides are taken as they are."""
-    if query.dim() != 4:
-        raise ValueError(f"query must be [B, T, heads, dk], got {tuple(query.shape)}")
-    B, T = query.shape[:2]
-    if cu_seqlens is not None and B != 1:
-        raise ValueError(f"cu_seqlens takes one batch row holding every sequence, got {B}")
-    for name, t, dim in (("key", key, 4), ("value", value, 4), ("g", g, 3), ("beta", beta, 3)):
-        if t.dim() != dim or t.shape[:2] != (B, T):
-            raise ValueError(f"{name} must be [{B}, {T}, ...] with {dim} dimensions, got {tuple(t.shape)}")
-    if out is not None:
-        if tuple(out.shape) != (B, T) + tuple(value.shape[2:]) or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous [{B}, {T}, {value.shape[2]}, {value.shape[3]}], "
-                             f"got {tuple(out.shape)}")
-        out = out.view(B * T, *out.shape[2:])
-    o, S = op("deltanet_chunk")(query.flatten(0, 1), key.flatten(0, 1), value.flatten(0, 1), g.flatten(0, 1),
-                                beta.flatten(0, 1), B, cu_seqlens, initial_state, final_state, out)
-    return o.view(B, T, *o.shape[1:]), S
+    return op("deltanet_chunk")(query, key, value, g, beta, cu_seqlens, initial_state, final_state, out)
 
 
 def step_gated_delta_rule(query, key, value, g, beta, state, state_index=None, out_state=None, out=None):

@@ -184,40 +184,58 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   return x < y + (nb + 1) * b.element_size() && y < x + (na + 1) * a.element_size();
 }
 
-// q, k [R, Hq, dk], v [R, H, dv], g, beta [R, H] of the batched delta rule: views of any row and head stride whose
-// last dimension is dense (others are copied).
+// One operand of the batched delta rule as rows: [.., heads(, d)] after one or two leading dimensions that
+// count as one.  Views are taken as they are if their last dimension is dense and their leading ones can be
+// counted as one; others are copied.
+struct DeltaOperand {
+  at::Tensor t;
+  int64_t row, head;
+  DeltaOperand(const at::Tensor& x, int lead, bool vectors) : t(x) {
+    const int64_t d = lead + 1;   // the vectors' dimension
+    const bool dense = !vectors || t.stride(d) == 1;
+    const bool merge = lead == 1 || t.size(0) <= 1 || t.size(1) <= 1 || t.stride(0) == t.size(1) * t.stride(1);
+    if (!dense || !merge) t = t.contiguous();
+    row = lead == 2 && t.size(1) <= 1 && t.size(0) > 1 ? t.stride(0) : t.stride(lead - 1);
+    head = t.stride(lead);
+  }
+};
+
+// q, k [.., Hq, dk], v [.., H, dv], g, beta [.., H] with the same one or two leading dimensions.
 struct DeltaRows {
-  at::Tensor q, k, v, g, beta;
-  int64_t strides[10];
+  const at::Tensor& q_;
+  int lead;
+  int64_t rows;
   int H, Hq, dk, dv;
-  DeltaRows(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& g_,
-            const at::Tensor& beta_)
-      : q(q_), k(k_), v(v_), g(g_), beta(beta_) {
+  DeltaOperand q, k, v, g, beta;
+  int64_t strides[10];
+  static const at::Tensor& checked(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
+                                   const at::Tensor& beta, int lead) {
+    TORCH_CHECK_VALUE(q.dim() == lead + 2, "query must be [", lead == 2 ? "B, T, " : "R, ", "heads, dk], got ", q.sizes());
+    TORCH_CHECK_VALUE(k.sizes() == q.sizes(), "key must have query's shape ", q.sizes(), ", got ", k.sizes());
+    TORCH_CHECK_VALUE(v.dim() == lead + 2 && v.sizes().slice(0, lead) == q.sizes().slice(0, lead) && q.size(lead) >= 1 &&
+                          v.size(lead) >= 1 && v.size(lead) % q.size(lead) == 0,
+                      "value must be ", q.sizes().slice(0, lead), " x a multiple of query's ", q.size(lead),
+                      " heads x dv, got ", v.sizes());
+    TORCH_CHECK_VALUE(g.dim() == lead + 1 && g.sizes() == v.sizes().slice(0, lead + 1), "g must be ",
+                      v.sizes().slice(0, lead + 1), ", got ", g.sizes());
+    TORCH_CHECK_VALUE(beta.sizes() == g.sizes(), "beta must be ", g.sizes(), ", got ", beta.sizes());
     req_view(q, "query", at::kBFloat16, q, "query");
     req_view(k, "key", at::kBFloat16, q, "query");
     req_view(v, "value", at::kBFloat16, q, "query");
     req_view(g, "g", at::kFloat, q, "query");
     req_view(beta, "beta", at::kBFloat16, q, "query");
-    TORCH_CHECK_VALUE(q.dim() == 3 && k.sizes() == q.sizes(),
-                      "query and key must have the same shape, with heads and dk last; got ", q_.sizes(), ", ",
-                      k_.sizes());
-    const int64_t R = q.size(0);
-    TORCH_CHECK_VALUE(v.dim() == 3 && v.size(0) == R && q.size(1) >= 1 && v.size(1) >= 1 && v.size(1) % q.size(1) == 0,
-                      "value must hold a multiple of query's ", q.size(1), " heads for its ", R, " tokens; got ",
-                      v_.sizes());
-    TORCH_CHECK_VALUE(g.dim() == 2 && g.size(0) == R && g.size(1) == v.size(1) && beta.sizes() == g.sizes(),
-                      "g and beta must hold ", R, " x ", v.size(1), " values; got ", g_.sizes(), ", ", beta_.sizes());
-    if (q.stride(2) != 1) q = q.contiguous();
-    if (k.stride(2) != 1) k = k.contiguous();
-    if (v.stride(2) != 1) v = v.contiguous();
-    H = static_cast<int>(v.size(1));
-    Hq = static_cast<int>(q.size(1));
-    dk = static_cast<int>(q.size(2));
-    dv = static_cast<int>(v.size(2));
-    const at::Tensor* all[] = {&q, &k, &v, &g, &beta};
+    return q;
+  }
+  DeltaRows(const at::Tensor& q0, const at::Tensor& k0, const at::Tensor& v0, const at::Tensor& g0,
+            const at::Tensor& beta0, int lead_)
+      : q_(checked(q0, k0, v0, g0, beta0, lead_)), lead(lead_), rows(lead == 2 ? q0.size(0) * q0.size(1) : q0.size(0)),
+        H(static_cast<int>(v0.size(lead))), Hq(static_cast<int>(q0.size(lead))), dk(static_cast<int>(q0.size(lead + 1))),
+        dv(static_cast<int>(v0.size(lead + 1))), q(q0, lead, true), k(k0, lead, true), v(v0, lead, true),
+        g(g0, lead, false), beta(beta0, lead, false) {
+    const DeltaOperand* all[] = {&q, &k, &v, &g, &beta};
     for (int i = 0; i < 5; ++i) {
-      strides[2 * i] = all[i]->stride(0);
-      strides[2 * i + 1] = all[i]->stride(1);
+      strides[2 * i] = all[i]->row;
+      strides[2 * i + 1] = all[i]->head;
     }
   }
 };
@@ -225,33 +243,36 @@ struct DeltaRows {
 const uint16_t* u16(const at::Tensor& t) { return static_cast<const uint16_t*>(t.data_ptr()); }
 
 void req_state(const at::Tensor& S, const char* name, int64_t n, const DeltaRows& r) {
-  req_view(S, name, at::kFloat, r.q, "query");
+  req_view(S, name, at::kFloat, r.q_, "query");
   TORCH_CHECK_VALUE(S.dim() == 4 && (n < 0 || S.size(0) == n) && S.size(1) == r.H && S.size(2) == r.dk &&
                         S.size(3) == r.dv && S.is_contiguous(),
                     name, " must be a contiguous fp32 [", n < 0 ? std::string("slots") : std::to_string(n), ", ", r.H, ", ",
                     r.dk, ", ", r.dv, "], got ", S.sizes());
 }
 
-at::Tensor req_out(const std::optional<at::Tensor>& out, const DeltaRows& r) {
-  if (!out) return at::empty({r.q.size(0), r.H, r.dv}, r.q.options());
-  req_view(*out, "out", at::kBFloat16, r.q, "query");
-  TORCH_CHECK_VALUE(out->is_contiguous() && out->dim() == 3 && out->size(0) == r.q.size(0) && out->size(1) == r.H &&
-                        out->size(2) == r.dv,
-                    "out must be a contiguous bf16 [..., ", r.q.size(0), ", ", r.H, ", ", r.dv, "], got ", out->sizes());
-  TORCH_CHECK_VALUE(!overlap(*out, r.q) && !overlap(*out, r.k) && !overlap(*out, r.v) && !overlap(*out, r.g) &&
-                        !overlap(*out, r.beta),
+at::Tensor req_out(const std::optional<at::Tensor>& out, const at::Tensor& value, const DeltaRows& r) {
+  if (!out) return at::empty(value.sizes(), r.q_.options());
+  req_view(*out, "out", at::kBFloat16, r.q_, "query");
+  TORCH_CHECK_VALUE(out->is_contiguous() && out->sizes() == value.sizes(), "out must be a contiguous ", value.sizes(),
+                    ", got ", out->sizes());
+  TORCH_CHECK_VALUE(!overlap(*out, r.q.t) && !overlap(*out, r.k.t) && !overlap(*out, r.v.t) && !overlap(*out, r.g.t) &&
+                        !overlap(*out, r.beta.t),
                     "out overlaps an input");
   return *out;
 }
 
-// Rows are the tokens of all sequences; n_seqs sequences of equal length, or those of cu_seqlens.
+// query, key [B, T, Hq, dk], value [B, T, H, dv], g, beta [B, T, H]: B sequences, or (B = 1) those of cu_seqlens.
 std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                  const at::Tensor& g, const at::Tensor& beta, int64_t n_seqs,
+                                                  const at::Tensor& g, const at::Tensor& beta,
                                                   const std::optional<at::Tensor>& cu,
                                                   const std::optional<at::Tensor>& s_in,
                                                   const std::optional<at::Tensor>& s_out,
                                                   const std::optional<at::Tensor>& out_) {
-  const DeltaRows r(q, k, v, g, beta);
+  TORCH_CHECK_VALUE(!cu || (q.dim() == 4 && q.size(0) == 1),
+                    "cu_seqlens takes one batch row holding every sequence, got query ", q.sizes());
+  TORCH_CHECK_VALUE(!out_ || out_->sizes() == v.sizes(), "out must be a contiguous ", v.sizes());
+  const DeltaRows r(q, k, v, g, beta, 2);
+  int64_t n_seqs = q.size(0);
   if (cu) {
     req_cuda(*cu, "cu_seqlens");
     req_type(*cu, "cu_seqlens", at::kInt);
@@ -263,14 +284,13 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
   if (s_in) req_state(*s_in, "initial_state", n_seqs, r);
   if (s_out) req_state(*s_out, "final_state", n_seqs, r);
   c10::cuda::CUDAGuard guard(q.device());
-  const int64_t R = q.size(0);
-  at::Tensor out = req_out(out_, r);
+  at::Tensor out = req_out(out_, v, r);
   at::Tensor S = s_out ? *s_out : at::empty({n_seqs, r.H, r.dk, r.dv}, g.options());
-  const size_t nbytes = qfn_deltanet_chunk_workspace(R, n_seqs, r.H, r.Hq, r.dk, r.dv);
+  const size_t nbytes = qfn_deltanet_chunk_workspace(r.rows, n_seqs, r.H, r.Hq, r.dk, r.dv);
   at::Tensor ws;
   if (nbytes) ws = at::empty({static_cast<int64_t>(nbytes)}, q.options().dtype(at::kByte));
-  check_rc(qfn_deltanet_chunk(u16(r.q), u16(r.k), u16(r.v), r.g.data_ptr<float>(), u16(r.beta), r.strides,
-                              cu ? cu->data_ptr<int32_t>() : nullptr, n_seqs, R,
+  check_rc(qfn_deltanet_chunk(u16(r.q.t), u16(r.k.t), u16(r.v.t), r.g.t.data_ptr<float>(), u16(r.beta.t), r.strides,
+                              cu ? cu->data_ptr<int32_t>() : nullptr, n_seqs, r.rows,
                               s_in ? s_in->data_ptr<float>() : nullptr, S.data_ptr<float>(),
                               static_cast<uint16_t*>(out.data_ptr()), r.H, r.Hq, r.dk, r.dv,
                               nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(q)),
@@ -281,8 +301,8 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
 at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
                          const at::Tensor& beta, const at::Tensor& state, const std::optional<at::Tensor>& index,
                          at::Tensor out_state, const std::optional<at::Tensor>& out_) {
-  const DeltaRows r(q, k, v, g, beta);
-  const int64_t R = q.size(0);
+  const DeltaRows r(q, k, v, g, beta, 1);
+  const int64_t R = r.rows;
   req_state(state, "state", -1, r);
   req_state(out_state, "out_state", state.size(0), r);
   TORCH_CHECK_VALUE(R == 0 || state.size(0) >= 1, "state has no slots");
@@ -296,9 +316,9 @@ at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Ten
   TORCH_CHECK_VALUE(index || R <= state.size(0), "state has ", state.size(0), " slots for ", R,
                     " tokens (pass state_index)");
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = req_out(out_, r);
+  at::Tensor out = req_out(out_, v, r);
   if (R == 0) return out;
-  check_rc(qfn_deltanet_step_batch(u16(r.q), u16(r.k), u16(r.v), r.g.data_ptr<float>(), u16(r.beta), r.strides,
+  check_rc(qfn_deltanet_step_batch(u16(r.q.t), u16(r.k.t), u16(r.v.t), r.g.t.data_ptr<float>(), u16(r.beta.t), r.strides,
                                    index ? index->data_ptr<int32_t>() : nullptr, state.size(0),
                                    state.data_ptr<float>(), out_state.data_ptr<float>(),
                                    static_cast<uint16_t*>(out.data_ptr()), R, r.H, r.Hq, r.dk, r.dv, stream_of(q)),
@@ -398,7 +418,7 @@ TORCH_LIBRARY(qfn, m) {
   m.def("moe_prefill(Tensor x, Tensor ti, Tensor tv, Tensor table, Tensor s2, int L) -> Tensor", &moe_prefill);
   m.def("gemv(Tensor q, Tensor s, Tensor x, bool out_f32) -> Tensor", &gemv);
   m.def("linear(Tensor x, Tensor q, Tensor s) -> Tensor", &linear);
-  m.def("deltanet_chunk(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, int n_seqs, Tensor? cu_seqlens, "
+  m.def("deltanet_chunk(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? cu_seqlens, "
         "Tensor? initial_state, Tensor(a!)? final_state, Tensor(b!)? out) -> (Tensor, Tensor)",
         &deltanet_chunk);
   m.def("deltanet_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor state, Tensor? state_index, "

@@ -245,6 +245,7 @@ def test_chunk_equal_batch_and_pieces(T):
 
 @pytest.mark.parametrize("T", [12, 90])
 def test_chunk_leaves_rows_outside_the_sequences(T):
+    """(Padded tokens before, between the last sequence and the end.)"""
     H, Hk, dk, dv = 2, 2, 64, 32
     q, k, v, g, beta = inputs(T, H, Hk, dk, dv, seed=2)
     for t in (q, k, v, g, beta):   # nothing outside may be read either
@@ -279,6 +280,12 @@ def test_chunk_nothing_to_do():
     assert S.shape == (0, H, dk, dv)
     out, S = deltanet.chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None])
     assert S.shape == (1, H, dk, dv) and (S == 0).all()
+    q, k, v, g, beta = inputs(70, H, 1, dk, dv, seed=2)   # rows of which no sequence is left
+    out = torch.full((1, 70, H, dv), 7.0, dtype=torch.bfloat16, device=DEV)
+    _, S = deltanet.chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], cu_seqlens=offsets([]), out=out)
+    assert S.shape == (0, H, dk, dv) and (out == 7).all()
+    _, S = deltanet.chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], S0, offsets([0, 0]), out=out)
+    assert torch.equal(S, S0) and (out == 7).all()
 
 
 def extreme(case, q, k, v, g, beta, S0):

@@ -41,7 +41,7 @@ def chunk(q=FAKE, cu=FAKE, n=2, T=100, s_in=FAKE, s_out=FAR, ws=FAR, bytes_=None
 
 def test_chunk_refusals():
     assert chunk(q=None) == 1 and chunk(s_out=None) == 1
-    assert chunk(n=-1) == 1 and chunk(T=-1) == 1 and chunk(n=0) == 1
+    assert chunk(n=-1) == 1 and chunk(T=-1) == 1 and chunk(n=0, cu=None) == 1
     assert chunk(cu=None, n=3) == 1               # 100 tokens are not three equal sequences
     assert chunk(Hk=3) == 1 and chunk(dk=32) == 4 and chunk(dv=48) == 4
     assert chunk(s_in=ODD) == 2
@@ -51,7 +51,7 @@ def test_chunk_refusals():
     assert need > 0 and chunk(bytes_=need - 1) == 5 and chunk(ws=None) == 5
     assert chunk(ws=ctypes.c_void_p(0x7f0000000010)) == 2
     assert _lib.lib().qfn_deltanet_chunk_workspace(100, 0, 4, 2, 128, 128) == 0
-    assert chunk(n=0, T=0) == 0 and chunk(n=0, T=0, q=None, s_out=None) == 0
+    assert chunk(n=0) == 0 and chunk(n=0, T=0) == 0 and chunk(n=0, T=0, q=None, s_out=None) == 0
 
 
 def test_gated_norm_refusals():
