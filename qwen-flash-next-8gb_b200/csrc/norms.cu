@@ -260,74 +260,120 @@ __global__ void __launch_bounds__(kPieceThreads, 2) norm_residual_piece_kernel(c
   }
 }
 
-// Other rows: CTA = one row; a thread holds PARTS pieces of WIDTH neighbouring elements
-// (8, or 1 where alignment or dim rule 16-byte pieces out), blockDim.x pieces apart.
+// Other rows: CTA = one row; a thread holds PARTS pieces of WIDTH neighbouring
+// elements, blockDim.x pieces apart: 8 where 16-byte pieces are possible
+// (dim > 4096), 2 or 1 where alignment or dim rule them out.  The type is
+// asked once for all of an operand's pieces, so that their loads go out together.
+template <int WIDTH, bool F32>
+__device__ __forceinline__ void load_piece(const void* p, int64_t i, float (&v)[WIDTH]) {
+  if constexpr (WIDTH == 8) {
+    load8(p, F32 ? QFN_DTYPE_F32 : QFN_DTYPE_BF16, i, v);
+  } else if constexpr (WIDTH == 2) {
+    if constexpr (F32) {
+      const float2 f = *reinterpret_cast<const float2*>(static_cast<const float*>(p) + i);
+      v[0] = f.x;
+      v[1] = f.y;
+    } else {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+      v[0] = __uint_as_float(u << 16);
+      v[1] = __uint_as_float(u & 0xffff0000u);
+    }
+  } else {
+    v[0] = load1(p, F32 ? QFN_DTYPE_F32 : QFN_DTYPE_BF16, i);
+  }
+}
+template <int WIDTH, int PARTS, bool F32>
+__device__ __forceinline__ void load_row_as(const void* p, int64_t base, int dim, float (&v)[PARTS][WIDTH]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * WIDTH;
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) v[k][j] = 0.f;
+    if (c < dim) load_piece<WIDTH, F32>(p, base + c, v[k]);
+  }
+}
 template <int WIDTH, int PARTS>
-__global__ void __launch_bounds__(1024) norm_residual_kernel(const NormResidual a) {
+__device__ __forceinline__ void load_row(const void* p, int dtype, int64_t base, int dim, float (&v)[PARTS][WIDTH]) {
+  if (dtype == QFN_DTYPE_F32) load_row_as<WIDTH, PARTS, true>(p, base, dim, v);
+  else load_row_as<WIDTH, PARTS, false>(p, base, dim, v);
+}
+template <int WIDTH, int PARTS, bool F32>
+__device__ __forceinline__ void store_row_as(void* p, int64_t base, int dim, const float (&v)[PARTS][WIDTH]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * WIDTH;
+    if (c >= dim) continue;
+    constexpr int dtype = F32 ? QFN_DTYPE_F32 : QFN_DTYPE_BF16;
+    if constexpr (WIDTH == 8) store8(p, dtype, base + c, v[k]);
+    else if constexpr (WIDTH == 2 && F32)
+      *reinterpret_cast<float2*>(static_cast<float*>(p) + base + c) = make_float2(v[k][0], v[k][1]);
+    else if constexpr (WIDTH == 2)
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + base + c) = pack2(v[k][0], v[k][1]);
+    else store1(p, dtype, base + c, v[k][0]);
+  }
+}
+
+template <int WIDTH, int PARTS, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_residual_kernel(const NormResidual a) {
+  // what is requested before the block's norm is known; the rest comes after it
+  constexpr bool kAhead = PARTS * WIDTH <= 16;
   __shared__ float red[2][32];
   pdl_wait();
   pdl_launch_dependents();
   const int64_t row = blockIdx.x;
-  float b[PARTS][WIDTH], ss = 0.f;
-#pragma unroll
-  for (int p = 0; p < PARTS; ++p) {
-    const int c = (p * blockDim.x + threadIdx.x) * WIDTH;
-    if (c < a.dim) {
-      if constexpr (WIDTH == 8) load8(a.block, a.block_dtype, row * a.block_row + c, b[p]);
-      else b[p][0] = load1(a.block, a.block_dtype, row * a.block_row + c);
-    } else {
-#pragma unroll
-      for (int j = 0; j < WIDTH; ++j) b[p][j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < WIDTH; ++j) ss = fmaf(b[p][j], b[p][j], ss);
+  float b[PARTS][WIDTH], r[PARTS][WIDTH], g[PARTS][WIDTH], ss = 0.f;
+  load_row(a.block, a.block_dtype, row * a.block_row, a.dim, b);
+  if constexpr (kAhead) {
+    load_row(a.residual, a.residual_dtype, row * a.residual_row, a.dim, r);
+    if (a.gate_kind == 2) load_row(a.gate, a.gate_dtype, row * a.gate_row, a.dim, g);
   }
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) ss = fmaf(b[k][j], b[k][j], ss);
   float m = a.scale;
   if (a.gate_kind == 1) {
-    const float g = load1(a.gate, a.gate_dtype, row * a.gate_row);
-    m *= a.sigmoid ? sigmoidf(g) : g;
+    const float x = load1(a.gate, a.gate_dtype, row * a.gate_row);
+    m *= a.sigmoid ? sigmoidf(x) : x;
   }
   if (a.w_post) m *= rsqrtf(block_sum(ss, red[0]) / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) b[k][j] *= m;
+  if (a.gate_kind == 2) {
+    if constexpr (!kAhead) load_row(a.gate, a.gate_dtype, row * a.gate_row, a.dim, g);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+      for (int j = 0; j < WIDTH; ++j) b[k][j] *= a.sigmoid ? sigmoidf(g[k][j]) : g[k][j];
+  }
+  if (a.w_post) {
+    load_row(a.w_post, a.post_dtype, 0, a.dim, g);
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+      for (int j = 0; j < WIDTH; ++j) b[k][j] *= g[k][j];
+  }
+  if constexpr (!kAhead) load_row(a.residual, a.residual_dtype, row * a.residual_row, a.dim, r);
   float s2 = 0.f;
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) {
-    const int c = (p * blockDim.x + threadIdx.x) * WIDTH;
-    if (c >= a.dim) continue;
-    float r[WIDTH], w[WIDTH], g[WIDTH];
-    if constexpr (WIDTH == 8) {
-      load8(a.residual, a.residual_dtype, row * a.residual_row + c, r);
-      if (a.w_post) load8(a.w_post, a.post_dtype, c, w);
-      if (a.gate_kind == 2) load8(a.gate, a.gate_dtype, row * a.gate_row + c, g);
-    } else {
-      r[0] = load1(a.residual, a.residual_dtype, row * a.residual_row + c);
-      if (a.w_post) w[0] = load1(a.w_post, a.post_dtype, c);
-      if (a.gate_kind == 2) g[0] = load1(a.gate, a.gate_dtype, row * a.gate_row + c);
-    }
+  for (int k = 0; k < PARTS; ++k)
 #pragma unroll
     for (int j = 0; j < WIDTH; ++j) {
-      float v = b[p][j] * m;
-      if (a.w_post) v *= w[j];
-      if (a.gate_kind == 2) v *= a.sigmoid ? sigmoidf(g[j]) : g[j];
-      b[p][j] = r[j] + v;
-      s2 = fmaf(b[p][j], b[p][j], s2);
+      b[k][j] += r[k][j];
+      s2 = fmaf(b[k][j], b[k][j], s2);
     }
-    if constexpr (WIDTH == 8) store8(a.r_out, a.residual_dtype, row * a.dim + c, b[p]);
-    else store1(a.r_out, a.residual_dtype, row * a.dim + c, b[p][0]);
-  }
+  if (a.residual_dtype == QFN_DTYPE_F32) store_row_as<WIDTH, PARTS, true>(a.r_out, row * a.dim, a.dim, b);
+  else store_row_as<WIDTH, PARTS, false>(a.r_out, row * a.dim, a.dim, b);
   if (!a.w_next) return;
   const float rn = rsqrtf(block_sum(s2, red[1]) / static_cast<float>(a.dim) + a.eps);
+  load_row(a.w_next, a.next_dtype, 0, a.dim, g);
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) {
-    const int c = (p * blockDim.x + threadIdx.x) * WIDTH;
-    if (c >= a.dim) continue;
-    float w[WIDTH];
-    if constexpr (WIDTH == 8) load8(a.w_next, a.next_dtype, c, w);
-    else w[0] = load1(a.w_next, a.next_dtype, c);
+  for (int k = 0; k < PARTS; ++k)
 #pragma unroll
-    for (int j = 0; j < WIDTH; ++j) w[j] *= b[p][j] * rn;
-    if constexpr (WIDTH == 8) store8(a.n_out, QFN_DTYPE_BF16, row * a.dim + c, w);
-    else store1(a.n_out, QFN_DTYPE_BF16, row * a.dim + c, w[0]);
-  }
+    for (int j = 0; j < WIDTH; ++j) g[k][j] *= b[k][j] * rn;
+  store_row_as<WIDTH, PARTS, false>(a.n_out, row * a.dim, a.dim, g);
 }
 
 namespace {
@@ -351,10 +397,13 @@ int launch(const char* what, Kernel kernel, int64_t blocks, int threads, qfn_str
 
 bool dtype_ok(int d) { return d == QFN_DTYPE_F32 || d == QFN_DTYPE_BF16; }
 
-// Whether rows of `dim` elements at p, row_a and row_b elements apart, can be moved 8 elements at a time.
+// Whether rows at p, row_a and row_b elements apart, can be moved 8 elements at a time (16 bytes), or two.
 bool wide(const void* p, int dtype, int64_t row_a, int64_t row_b) {
   return !p || (aligned(p, 16) && (row_a * (dtype == QFN_DTYPE_F32 ? 4 : 2)) % 16 == 0 &&
                 (row_b * (dtype == QFN_DTYPE_F32 ? 4 : 2)) % 16 == 0);
+}
+bool two(const void* p, int dtype, int64_t row) {
+  return !p || (aligned(p, dtype == QFN_DTYPE_F32 ? 8 : 4) && row % 2 == 0);
 }
 
 }  // namespace
@@ -427,13 +476,27 @@ extern "C" int qfn_norm_residual(const void* block, int block_dtype, int64_t blo
     const int64_t resident = static_cast<int64_t>(dev->sm_count) * (1024 / threads);
     return launch(what, kernel, rows < resident ? rows : resident, threads, stream, a, rows);
   }
-  const int parts = (pieces + 1023) / 1024;   // pieces of a thread
-  const int per = (pieces + parts - 1) / parts;
-  const int threads = (per + 31) / 32 * 32;
-  auto kernel = v ? (parts <= 1 ? norm_residual_kernel<8, 1> : parts <= 2 ? norm_residual_kernel<8, 2>
-                                                                          : norm_residual_kernel<8, 4>)
-                  : (parts <= 1 ? norm_residual_kernel<1, 1> : parts <= 4 ? norm_residual_kernel<1, 4>
-                                                             : parts <= 8 ? norm_residual_kernel<1, 8>
-                                                                          : norm_residual_kernel<1, 32>);
+  if (v) {
+    const int parts = (pieces + 1023) / 1024, per = (pieces + parts - 1) / parts;
+    auto kernel = parts <= 1 ? norm_residual_kernel<8, 1, 1024>
+                             : parts <= 2 ? norm_residual_kernel<8, 2, 1024> : norm_residual_kernel<8, 4, 1024>;
+    return launch(what, kernel, rows, (per + 31) / 32 * 32, stream, a);
+  }
+  const bool pairs = dim % 2 == 0 && two(block, block_dtype, block_row) && two(residual, residual_dtype, residual_row) &&
+                     two(w_post, post_dtype, 0) && (gate_kind != 2 || two(gate, gate_dtype, gate_row)) &&
+                     two(w_next, next_dtype, 0) && two(residual_out, residual_dtype, 0) && two(normed, QFN_DTYPE_BF16, 0);
+  const int n = pairs ? dim / 2 : dim;
+  // up to 512 threads with all of a row's pieces on their way at once; longer rows, 1024 threads in two steps
+  if (n <= 4096) {
+    const int parts = n <= 512 ? 2 : n <= 2048 ? 4 : 8;
+    const int threads = ((n + parts - 1) / parts + 31) / 32 * 32;
+    auto kernel = pairs ? (parts == 2 ? norm_residual_kernel<2, 2, 512> : parts == 4 ? norm_residual_kernel<2, 4, 512>
+                                                                                     : norm_residual_kernel<2, 8, 512>)
+                        : (parts == 2 ? norm_residual_kernel<1, 2, 512> : parts == 4 ? norm_residual_kernel<1, 4, 512>
+                                                                                     : norm_residual_kernel<1, 8, 512>);
+    return launch(what, kernel, rows, threads, stream, a);
+  }
+  const int parts1 = (dim + 1023) / 1024, threads = ((dim + parts1 - 1) / parts1 + 31) / 32 * 32;
+  auto kernel = parts1 <= 8 ? norm_residual_kernel<1, 8, 1024> : norm_residual_kernel<1, 32, 1024>;
   return launch(what, kernel, rows, threads, stream, a);
 }
