@@ -418,11 +418,12 @@ cudaError_t launch(Kernel kernel, int64_t blocks, int threads, size_t smem, cuda
 }
 
 // Which walk: the quads' for few states, the warps' for many.  Measured for a chunk of dk = 128: a block of 32
-// columns takes 2.6 us in the quads' walk; in the warps' one of 128 columns takes 6 us, of up to 64 3.8 us (one
-// warp to a scheduler).  Blocks come in rounds of one per SM.
+// columns takes 2.6 us in the quads' walk; in the warps' one of 64 columns takes 3.8 us, of 128 6 us.  Blocks
+// come in rounds of one per SM.
 bool quad_walk(int64_t states, int dv, int sms) {
-  const int64_t quads = states * (dv / kQuadCols), blocks = states * ((dv + kWarpCols - 1) / kWarpCols);
-  return (quads + sms - 1) / sms * 26 <= (blocks + sms - 1) / sms * (dv <= 64 ? 38 : 60);
+  auto rounds = [&](int cols) { return (states * ((dv + cols - 1) / cols) + sms - 1) / sms; };
+  const int64_t narrow = rounds(kWarpCols / 2) * 38, wide = rounds(kWarpCols) * 60;
+  return rounds(kQuadCols) * 26 <= (narrow < wide ? narrow : wide);
 }
 
 template <int DK>
@@ -432,7 +433,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
   const int key_heads = a.heads / a.ratio;
   const int64_t slots = tokens / C + n_seqs, seg = segment_slots(n_seqs, slots, a.heads, key_heads, DK);
   const bool quad = quad_walk(n_seqs * a.heads, a.dv, dev.sm_count);
-  const int cols = quad ? kQuadCols : kWarpCols;
+  const int cols = quad ? kQuadCols : kWarpCols / 2;
   const int64_t blocks = n_seqs * a.heads * ((a.dv + cols - 1) / cols);
   QFN_REQUIRE(blocks <= 0x7fffffff && seg * key_heads <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many sequences",
               what);
@@ -441,8 +442,6 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
   };
   const bool kq_vec = even(a.q, a.q_row, a.q_head) && even(a.k, a.k_row, a.k_head);
   const bool v_vec = even(a.v, a.v_row, a.v_head);
-  auto walk = quad ? dn_walk_quad_kernel<DK> : dn_walk_warp_kernel<DK>;
-  const size_t walk_smem = quad ? sizeof(QuadSmem<DK>) : sizeof(WarpSmem<DK>);
   // the kernels' shared memory, once for each device
   static std::atomic<uint64_t> prepared{0};
   const uint64_t bit = uint64_t{1} << dev.device;
@@ -463,8 +462,10 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
     e = launch(dn_prep_kernel<DK>, (s1 - s0) * key_heads, kPrepThreads, sizeof(PrepSmem<DK>), as_stream(stream), a, plan,
                work, s0, kq_vec);
     if (e == cudaSuccess)
-      e = launch(walk, blocks, quad ? kQuadThreads : kWarpThreads, walk_smem, as_stream(stream), a, plan, work, s0, s1,
-                 v_vec);
+      e = quad ? launch(dn_walk_quad_kernel<DK>, blocks, kQuadThreads, sizeof(QuadSmem<DK>), as_stream(stream), a, plan,
+                        work, s0, s1, v_vec)
+               : launch(dn_walk_warp_kernel<DK>, blocks, kWarpThreads, sizeof(WarpSmem<DK>), as_stream(stream), a, plan,
+                        work, s0, s1, v_vec, dev.sm_count);
   }
   if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
   return check_launch(what);

@@ -1,5 +1,5 @@
-// The walk for many sequences (deltanet_chunk.cu): a block takes 128 columns of
-// a head's S, a warp 16 of them on its own.
+// The walk for many sequences (deltanet_chunk.cu): a block takes 64 or 128
+// columns of a head's S, a warp 16 of them on its own.
 #pragma once
 
 #include "deltanet_chunk_parts.cuh"
@@ -44,15 +44,34 @@ __device__ __forceinline__ void spoil(float (&d)[8][4], int bad0, int bad1, floa
 // warps of the block read from shared memory.
 template <int DK>
 __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnRows a, const Plan plan, const Work work,
-                                                                       int64_t slot0, int64_t slot1, bool vec) {
+                                                                       int64_t slot0, int64_t slot1, bool vec, int sms) {
   constexpr int kStages = kWarpStages, kVRow = kWarpCols * 2;
   extern __shared__ __align__(1024) unsigned char raw[];
   WarpSmem<DK>& sm = *reinterpret_cast<WarpSmem<DK>*>(raw);
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int cb = (a.dv + kWarpCols - 1) / kWarpCols;
-  const int c0 = static_cast<int>(blockIdx.x % cb) * kWarpCols;
+  const int cb = (a.dv + kWarpCols / 2 - 1) / (kWarpCols / 2);
+  const int c0 = static_cast<int>(blockIdx.x % cb) * (kWarpCols / 2);
   const int h = static_cast<int>(blockIdx.x / cb % a.heads);
-  const int warps = min(kWarpCols / 16, (a.dv - c0) / 16);   // those with columns
+  pdl_wait();
+  const Part part = choose(plan, blockIdx.x / cb / a.heads, slot0, slot1, sm.length, &sm.seq);
+  if (part.none(slot1)) return;
+  const int64_t seq = part.seq, begin = part.begin, len = part.len, base = part.base, first = part.first, last = part.last;
+  const bool ok = part.ok;
+  const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
+
+  // Four warps have a scheduler each and walk a chunk in 3.8 us, eight in 6.  Blocks have 128 columns, and every
+  // second block of 64 none, but for sequences that would take longer so than their share of all SMs' time, where
+  // these are few enough for all their blocks of 64 columns to run at once.
+  bool wide = true;
+  if (plan.n_seqs <= kSorted && ok) {
+    const int64_t all = (slot1 - slot0) * a.heads * ((cb + 1) / 2);
+    const int64_t sequences = plan.cu ? __syncthreads_count(tid < plan.n_seqs && (sm.length[tid] + C - 1) / C *
+                                                                                    static_cast<int64_t>(sms) > all)
+                                      : plan.n_seqs;
+    wide = static_cast<int64_t>(n) * sms <= all || sequences * a.heads * cb > sms;
+  }
+  if (wide && (c0 & (kWarpCols / 2))) return;
+  const int warps = min(wide ? kWarpCols / 16 : kWarpCols / 32, (a.dv - c0) / 16);   // those with columns
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&sm.full[i], 1 + warps * 32);   // the bulk copies' bytes, the lanes' copies of v
@@ -60,12 +79,7 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
     }
     fence_mbar_init();
   }
-  pdl_wait();
-  const Part part = choose(plan, blockIdx.x / cb / a.heads, slot0, slot1, sm.length, &sm.seq);
-  if (part.none(slot1)) return;
-  const int64_t seq = part.seq, begin = part.begin, len = part.len, base = part.base, first = part.first, last = part.last;
-  const bool ok = part.ok;
-  const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
+  __syncthreads();
 
   if (w < warps) {
     constexpr int NT = DK / 8, KT = DK / 16;
