@@ -280,14 +280,15 @@ int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t
  *   16-byte aligned; out 4-byte aligned.  dk in {64, 128, 256}; dv % 32 == 0,
  *   dv <= 4096.  q, k and v are read in 16-byte pieces where their bases and
  *   strides allow it, else element by element.
- *   dk <= 128 and more than 8 tokens run 64 tokens at a time on the tensor
- *   cores (two launches for each segment of the workspace); others token by
- *   token.  Both hold S and every sum in fp32; g is the log of the decay, and
+ *   dk <= 128 and more than 8 tokens (of each sequence without cu_seqlens, in
+ *   all with it) run 64 tokens at a time on the tensor cores (two launches for
+ *   each segment of the workspace); others token by token.  Both hold S and every sum in fp32; g is the log of the decay, and
  *   -inf clears the state.  Results do not depend on the other sequences'
  *   contents; they differ in their last bits between calls of few and of many
  *   states, which run different kernels.
  *   workspace: device scratch of qfn_deltanet_chunk_workspace(...) bytes,
- *   256-byte aligned (may be NULL where that is 0).  Calls that can overlap
+ *   256-byte aligned (may be NULL where that is 0, and where cu_seqlens is
+ *   NULL and it is 0 for one sequence of tokens / n_seqs tokens).  Calls that can overlap
  *   on the device need workspaces of their own.
  */
 size_t qfn_deltanet_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk, int dv);

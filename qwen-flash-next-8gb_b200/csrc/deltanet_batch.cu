@@ -293,7 +293,7 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
   QFN_REQUIRE(tokens < (int64_t{1} << 31) - 64, QFN_ERR_UNSUPPORTED, "%s: tokens=%lld", what,
               static_cast<long long>(tokens));
   if (n_seqs == 0) return QFN_OK;
-  const bool chunked = dn_chunk_takes(tokens, dk);
+  const bool chunked = dn_chunk_takes(cu_seqlens ? tokens : tokens / n_seqs, dk);
   if (chunked) {
     const size_t need = dn_chunk_workspace(tokens, n_seqs, n_heads, n_key_heads, dk);
     QFN_REQUIRE(workspace && workspace_bytes >= need, QFN_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what,

@@ -473,7 +473,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
 
 }  // namespace
 
-bool dn_chunk_takes(int64_t tokens, int dk) { return dk <= 128 && tokens > kRecurrenceTokens; }
+bool dn_chunk_takes(int64_t longest, int dk) { return dk <= 128 && longest > kRecurrenceTokens; }
 
 size_t dn_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk) {
   const int64_t slots = tokens / C + n_seqs;

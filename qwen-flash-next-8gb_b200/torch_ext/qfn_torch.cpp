@@ -286,7 +286,10 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = req_out(out_, v, r);
   at::Tensor S = s_out ? *s_out : at::empty({n_seqs, r.H, r.dk, r.dv}, g.options());
-  const size_t nbytes = qfn_deltanet_chunk_workspace(r.rows, n_seqs, r.H, r.Hq, r.dk, r.dv);
+  // equal sequences need no workspace where one of them alone needs none
+  const size_t nbytes = !cu && qfn_deltanet_chunk_workspace(q.size(1), 1, r.H, r.Hq, r.dk, r.dv) == 0
+                            ? 0
+                            : qfn_deltanet_chunk_workspace(r.rows, n_seqs, r.H, r.Hq, r.dk, r.dv);
   at::Tensor ws;
   if (nbytes) ws = at::empty({static_cast<int64_t>(nbytes)}, q.options().dtype(at::kByte));
   check_rc(qfn_deltanet_chunk(u16(r.q.t), u16(r.k.t), u16(r.v.t), r.g.t.data_ptr<float>(), u16(r.beta.t), r.strides,

@@ -243,6 +243,24 @@ def test_chunk_equal_batch_and_pieces(T):
         check(last[b][None], S[b], tuple(x[-1:] if i in (0, 2) else x for i, x in enumerate(ref)), T + 1)
 
 
+@pytest.mark.parametrize("H,Hk,dk,dv", HEADS)
+@pytest.mark.parametrize("N,T", [(3, 8), (20, 1), (20, 8), (20, 9)])
+def test_chunk_batch_of_short_sequences(N, T, H, Hk, dk, dv):
+    """Equal lengths on both sides of the token recurrence's longest; the bounds given as well."""
+    q, k, v, g, beta = (t.unflatten(0, (N, T)) for t in inputs(N * T, H, Hk, dk, dv, 31))
+    S0 = states(N, H, dk, dv, 31)
+    out, S = deltanet.chunk_gated_delta_rule(q, k, v, g, beta, S0)
+    flat = [t.flatten(0, 1)[None] for t in (q, k, v, g, beta)]
+    out_cu, S_cu = deltanet.chunk_gated_delta_rule(*flat, S0, offsets([T] * N))
+    for n in range(N):
+        ref = oracle(q[n], k[n], v[n], g[n], beta[n], S0[n])
+        check(out[n], S[n], ref, T)
+        check(out_cu[0, n * T:(n + 1) * T], S_cu[n], ref, T)
+    carried = S0.clone()
+    deltanet.chunk_gated_delta_rule(q, k, v, g, beta, carried, final_state=carried)
+    assert torch.equal(carried, S)
+
+
 @pytest.mark.parametrize("T", [12, 90])
 def test_chunk_leaves_rows_outside_the_sequences(T):
     """(Padded tokens before, between the last sequence and the end.)"""
