@@ -9,7 +9,7 @@
 // Both are bound by memory: a row is read once, held in registers as fp32
 // through its sums, and written once.  n is formed from r' before its
 // rounding, so each output carries one rounding.  Rows whose bases, strides and length allow it move
-// in 16-byte pieces of 8 elements (two for fp32); the others go element by element.
+// in 16-byte pieces of 8 elements (two for fp32); the others go by two elements or one.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -87,6 +87,7 @@ struct GatedNorm {
 
 // LANES lanes of a warp share one row of dim <= 8 LANES; a thread takes its
 // piece of ROWS rows, one block's worth apart, and requests all of them first.
+// Measured: 16384 x 32 rows of 128 in 70 to 74 us, 5.4 to 5.8 TB/s (issue slots 70 %).
 template <int LANES, int ROWS>
 __global__ void __launch_bounds__(256) gated_norm_kernel(const GatedNorm a) {
   constexpr int kPer = 256 / LANES;   // rows of a block at a time
@@ -173,7 +174,9 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // Rows of one 8-element piece a thread (dim <= 8 x 512).  A CTA takes row after
 // row, gridDim.x apart, and requests the next row's block, residual and gate
 // while this one's sums are formed, so that two barriers a row leave no gap
-// in the stream of loads.  F32 flags: the operands' types.
+// in the stream of loads.  F32 flags: the operands' types; read at run time they
+// spilled registers (184 us).  Measured: 16384 rows of 2560 bf16 in 77 to 82 us,
+// 5.1 to 5.4 TB/s.
 constexpr int kPieceThreads = 512;
 
 template <bool F32>
