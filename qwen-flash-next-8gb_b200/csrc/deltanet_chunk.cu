@@ -19,10 +19,10 @@
 // k and q rows are bf16 and exact in f16 after theirs.  The products that
 // only reach the bf16 output (P d and S^T q) take one term.
 //
-// What bounds it: not the bytes (2048 tokens of 32 heads of 128 x 128 take 133 us,
-// their bytes 10.6) but the preparation's instructions (46 us on its own: 19,500
-// warp instructions a block, 45 % of the issue slots) and the walk's chain of
-// chunks.  Chunks of 64 keep that chain short and T invertible in one block; token
+// What bounds it: not the bytes (2048 tokens of 32 heads of 128 x 128 take 131 us,
+// their bytes 10.6) but the preparation's latency and instructions (44 us on its
+// own: 19,400 warp instructions a block, 47 % of the issue slots) and the walk's
+// chain of chunks.  Chunks of 64 keep that chain short and T invertible in one block; token
 // by token the same call takes 3.6 ms.
 #include <atomic>
 
@@ -52,16 +52,38 @@ struct PrepSmem {
   float p_scale;
 };
 
-// The inverse of I + A, A strictly lower triangular in t, in fp32: the two 32 x 32 halves of the
-// diagonal by substitution, a column per lane, then T21 = -T22 (A21 T11) by the whole block.
+// Four neighbouring sums over k < N of row[k] m[k][0 .. 3], in fp32.  LOWER: only k <= r, the part of a lower
+// triangular row r that is not zero (zeros would let a NaN of a later row into this one).
+template <int N, bool LOWER>
+__device__ __forceinline__ float4 row_product(const float* row, const float* m, int pitch, int r) {
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < N; k += 4) {
+    const float4 av = *reinterpret_cast<const float4*>(row + k);
+    const float ak[4] = {av.x, av.y, av.z, av.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 b = *reinterpret_cast<const float4*>(m + (k + i) * pitch);
+      if (!LOWER || k + i <= r) {
+        y.x = fmaf(ak[i], b.x, y.x); y.y = fmaf(ak[i], b.y, y.y); y.z = fmaf(ak[i], b.z, y.z); y.w = fmaf(ak[i], b.w, y.w);
+      }
+    }
+  }
+  return y;
+}
+
+// The inverse of I + A, A strictly lower triangular in t, in fp32: the four 16 x 16 blocks of the diagonal by
+// substitution, a column per lane, then T21 = -T22 (A21 T11) twice, for the two 32 x 32 halves and for the whole.
+// 4,400 of the block's 14,600 cycles where it has an SM to itself; two blocks of 32 and one merge take 7,200.
 template <int DK>
 __device__ __forceinline__ void invert(PrepSmem<DK>& sm) {
-  const int tid = threadIdx.x, w = tid >> 5, c = tid & 31;
-  if (w < 2) {
-    float* t = sm.t + w * 32 * (kGS + 1);
-    float x[32];
+  const int tid = threadIdx.x;
+  if (tid < 64) {
+    const int c = tid & 15;
+    float* t = sm.t + (tid >> 4) * 16 * (kGS + 1);
+    float x[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 16; ++i) {
       float s[4] = {i == c ? 1.f : 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < i; j += 4) {
@@ -75,29 +97,26 @@ __device__ __forceinline__ void invert(PrepSmem<DK>& sm) {
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) t[i * kGS + c] = x[i];
+    for (int i = 0; i < 16; ++i) t[i * kGS + c] = x[i];
   }
   __syncthreads();
-  // a thread: row r, columns c4 .. c4 + 3
-  const int r = tid >> 3, c4 = (tid & 7) * 4;
-  auto product = [&](const float* row, const float* m, int pitch) {
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-    for (int k = 0; k < 32; k += 4) {
-      const float4 av = *reinterpret_cast<const float4*>(row + k);
-      const float ak[4] = {av.x, av.y, av.z, av.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 b = *reinterpret_cast<const float4*>(m + (k + i) * pitch + c4);
-        y.x = fmaf(ak[i], b.x, y.x); y.y = fmaf(ak[i], b.y, y.y); y.z = fmaf(ak[i], b.z, y.z); y.w = fmaf(ak[i], b.w, y.w);
-      }
+  {   // half p: a thread of the first 128 has row r, columns c4 .. c4 + 3
+    const int p = (tid >> 6) & 1, r = (tid >> 2) & 15, c4 = (tid & 3) * 4;
+    float* t = sm.t + p * 32 * (kGS + 1);
+    float* y = sm.y + p * 16 * 20;
+    if (tid < 128) *reinterpret_cast<float4*>(&y[r * 20 + c4]) = row_product<16, false>(t + (16 + r) * kGS, t + c4, kGS, r);
+    __syncthreads();
+    if (tid < 128) {
+      const float4 v = row_product<16, true>(t + (16 + r) * kGS + 16, y + c4, 20, r);
+      *reinterpret_cast<float4*>(&t[(16 + r) * kGS + c4]) = make_float4(-v.x, -v.y, -v.z, -v.w);
     }
-    return y;
-  };
-  *reinterpret_cast<float4*>(&sm.y[r * 36 + c4]) = product(sm.t + (32 + r) * kGS, sm.t, kGS);
+    __syncthreads();
+  }
+  const int r = tid >> 3, c4 = (tid & 7) * 4;
+  *reinterpret_cast<float4*>(&sm.y[r * 36 + c4]) = row_product<32, false>(sm.t + (32 + r) * kGS, sm.t + c4, kGS, r);
   __syncthreads();
-  const float4 y = product(sm.t + (32 + r) * kGS + 32, sm.y, 36);
-  *reinterpret_cast<float4*>(&sm.t[(32 + r) * kGS + c4]) = make_float4(-y.x, -y.y, -y.z, -y.w);
+  const float4 v = row_product<32, true>(sm.t + (32 + r) * kGS + 32, sm.y + c4, 36, r);
+  *reinterpret_cast<float4*>(&sm.t[(32 + r) * kGS + c4]) = make_float4(-v.x, -v.y, -v.z, -v.w);
   __syncthreads();
 }
 
@@ -181,13 +200,27 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
     n = count - 1;
     if (n < 0 || !dn_plan_ok(plan.cu, plan.n_seqs, plan.tokens)) return;
   } else {
-    n = min(slot * C / (plan.tokens / plan.n_seqs + C), plan.n_seqs - 1);
+    n = plan.n_seqs == 1 ? 0 : min(slot * C / (plan.each + C), plan.n_seqs - 1);
     while (n + 1 < plan.n_seqs && plan.slot(n + 1) <= slot) ++n;
   }
   const int64_t t0 = plan.begin(n) + (slot - plan.slot(n)) * C;
   const int cnt = static_cast<int>(min(static_cast<int64_t>(C), plan.end(n) - t0));
   if (cnt <= 0) return;
 
+  // g and beta of tokens 2 lane and 2 lane + 1 for warp 0's running sum, a head ahead of it
+  float gv[2] = {0.f, 0.f};
+  uint16_t bv[2] = {0, 0};
+  auto request = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 2 * lane + i;
+      if (w == 0 && r < cnt) {
+        gv[i] = a.g[(t0 + r) * a.g_row + h * a.g_head];
+        bv[i] = a.beta[(t0 + r) * a.b_row + h * a.b_head];
+      }
+    }
+  };
+  request(hk * a.ratio);
   // k and q rows: a warp takes four rows at a time, eight of each in all
   {
     const uint16_t* src[2] = {a.k + hk * a.k_head + (lane & 7) * (DK / 8), a.q + hk * a.q_head + (lane & 7) * (DK / 8)};
@@ -247,12 +280,11 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
       float bt[2], rise = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = 2 * lane + i;
-        const float gv = r < cnt ? a.g[(t0 + r) * a.g_row + h * a.g_head] : 0.f;
-        rise += fmaxf(gv, 0.f);
-        s[i] = gv < -200.f ? -200.f : gv;
-        bt[i] = r < cnt ? bf16_bits_to_f32(a.beta[(t0 + r) * a.b_row + h * a.b_head]) : 0.f;
+        rise += fmaxf(gv[i], 0.f);
+        s[i] = gv[i] < -200.f ? -200.f : gv[i];
+        bt[i] = bf16_bits_to_f32(bv[i]);
       }
+      if (hv + 1 < a.ratio) request(h + 1);
       double run = s[0] + s[1];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -460,7 +492,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
     if (e != cudaSuccess) return set_error(QFN_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
     prepared.fetch_or(bit, std::memory_order_release);
   }
-  const Plan plan{cu, n_seqs, tokens};
+  const Plan plan{cu, n_seqs, tokens, cu ? 0 : tokens / n_seqs};
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const Work work{ws, ws + seg * key_heads * (2 * C * DK * 2)};
   for (int64_t s0 = 0; s0 < slots && e == cudaSuccess; s0 += seg) {

@@ -32,9 +32,9 @@ struct Work {
 // sequences never meet: cu / 64 rises by at least chunks - 1 per sequence.
 struct Plan {
   const int32_t* cu;
-  int64_t n_seqs, tokens;
-  __device__ int64_t begin(int64_t n) const { return cu ? cu[n] : n * (tokens / n_seqs); }
-  __device__ int64_t end(int64_t n) const { return cu ? cu[n + 1] : (n + 1) * (tokens / n_seqs); }
+  int64_t n_seqs, tokens, each;   // each: without cu, tokens / n_seqs (a 64-bit division takes a block hundreds of cycles)
+  __device__ int64_t begin(int64_t n) const { return cu ? cu[n] : n * each; }
+  __device__ int64_t end(int64_t n) const { return cu ? cu[n + 1] : (n + 1) * each; }
   __device__ int64_t slot(int64_t n) const { return begin(n) / C + n; }
 };
 

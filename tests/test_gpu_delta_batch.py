@@ -365,6 +365,24 @@ def test_chunk_nan_stays_in_its_sequence_and_column(T):
     check(zero(out[0, :T], keep), zero(S[0], keep[:, None]), (zero(r_out, keep), zero(r_S, keep[:, None]), mag, top), T)
 
 
+@pytest.mark.parametrize("n_seqs", [1, 40])
+@pytest.mark.parametrize("at", [3, 20, 40, 55, 70])
+def test_chunk_nan_key_leaves_earlier_tokens(at, n_seqs):
+    """A key that is not a number spoils its head from its token on, never the tokens before it."""
+    H, Hk, dk, dv, T = 4, 4, 128, 128, 130
+    q, k, v, g, beta = (t.unflatten(0, (n_seqs, T)) for t in inputs(n_seqs * T, H, Hk, dk, dv, 17))
+    k = k.clone()
+    k[0, at, 1, 5] = float("nan")
+    out, S = deltanet.chunk_gated_delta_rule(q, k, v, g, beta)
+    assert out[0, at:, 1].isnan().all() and S[0, 1].isnan().all()
+    ref_out, _, mag, top = oracle(*(t[0, :at] for t in (q, k, v, g, beta)), None)
+    tol = 2.0 ** -8 * ref_out.abs() + 2.0 ** -10 * mag + 2 * (U * (16 + 4 * math.sqrt(T)) * top)[:, None]
+    assert ((out[0, :at].double() - ref_out).abs() <= tol).all()
+    others = [0, 2, 3]
+    ref = oracle(*(t[0][:, others] for t in (q, k, v, g, beta)), None)
+    check(out[0][:, others], S[0, others], ref, T)
+
+
 def test_chunk_repeats_bit_for_bit_on_another_stream_and_in_a_graph():
     lens, H, Hk, dk, dv = [70, 3, 129], 4, 2, 128, 64
     stream_and_graph(lens, H, Hk, dk, dv, (lens, [1, 200, 1], [0, 0, 202]))
