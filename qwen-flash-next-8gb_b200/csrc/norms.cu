@@ -87,7 +87,7 @@ struct GatedNorm {
 
 // LANES lanes of a warp share one row of dim <= 8 LANES; a thread takes its
 // piece of ROWS rows, one block's worth apart, and requests all of them first.
-// Measured: 16384 x 32 rows of 128 in 70 to 74 us, 5.4 to 5.8 TB/s (issue slots 70 %).
+// Measured: 16384 x 32 rows of 128 in 70 to 75 us, 5.4 to 5.8 TB/s (issue slots 70 %).
 template <int LANES, int ROWS>
 __global__ void __launch_bounds__(256) gated_norm_kernel(const GatedNorm a) {
   constexpr int kPer = 256 / LANES;   // rows of a block at a time
@@ -175,7 +175,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // row, gridDim.x apart, and requests the next row's block, residual and gate
 // while this one's sums are formed, so that two barriers a row leave no gap
 // in the stream of loads.  F32 flags: the operands' types; read at run time they
-// spilled registers (184 us).  Measured: 16384 rows of 2560 bf16 in 77 to 82 us,
+// spilled registers (184 us).  Measured: 16384 rows of 2560 bf16 in 77 to 83 us,
 // 5.1 to 5.4 TB/s.
 constexpr int kPieceThreads = 512;
 
