@@ -282,10 +282,14 @@ int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t
  *   strides allow it, else element by element.
  *   dk <= 128 and more than 8 tokens (of each sequence without cu_seqlens, in
  *   all with it) run 64 tokens at a time on the tensor cores (two launches for
- *   each segment of the workspace); others token by token.  Both hold S and every sum in fp32; g is the log of the decay, and
- *   -inf clears the state.  Results do not depend on the other sequences'
- *   contents; they differ in their last bits between calls of few and of many
- *   states, which run different kernels.
+ *   each segment of the workspace); others token by token.  Both hold S and
+ *   every sum in fp32.  The chunks' products take bf16 terms of their operands,
+ *   each with fp32's range: three (24 bits) of all that S is made of, two (16 bits)
+ *   of what only reaches out.  g is the log of the decay, and -inf clears a
+ *   finite state; where g rises, its sum stays below 88 within any 64 tokens.
+ *   Rows of q and k have norms below 2^63.  Results do not depend on the other
+ *   sequences' contents; they differ in their last bits between calls of few and
+ *   of many states, which run different kernels.
  *   workspace: device scratch of qfn_deltanet_chunk_workspace(...) bytes,
  *   256-byte aligned (may be NULL where that is 0, and where cu_seqlens is
  *   NULL and it is 0 for one sequence of tokens / n_seqs tokens).  Calls that can overlap

@@ -9,15 +9,18 @@
 //   S'   = e^{G_64} S + sum_j e^{G_64 - G_j} k_j d_j^T
 //
 // Two kernels.  dn_prep_kernel does everything that does not need the state,
-// a block per (chunk, key head): k and q as f16 rows, T, P and the decays of
-// each token.  A walk over a sequence's chunks follows, with S in registers:
+// a block per (chunk, key head): k and q as rows, T, P and the decays of each
+// token.  A walk over a sequence's chunks follows, with S in registers:
 // dn_walk_quad_kernel for few sequences, dn_walk_warp_kernel for many.
 //
-// Precision.  S leaves as fp32, so its factors need more than f16's 11 bits:
-// every operand of an S or d product that is not exact is split into two f16
-// terms (22 bits) after a power-of-two scale from a bound on its largest element;
-// k and q rows are bf16 and exact in f16 after theirs.  The products that
-// only reach the bf16 output (P d and S^T q) take one term.
+// Precision.  S, d and R are fp32 sums, and the tensor cores take them, and T,
+// as three bf16 terms (24 bits, fp32's range): products of a three-term operand
+// with k are exact, T R leaves out what is below 2^-24 of its terms.  k and q rows
+// are bf16 as they come; their norms' reciprocals are in the tokens' factors.  The
+// products that only reach the bf16 output, P d and S^T q, take two terms of P, d
+// and S: 2^-16 before a rounding to 2^-9.
+// (Before, one power-of-two scale and two f16 terms served 16 columns and 64
+// tokens: values 2^-20 of the largest there lost their digits.)
 //
 // What bounds it: not the bytes (2048 tokens of 32 heads of 128 x 128 take 131 us,
 // their bytes 10.6) but the preparation's latency and instructions (44 us on its
@@ -39,17 +42,15 @@ template <int DK>
 struct PrepSmem {
   union {
     struct {
-      unsigned char k[C * DK * 2], q[C * DK * 2];   // f16 rows, swizzled
+      unsigned char k[C * DK * 2], q[C * DK * 2];   // bf16 rows, swizzled
     };
     struct {
       float t[C * kGS];     // A, then T
       float y[32 * 36];     // A21 T11
     };
   };
-  float gk[C * kGS], gq[C * kGS];   // k_i . k_j, q_i . k_j of the scaled rows
-  float g_hi[C], g_lo[C], ck[C], cq[C], beta[C], w[C];
-  uint32_t red[3][kPrepThreads / 32];
-  float p_scale;
+  float gk[C * kGS], gq[C * kGS];   // k_i . k_j, q_i . k_j of the rows as they are
+  float g_hi[C], g_lo[C], ck[C], cq[C], beta[C];
 };
 
 // Four neighbouring sums over k < N of row[k] m[k][0 .. 3], in fp32.  LOWER: only k <= r, the part of a lower
@@ -138,46 +139,40 @@ __device__ __forceinline__ void load_row(const uint16_t* p, bool in, bool vec, u
   }
 }
 
-// Eight lanes hold a bf16 row of q or k: as f16 after a power-of-two scale 2^e (bf16 is exact in f16 then) to
-// shared memory and to the workspace, both swizzled; the row's factor (1 / norm) 2^-e.
+// Eight lanes hold a bf16 row of q or k: to shared memory and to the workspace, both swizzled; the row's factor.
 template <int DK>
-__device__ __forceinline__ void f16_row(const uint4 (&x)[DK / 64], unsigned char* tile, unsigned char* copy, int row,
-                                        float* factor, float divide) {
+__device__ __forceinline__ void keep_row(const uint4 (&x)[DK / 64], unsigned char* tile, unsigned char* copy, int row,
+                                         float* factor, float divide) {
   const int part = threadIdx.x & 7;
-  constexpr int N = DK / 8;
-  float v[N], ss[2] = {0.f, 0.f}, m[2] = {0.f, 0.f};
+  float ss[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < DK / 64; ++i) {
     const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[i * 8 + 2 * j] = __uint_as_float(u[j] << 16);
-      v[i * 8 + 2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+      const float lo = __uint_as_float(u[j] << 16), hi = __uint_as_float(u[j] & 0xffff0000u);
+      ss[0] = fmaf(lo, lo, ss[0]);
+      ss[1] = fmaf(hi, hi, ss[1]);
     }
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    ss[i & 1] = fmaf(v[i], v[i], ss[i & 1]);
-    m[i & 1] = fmaxf(m[i & 1], fabsf(v[i]));
-  }
-  float s = ss[0] + ss[1], mm = fmaxf(m[0], m[1]);
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  }
-  const int e = scale_exp(__float_as_uint(mm));
-  const float sc = exp2i(e);
-#pragma unroll
-  for (int i = 0; i < DK / 64; ++i) {
-    const uint4 h = make_uint4(pack_h2(v[i * 8] * sc, v[i * 8 + 1] * sc), pack_h2(v[i * 8 + 2] * sc, v[i * 8 + 3] * sc),
-                               pack_h2(v[i * 8 + 4] * sc, v[i * 8 + 5] * sc), pack_h2(v[i * 8 + 6] * sc, v[i * 8 + 7] * sc));
     const uint32_t at = swz<DK * 2>(row, part * (DK / 64) + i);
-    *reinterpret_cast<uint4*>(tile + at) = h;
-    *reinterpret_cast<uint4*>(copy + at) = h;
+    *reinterpret_cast<uint4*>(tile + at) = x[i];
+    *reinterpret_cast<uint4*>(copy + at) = x[i];
   }
-  // a row of zeros counts for nothing: its factor, up to 1000, would take the others' digits
-  if (part == 0) *factor = s == 0.f ? 0.f : rsqrtf(s + 1e-6f) / divide * exp2i(-e);
+  float s = ss[0] + ss[1];
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (part == 0) *factor = rsqrtf(s + 1e-6f) / divide;
+}
+
+// Eight neighbouring values of a row as N terms, a matrix apart.
+template <int N>
+__device__ __forceinline__ void store_terms(const float (&v)[8], unsigned char* dst) {
+  uint32_t u[4][N];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(v[2 * i], v[2 * i + 1], u[i]);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    *reinterpret_cast<uint4*>(dst + n * kTermBytes) = make_uint4(u[0][n], u[1][n], u[2][n], u[3][n]);
 }
 
 template <int DK>
@@ -235,8 +230,8 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = w * 8 + (i & 1) * 4 + (lane >> 3);
-      f16_row<DK>(x[i], i < 2 ? sm.k : sm.q, copy + (i < 2 ? 0 : C * DK * 2), r, i < 2 ? &sm.ck[r] : &sm.cq[r],
-                  i < 2 ? 1.f : a.q_scale);
+      keep_row<DK>(x[i], i < 2 ? sm.k : sm.q, copy + (i < 2 ? 0 : C * DK * 2), r, i < 2 ? &sm.ck[r] : &sm.cq[r],
+                   i < 2 ? 1.f : a.q_scale);
     }
   }
   __syncthreads();
@@ -272,15 +267,14 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
   for (int hv = 0; hv < a.ratio; ++hv) {
     const int h = hk * a.ratio + hv;
     unsigned char* dst = work.heads + ((slot - slot0) * a.heads + h) * static_cast<int64_t>(kHeadBytes);
-    float* factors = reinterpret_cast<float*>(dst + 2 * kMat);
+    float* factors = reinterpret_cast<float*>(dst + 3 * kTermBytes);
     // Running sum of g in 64 bits, kept as two floats: differences of far tokens' sums keep their
     // digits.  exp(-200) is 0 in fp32, and a finite sum keeps exp(G_i - G_j) a number.
     if (w == 0) {
       double s[2];
-      float bt[2], rise = 0.f;
+      float bt[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        rise += fmaxf(gv[i], 0.f);
         s[i] = gv[i] < -200.f ? -200.f : gv[i];
         bt[i] = bf16_bits_to_f32(bv[i]);
       }
@@ -291,8 +285,6 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         const double up = __shfl_up_sync(0xffffffffu, run, o);
         if (lane >= o) run += up;
       }
-      rise = warp_sum(rise);
-      float bmax = 0.f;
       const double G[2] = {run - s[1], run};
       const double last = __shfl_sync(0xffffffffu, run, 31);
 #pragma unroll
@@ -302,36 +294,24 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         sm.g_hi[r] = hi;
         sm.g_lo[r] = static_cast<float>(G[i] - hi);
         sm.beta[r] = bt[i];
-        const float eg = expf(hi), wt = expf(static_cast<float>(last - G[i])) * sm.ck[r];
-        sm.w[r] = wt;
-        bmax = fmaxf(bmax, fabsf(bt[i]) * eg);
+        const float eg = expf(hi);
         factors[kFA + r] = -bt[i] * eg * sm.ck[r];
         factors[kFB + r] = bt[i];
         factors[kFQ + r] = eg * sm.cq[r];
-        factors[kFW + r] = wt;
+        factors[kFW + r] = expf(static_cast<float>(last - G[i])) * sm.ck[r];
       }
-      bmax = __uint_as_float(__reduce_max_sync(0xffffffffu, finite_bits(bmax)));
-      if (lane == 0) {
-        factors[kFEnd + 5] = bmax;
-        // |q_i . k_j| <= 1 / q_scale after the norms, and no decay is above the sum of the rises
-        const float bound = expf(rise) / a.q_scale * 1.01f;
-        const int e = bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
-        sm.p_scale = exp2i(e);
-        factors[kFEnd] = expf(static_cast<float>(last));
-        factors[kFEnd + 2] = exp2i(-e);
-      }
+      if (lane == 0) factors[kFEnd] = expf(static_cast<float>(last));
     }
     __syncthreads();
     // A into t and P out: eight columns j0 .. j0 + 7 a warp, a row per lane
     const int j0 = w * 8;
     {
-      const float psc = sm.p_scale;
 #pragma unroll 1
       for (int s = 0; s < 2; ++s) {
         const int i = s * 32 + lane;
         float av[8], pv[8];
         if (j0 < (s + 1) * 32) {
-          const float gh = sm.g_hi[i], gl = sm.g_lo[i], bi = sm.beta[i] * sm.ck[i], qi = sm.cq[i] * psc;
+          const float gh = sm.g_hi[i], gl = sm.g_lo[i], bi = sm.beta[i] * sm.ck[i], qi = sm.cq[i];
 #pragma unroll
           for (int j4 = 0; j4 < 8; j4 += 4) {
             const float4 h4 = *reinterpret_cast<const float4*>(&sm.g_hi[j0 + j4]);
@@ -346,8 +326,8 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
             for (int j = 0; j < 4; ++j) {
               const int jj = j0 + j4 + j;
               const float f = expf((gh - hj[j]) + (gl - lj[j])) * cj[j];
-              pv[j4 + j] = jj <= i ? f * qi * qj[j] : 0.f;
-              av[j4 + j] = jj < i ? f * bi * kj[j] : 0.f;
+              pv[j4 + j] = jj <= i ? qj[j] * qi * f : 0.f;
+              av[j4 + j] = jj < i ? kj[j] * bi * f : 0.f;
             }
           }
         } else {
@@ -356,69 +336,29 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         }
         *reinterpret_cast<float4*>(&sm.t[i * kGS + j0]) = make_float4(av[0], av[1], av[2], av[3]);
         *reinterpret_cast<float4*>(&sm.t[i * kGS + j0 + 4]) = make_float4(av[4], av[5], av[6], av[7]);
-        *reinterpret_cast<uint4*>(dst + kRecBytes + swz<128>(i, w)) =
-            make_uint4(pack_h2(pv[0], pv[1]), pack_h2(pv[2], pv[3]), pack_h2(pv[4], pv[5]), pack_h2(pv[6], pv[7]));
+        if (w / 2 <= i / 16) store_terms<2>(pv, dst + kRecBytes + tri_at(i, w));
       }
     }
     __syncthreads();
     invert(sm);
-    // T's scale, and a bound of the weighted d for the walk: the largest row sum of w |T| (eight lanes a row)
-    float tv[2][8];
-    uint32_t tm = 0, wm = 0, top = 0;
+    // T's terms, eight lanes a row
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int i = s * 32 + (tid >> 3), jt = (tid & 7) * 8;
-      float sum = 0.f;
+      if (jt / 16 > i / 16) continue;
+      float tv[8];
 #pragma unroll
       for (int j4 = 0; j4 < 8; j4 += 4) {
         const float4 v = *reinterpret_cast<const float4*>(&sm.t[i * kGS + jt + j4]);
-        tv[s][j4] = v.x; tv[s][j4 + 1] = v.y; tv[s][j4 + 2] = v.z; tv[s][j4 + 3] = v.w;
+        tv[j4] = v.x; tv[j4 + 1] = v.y; tv[j4 + 2] = v.z; tv[j4 + 3] = v.w;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (jt + j > i) tv[s][j] = 0.f;
-        const uint32_t b = finite_bits(tv[s][j]);
-        tm = max(tm, b);
-        sum += __uint_as_float(b);
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      wm = max(wm, finite_bits(sum * sm.w[i]));
-      top = max(top, finite_bits(sum));
+      for (int j = 0; j < 8; ++j)
+        if (jt + j > i) tv[j] = 0.f;
+      store_terms<3>(tv, dst + tri_at(i, tid & 7));
     }
-    tm = __reduce_max_sync(0xffffffffu, tm);
-    wm = __reduce_max_sync(0xffffffffu, wm);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) {
-      sm.red[0][w] = tm;
-      sm.red[1][w] = wm;
-      sm.red[2][w] = top;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPrepThreads / 32; ++i) {
-      tm = max(tm, sm.red[0][i]);
-      wm = max(wm, sm.red[1][i]);
-      top = max(top, sm.red[2][i]);
-    }
-    const int et = scale_exp(tm);
-    const float sc = exp2i(et);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) split2(tv[s][2 * j] * sc, tv[s][2 * j + 1] * sc, hi[j], lo[j]);
-      const uint32_t at = swz<128>(s * 32 + (tid >> 3), tid & 7);
-      *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(dst + kMat + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    if (tid == 0) {
-      factors[kFEnd + 1] = exp2i(-et);
-      factors[kFEnd + 3] = __uint_as_float(wm) * 1.0001f;   // the sum's own rounding
-      factors[kFEnd + 4] = __uint_as_float(top) * 1.0001f;
-    }
-    // the next head's factors overwrite this one's only after every thread has passed the barrier above,
-    // its A only after the next one
+    // the next head's sums and decays are written after every thread has read this one's (the inverse's barriers),
+    // its A after the barrier behind them
   }
 }
 
@@ -455,13 +395,14 @@ cudaError_t launch(Kernel kernel, int64_t blocks, int threads, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Which walk: the quads' for few states, the warps' for many.  Measured for a chunk of dk = 128: a block of 32
-// columns takes 2.6 us in the quads' walk; in the warps' one of 64 columns takes 3.9 us, of 128 5.9 us.  Blocks
-// come in rounds of one per SM.
+// Which walk: the quads' for few states, the warps' for many.  Blocks come in rounds of one per SM, and a chunk of
+// a block takes, in 0.1 us (one head, from 2048 to 6144 tokens): 32 columns in the quads' walk 29 for dk = 128 and
+// 23 for dk = 64, 64 columns in the warps' 50 and 36, 128 columns 78 and 54.
+template <int DK>
 bool quad_walk(int64_t states, int dv, int sms) {
   auto rounds = [&](int cols) { return (states * ((dv + cols - 1) / cols) + sms - 1) / sms; };
-  const int64_t narrow = rounds(kWarpCols / 2) * 38, wide = rounds(kWarpCols) * 60;
-  return rounds(kQuadCols) * 26 <= (narrow < wide ? narrow : wide);
+  const int64_t narrow = rounds(kWarpCols / 2) * (DK == 128 ? 50 : 36), wide = rounds(kWarpCols) * (DK == 128 ? 78 : 54);
+  return rounds(kQuadCols) * (DK == 128 ? 29 : 23) <= (narrow < wide ? narrow : wide);
 }
 
 template <int DK>
@@ -470,7 +411,7 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
   constexpr const char* what = "qfn_deltanet_chunk";
   const int key_heads = a.heads / a.ratio;
   const int64_t slots = tokens / C + n_seqs, seg = segment_slots(n_seqs, slots, a.heads, key_heads, DK);
-  const bool quad = quad_walk(n_seqs * a.heads, a.dv, dev.sm_count);
+  const bool quad = quad_walk<DK>(n_seqs * a.heads, a.dv, dev.sm_count);
   const int cols = quad ? kQuadCols : kWarpCols / 2;
   const int64_t blocks = n_seqs * a.heads * ((a.dv + cols - 1) / cols);
   QFN_REQUIRE(blocks <= 0x7fffffff && seg * key_heads <= 0x7fffffff, QFN_ERR_UNSUPPORTED, "%s: too many sequences",

@@ -1,5 +1,5 @@
-// What the kernels of deltanet_chunk.cu share: the workspace's layout, scales
-// and f16 terms, fragments, the sequences' plan.
+// What the kernels of deltanet_chunk.cu share: the workspace's layout, bf16
+// terms, fragments, the sequences' plan.
 #pragma once
 
 #include "deltanet_batch.cuh"
@@ -12,19 +12,27 @@ constexpr int kSorted = 64;      // sequences up to which the longest are walked
 constexpr int kPrepThreads = 256;
 constexpr int kGS = 68;          // row pitch of the 64 x 64 fp32 matrices of dn_prep_kernel
 
-// Per chunk and value head: T hi, T lo (f16, 128-byte rows, swizzled), the
-// tokens' factors and the chunk's scales, then P (as T).
-constexpr int kMat = C * C * 2;
-enum { kFA = 0, kFB = C, kFQ = 2 * C, kFW = 3 * C, kFEnd = 4 * C };   // -beta e^G ck, beta, e^G cq, e^(G64 - G) ck
-// + e^G64, scale of T, scale of P, largest row sums of e^(G64 - G) ck |T| and of |T|, largest |beta| e^G
-constexpr int kFactors = 4 * C + 8;
-constexpr int kRecBytes = 2 * kMat + kFactors * 4;
-constexpr int kHeadBytes = kRecBytes + kMat;
+// Lower triangular 64 x 64 matrices (T, P) are kept as their 10 blocks of 16 x 16
+// on and below the diagonal, each term by itself: a block is its four 8 x 8
+// quarters, rows of 16 bytes, so that a warp's ldmatrix of a block reads 512
+// bytes in the lanes' order.
+constexpr int kBlockBytes = 512, kTermBytes = 10 * kBlockBytes;
+__host__ __device__ constexpr int tri_block(int i, int j) { return (i * (i + 1) / 2 + j) * kBlockBytes; }
+__device__ __forceinline__ uint32_t tri_at(int row, int col8) {   // the 16 bytes of row `row`, columns 8 col8 .. + 7
+  return tri_block(row >> 4, col8 >> 1) + ((row >> 3 & 1) * 2 + (col8 & 1)) * 128 + (row & 7) * 16;
+}
+
+// Per chunk and value head: T in three terms, the tokens' factors and e^G64, then P in two terms.
+enum { kFA = 0, kFB = C, kFQ = 2 * C, kFW = 3 * C, kFEnd = 4 * C };   // -beta e^G ck, beta, e^G cq, e^(G64 - G) ck; e^G64
+constexpr int kFactors = 4 * C + 4;
+constexpr int kRecBytes = 3 * kTermBytes + kFactors * 4;
+constexpr int kPBytes = 2 * kTermBytes;
+constexpr int kHeadBytes = kRecBytes + kPBytes;
 
 __device__ unsigned int g_dn_status;
 
 struct Work {
-  unsigned char* kq;     // [slots][key heads][2][64][dk] f16
+  unsigned char* kq;     // [slots][key heads][2][64][dk] bf16
   unsigned char* heads;  // [slots][heads][kHeadBytes]
 };
 
@@ -38,37 +46,34 @@ struct Plan {
   __device__ int64_t slot(int64_t n) const { return begin(n) / C + n; }
 };
 
-__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
-
-// Exponent e with max * 2^e in [2^14, 2^15); any value of max gives 2^e and 2^-e as normal numbers.
-__device__ __forceinline__ int scale_exp(uint32_t max_bits) {
-  const int ex = static_cast<int>(max_bits >> 23) - 126;   // max in [2^(ex-1), 2^ex)
-  return max_bits == 0 ? 0 : min(15 - ex, 120);
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-  return b >= 0x7f800000u ? 0u : b;
+// Two values less their bf16 roundings in u, exactly.
+__device__ __forceinline__ void less(float& a, float& b, uint32_t u) {
+  a -= __uint_as_float(u << 16);
+  b -= __uint_as_float(u & 0xffff0000u);
 }
 
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// Two values as sums of bf16 terms.  Three terms hold fp32's 24 bits: 8 each, and what two leave has no more
+// than 8 bits, so that its upper half is all of it.  A term has fp32's exponent, so no value needs a scale, and
+// none loses digits to a larger one beside it.  Two terms are within 2^-16.
+__device__ __forceinline__ void split(float a, float b, uint32_t (&u)[3]) {
+  u[0] = pack_bf2(a, b);
+  less(a, b, u[0]);
+  u[1] = pack_bf2(a, b);
+  less(a, b, u[1]);
+  u[2] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}
+__device__ __forceinline__ void split(float a, float b, uint32_t (&u)[2]) {
+  u[0] = pack_bf2(a, b);
+  less(a, b, u[0]);
+  u[1] = pack_bf2(a, b);
 }
 
-// Two values as f16 hi and lo pairs (each scaled before).
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = pack_h2(a - f.x, b - f.y);
-}
-
-// max(m, |a|, |b|), NaN dropped or kept
-__device__ __forceinline__ float max_abs(float m, float a, float b) {
-  asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
-  return m;
-}
+// max(m, |a|, |b|), NaN kept
 __device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
   asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
   return m;
@@ -77,13 +82,13 @@ __device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
 // D += A B and, for the first product of an accumulator, D = A B.  Not volatile: the compiler may
 // move the products between the loads.
 __device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
@@ -119,44 +124,29 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
   __syncwarp();
 }
 
-// max(m, magnitudes of a lane's values), NaN dropped.
+// Whether any of a warp's values is not finite.
 template <int N>
-__device__ __forceinline__ float lane_max(const float (&v)[N][4]) {
+__device__ __forceinline__ bool any_not_finite(const float (&v)[N][4]) {
   float m0 = 0.f, m1 = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    m0 = max_abs(m0, v[i][0], v[i][1]);
-    m1 = max_abs(m1, v[i][2], v[i][3]);
+    m0 = max_abs_nan(m0, v[i][0], v[i][1]);
+    m1 = max_abs_nan(m1, v[i][2], v[i][3]);
   }
-  return fmaxf(m0, m1);
+  return __any_sync(0xffffffffu, !(max_abs_nan(m0, m1, 0.f) < CUDART_INF_F));
 }
 
-// The largest finite magnitude of a warp's values, the same in every lane.
+// Accumulators of two neighbouring 16 x 8 tiles as the fragments of a 16 x 16 operand's N terms.
 template <int N>
-__device__ __forceinline__ float warp_max(const float (&v)[N][4]) {
-  uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(lane_max(v)));
-  if (b >= 0x7f800000u) {   // an infinity somewhere: the other columns keep their scale
-    b = 0;
+__device__ __forceinline__ void frag_split(const float (&a)[4], const float (&b)[4], uint32_t (&f)[N][4]) {
+  const float v[4][2] = {{a[0], a[1]}, {a[2], a[3]}, {b[0], b[1]}, {b[2], b[3]}};
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+  for (int i = 0; i < 4; ++i) {
+    uint32_t u[N];
+    split(v[i][0], v[i][1], u);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b = max(b, finite_bits(v[i][j]));
-    b = __reduce_max_sync(0xffffffffu, b);
+    for (int n = 0; n < N; ++n) f[n][i] = u[n];
   }
-  return __uint_as_float(b);
-}
-
-// Power-of-two scale for a bound; not finite: the smallest scale.
-__device__ __forceinline__ int bound_exp(float bound) {
-  return bound < 0x1p127f ? scale_exp(__float_as_uint(bound)) : -112;
-}
-
-// Accumulators of two neighbouring 16 x 8 tiles as the hi and lo fragments of a 16 x 16 operand.
-__device__ __forceinline__ void frag_split(const float (&a)[4], const float (&b)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-  split2(a[0], a[1], hi[0], lo[0]);
-  split2(a[2], a[3], hi[1], lo[1]);
-  split2(b[0], b[1], hi[2], lo[2]);
-  split2(b[2], b[3], hi[3], lo[3]);
 }
 
 // A block's part of a launch: chunks first .. last - 1 of a sequence.

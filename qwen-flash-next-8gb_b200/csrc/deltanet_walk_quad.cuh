@@ -5,10 +5,9 @@
 // the quarters' parts of S^T k, R, and d.  Four more warps form the outputs
 // behind them and copy the chunks to come.
 //
-// Bound by the chain of those exchanges: 2.6 us a chunk of dk = 128 (one head, slope
-// from 2048 to 6144 tokens), about 5,000 cycles with the tensor pipe busy 35 % and
-// 2,900 shared-memory wavefronts.  A warp per 16 columns (the walk for many
-// sequences) takes 3.9 us there.
+// Bound by the chain of those exchanges: 2.9 us a chunk of dk = 128, 2.3 of dk = 64
+// (one head, slope from 2048 to 6144 tokens).  A warp per 16 columns (the walk for
+// many sequences) takes 5.0 and 3.6 there.
 #pragma once
 
 #include "deltanet_chunk_parts.cuh"
@@ -17,36 +16,35 @@ namespace qfn {
 namespace {
 
 constexpr int kQuadCols = 32;            // state columns of a block
-constexpr int kQuadStages = 3;           // chunks of what the recurrence reads
+template <int DK>
+constexpr int kQuadStages = DK == 128 ? 2 : 3;   // chunks of what the recurrence reads: as many as fit
 constexpr int kQuadOutStages = 2;        // chunks of what only the outputs read
 constexpr int kQuadThreads = 12 * 32;    // 8 warps of the recurrence, 4 of the outputs and the copies
 
 template <int DK>
 struct QuadStage {
   unsigned char k[C * DK * 2];
-  unsigned char t_hi[kMat], t_lo[kMat];
+  unsigned char t[3 * kTermBytes];
   float f[kFactors];
   unsigned char v[C * kQuadCols * 2];
 };
 template <int DK>
 struct QuadOutStage {
-  unsigned char q[C * DK * 2], p[kMat];
+  unsigned char q[C * DK * 2], p[kPBytes];
 };
 
-// Fragments travel as 16 bytes per lane.
+// Fragments travel as 16 bytes per lane and term.
 template <int DK>
 struct QuadSmem {
-  QuadStage<DK> stage[kQuadStages];
+  QuadStage<DK> stage[kQuadStages<DK>];
   QuadOutStage<DK> out_stage[kQuadOutStages];
-  uint4 s_hi[2][2][4][DK / 64][32];   // [buffer][columns][quarter of dk][k tile][lane]
-  uint4 d_hi[2][2][4][32];            // [buffer][columns][token block][lane]
+  uint4 s[2][2][4][DK / 64][2][32];   // S [buffer][columns][quarter of dk][k tile][term][lane]
+  uint4 d[2][2][4][2][32];            // d [buffer][columns][token block][term][lane]
   float4 x[2][4][3][2][32];           // partial S^T k [columns][quarter][block - quarter - 1][tile][lane]
-  uint4 rx[2][4][2][32];              // R [columns][token block][hi, lo][lane]
-  uint4 dx[2][4][2][32];              // weighted d, likewise
-  int bad[2][2][16];                  // [buffer][columns][column] first token whose R is not finite, or C
-  float s_inv[2][2], d_inv[2][2];     // [buffer][columns]
-  float s_max[2][4], v_max[2][4];     // [columns][quarter]
-  uint64_t full[kQuadStages], empty[kQuadStages], out_full[kQuadOutStages], out_empty[kQuadOutStages];
+  uint4 rx[2][4][3][32];              // R [columns][token block][term][lane]
+  uint4 dx[2][4][3][32];              // weighted d, likewise
+  int bad[2][2][16];                  // [buffer][columns][column] first token whose R or d is not finite, or C
+  uint64_t full[kQuadStages<DK>], empty[kQuadStages<DK>], out_full[kQuadOutStages], out_empty[kQuadOutStages];
   int length[kSorted], seq;
   uint64_t s_full[2][2], d_full[2][2], out_done[2][2];   // [buffer][columns]
 };
@@ -69,14 +67,14 @@ __device__ __forceinline__ void from_uint4(uint32_t (&r)[4], uint4 v) { r[0] = v
 // the same time: 0 and 3 to one, 1 and 2 to the other.
 __device__ __forceinline__ int block_of(int half, int i) { return half ? 1 + i : 3 * i; }
 
-// A block's values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
-__device__ __forceinline__ void spoil_block(float* d, int block, int bad0, int bad1, float v) {
+// A block's values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become NaN.
+__device__ __forceinline__ void spoil_block(float* d, int block, int bad0, int bad1) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int tok = block * 16 + i * 8 + 2 * (threadIdx.x & 3);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i * 4 + j] = v;
+      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i * 4 + j] = CUDART_NAN_F;
   }
 }
 
@@ -90,7 +88,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
   const int c0 = static_cast<int>(blockIdx.x % cb) * kQuadCols;
   const int h = static_cast<int>(blockIdx.x / cb % a.heads);
   if (tid == 0) {
-    for (int i = 0; i < kQuadStages; ++i) {
+    for (int i = 0; i < kQuadStages<DK>; ++i) {
       mbar_init(&sm.full[i], 129);   // the bulk copies' bytes, 128 lanes' copies of v
       mbar_init(&sm.empty[i], 12);
     }
@@ -121,7 +119,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
     constexpr int NT = DK / 32, KT = DK / 64;
     const int grp = w >> 2, qd = grp ? 3 - (w & 3) : w & 3, d0 = qd * (DK / 4);
     const float* src = s_from ? s_from + s_at + grp * 16 + g : nullptr;
-    float S[NT][4];   // S^T 2^e: rows are columns g and g + 8, columns are dk
+    float S[NT][4];   // S^T: rows are columns g and g + 8, columns are dk
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int64_t r = static_cast<int64_t>(d0 + i * 8 + 2 * t) * a.dv;
@@ -134,12 +132,11 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
 #pragma unroll
       for (int i = 0; i < NT; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = CUDART_NAN_F;
     }
-    float acc[8][4], vb[2][4];   // this quarter's part of S^T k 2^e, blocks qd, qd + 1, .. (mod 4); beta v of the block
-    float inv = 1.f;             // 2^-e
+    float acc[8][4], vb[2][4];   // this quarter's part of S^T k, blocks qd, qd + 1, .. (mod 4); beta v of the block
     uint32_t kx[KT][4][4];       // k's fragments of the chunk that comes next
     auto load_keys = [&](uint32_t n) {
-      wait(&sm.full[n % kQuadStages], (n / kQuadStages) & 1);
-      const uint32_t kb = smem_u32(sm.stage[n % kQuadStages].k);
+      wait(&sm.full[n % kQuadStages<DK>], (n / kQuadStages<DK>) & 1);
+      const uint32_t kb = smem_u32(sm.stage[n % kQuadStages<DK>].k);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -147,39 +144,34 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
           ldsm4(kx[kt][b], kb + swz<DK * 2>(((qd + b) & 3) * 16 + (lane & 7) + ((lane >> 4) << 3),
                                             d0 / 8 + kt * 2 + ((lane >> 3) & 1)));
     };
-    // S as f16 terms times the keys of chunk n; the hi terms go to the warps of the outputs too.  What chunk
+    // S's terms times the keys of chunk n; the first two terms go to the warps of the outputs too.  What chunk
     // n's R needs besides comes behind the products.
     auto times_keys = [&](uint32_t n) {
       const uint32_t bf = n & 1;
-      const QuadStage<DK>& sn = sm.stage[n % kQuadStages];
-      uint32_t hi[KT][4], lo[KT][4];
+      const QuadStage<DK>& sn = sm.stage[n % kQuadStages<DK>];
+      uint32_t f[KT][3][4];
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) frag_split(S[2 * kt], S[2 * kt + 1], hi[kt], lo[kt]);
+      for (int kt = 0; kt < KT; ++kt) frag_split(S[2 * kt], S[2 * kt + 1], f[kt]);
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (kt == 0) {
-            mma_first(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
-            mma_first(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
-          } else {
-            mma_add(acc[2 * b], hi[kt], kx[kt][b][0], kx[kt][b][1]);
-            mma_add(acc[2 * b + 1], hi[kt], kx[kt][b][2], kx[kt][b][3]);
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            if (kt == 0 && term == 0) {
+              mma_first(acc[2 * b], f[kt][term], kx[kt][b][0], kx[kt][b][1]);
+              mma_first(acc[2 * b + 1], f[kt][term], kx[kt][b][2], kx[kt][b][3]);
+            } else {
+              mma_add(acc[2 * b], f[kt][term], kx[kt][b][0], kx[kt][b][1]);
+              mma_add(acc[2 * b + 1], f[kt][term], kx[kt][b][2], kx[kt][b][3]);
+            }
           }
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          mma_add(acc[2 * b], lo[kt], kx[kt][b][0], kx[kt][b][1]);
-          mma_add(acc[2 * b + 1], lo[kt], kx[kt][b][2], kx[kt][b][3]);
-        }
-      }
       if (n >= 2) wait(&sm.out_done[bf][grp], ((n >> 1) + 1) & 1);
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) sm.s_hi[bf][grp][qd][kt][lane] = as_uint4(hi[kt]);
-      if (qd == 0) {
-        if (lane == 0) sm.s_inv[bf][grp] = inv;
-        if (lane < 16) sm.bad[bf][grp][lane] = C;
-      }
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int term = 0; term < 2; ++term) sm.s[bf][grp][qd][kt][term][lane] = as_uint4(f[kt][term]);
+      if (qd == 0 && lane < 16) sm.bad[bf][grp][lane] = C;
       warp_arrive(&sm.s_full[bf][grp]);
       uint32_t v[4];   // (columns 0-7 | 8-15) x (tokens 0-7), then tokens 8-15, transposed
       ldsm4t(v, smem_u32(sn.v) + swz<64>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), grp * 2 + ((lane >> 3) & 1)));
@@ -191,38 +183,16 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
         vb[j][2] = fb.x * __uint_as_float(v[2 * j + 1] << 16);
         vb[j][3] = fb.y * __uint_as_float(v[2 * j + 1] & 0xffff0000u);
       }
-      const float s_max = warp_max(S) * inv, v_max = warp_max(vb);
-      if (lane == 0) {
-        sm.s_max[grp][qd] = s_max;
-        sm.v_max[grp][qd] = v_max;
-      }
-    };
-    auto largest = [](const float (&v)[4]) {
-      const float4 x = *reinterpret_cast<const float4*>(v);
-      return fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
     };
     if (first < last) {
-      const float m = warp_max(S);
-      if (lane == 0) sm.s_max[grp][qd] = m;
-      quad_sync(grp);
-      const int e = scale_exp(__float_as_uint(largest(sm.s_max[grp])));
-      quad_sync(grp);   // s_max is written again below
-      const float s = exp2i(e);
-      inv = exp2i(-e);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) S[i][j] *= s;
       load_keys(0);
       times_keys(0);
     }
     for (int64_t ci = first; ci < last; ++ci) {
-      const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kQuadStages, buf = it & 1;
+      const uint32_t it = static_cast<uint32_t>(ci - first), st = it % kQuadStages<DK>, buf = it & 1;
       QuadStage<DK>& sg = sm.stage[st];
-      const uint32_t kb = smem_u32(sg.k);
+      const uint32_t kb = smem_u32(sg.k), tb = smem_u32(sg.t) + lane * 16;
       const bool more = ci + 1 < last;
-      const float4 fe = *reinterpret_cast<const float4*>(&sg.f[kFEnd]);
-      const float2 fm = *reinterpret_cast<const float2*>(&sg.f[kFEnd + 4]);
       // the quarters' parts meet, each in the warp of its token block
 #pragma unroll
       for (int b = 1; b < 4; ++b)
@@ -231,82 +201,61 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
           sm.x[grp][qd][b - 1][j][lane] = make_float4(acc[2 * b + j][0], acc[2 * b + j][1], acc[2 * b + j][2], acc[2 * b + j][3]);
       quad_sync(grp);
       float R[2][4];
-      const float s_all = largest(sm.s_max[grp]);
-      // |k| <= 1: S^T k is at most sqrt(dk) times S's largest
-      const float r_bound = fmaf(fm.y * (DK == 128 ? 11.4f : 8.1f), s_all, largest(sm.v_max[grp]));
-      const int re = bound_exp(r_bound);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float4 o1 = sm.x[grp][(qd + 1) & 3][2][j][lane];
         const float4 o2 = sm.x[grp][(qd + 2) & 3][1][j][lane];
         const float4 o3 = sm.x[grp][(qd + 3) & 3][0][j][lane];
         const float2 fa = *reinterpret_cast<const float2*>(&sg.f[kFA + qd * 16 + j * 8 + 2 * t]);
-        const float ax = fa.x * inv, ay = fa.y * inv;
-        R[j][0] = fmaf(ax, (acc[j][0] + o1.x) + (o2.x + o3.x), vb[j][0]);
-        R[j][1] = fmaf(ay, (acc[j][1] + o1.y) + (o2.y + o3.y), vb[j][1]);
-        R[j][2] = fmaf(ax, (acc[j][2] + o1.z) + (o2.z + o3.z), vb[j][2]);
-        R[j][3] = fmaf(ay, (acc[j][3] + o1.w) + (o2.w + o3.w), vb[j][3]);
+        R[j][0] = fmaf(fa.x, (acc[j][0] + o1.x) + (o2.x + o3.x), vb[j][0]);
+        R[j][1] = fmaf(fa.y, (acc[j][1] + o1.y) + (o2.y + o3.y), vb[j][1]);
+        R[j][2] = fmaf(fa.x, (acc[j][2] + o1.z) + (o2.z + o3.z), vb[j][2]);
+        R[j][3] = fmaf(fa.y, (acc[j][3] + o1.w) + (o2.w + o3.w), vb[j][3]);
       }
-      const float r_nan = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(0.f, R[0][0], R[0][1]), R[0][2], R[0][3]), R[1][0],
-                                                  R[1][1]), R[1][2], R[1][3]);
-      if (__any_sync(0xffffffffu, !(r_nan < CUDART_INF_F))) {
-        // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros:
-        // it is taken out here and put back into d from that token on.
+      // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros: it is taken out
+      // here and put back into d from that token on.
+      auto take_out = [&](float (&x)[2][4]) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (!(fabsf(R[i][j]) < CUDART_INF_F)) {
+            if (!(fabsf(x[i][j]) < CUDART_INF_F)) {
               atomicMin(&sm.bad[buf][grp][g + (j >> 1) * 8], qd * 16 + i * 8 + 2 * t + (j & 1));
-              R[i][j] = 0.f;
+              x[i][j] = 0.f;
             }
-      }
-      uint32_t rh[4], rl[4];
-      {
-        const float s = exp2i(re);
+      };
+      if (any_not_finite(R)) take_out(R);
+      uint32_t r[3][4];
+      frag_split(R[0], R[1], r);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int term = 0; term < 3; ++term) sm.rx[grp][qd][term][lane] = as_uint4(r[term]);
+      // d = T R of this block, R's blocks qd, qd - 1, .., 0; the products' sums by their size: p[0] of the first
+      // terms, p[1] 2^-8 and p[2] 2^-16 of it
+      float p[3][2][4];
+      auto times_t = [&](const uint32_t (&x)[3][4], int src, bool fresh) {
+        uint32_t y[3][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) R[i][j] *= s;
-        frag_split(R[0], R[1], rh, rl);
-        sm.rx[grp][qd][0][lane] = as_uint4(rh);
-        sm.rx[grp][qd][1][lane] = as_uint4(rl);
-      }
-      // T's rows of this block; beyond the diagonal they are zero, and all four warps go the same way
-      uint32_t yh[4][4], yl[4][4];
+        for (int term = 0; term < 3; ++term) ldsm4(y[term], tb + term * kTermBytes + tri_block(qd, src));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t at = swz<128>(qd * 16 + (lane & 7) + ((lane >> 4) << 3), ((qd + j) & 3) * 2 + ((lane >> 3) & 1));
-        ldsm4(yh[j], smem_u32(sg.t_hi) + at);
-        ldsm4(yl[j], smem_u32(sg.t_lo) + at);
-      }
+        for (int sum = 0; sum < 3; ++sum)
+#pragma unroll
+          for (int i = 0; i <= sum; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (fresh && i == 0) mma_first(p[sum][j], x[i], y[sum - i][2 * j], y[sum - i][2 * j + 1]);
+              else mma_add(p[sum][j], x[i], y[sum - i][2 * j], y[sum - i][2 * j + 1]);
+            }
+      };
+      times_t(r, qd, true);
       quad_sync(grp);
-      // d = T R of this block: source blocks qd, qd + 1, .. (mod 4), in two sets of accumulators
-      float p[2][2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t xh[4], xl[4];
-        if (j == 0) {
+      for (int j = 1; j < 4; ++j)
+        if (j <= qd) {
+          uint32_t x[3][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { xh[i] = rh[i]; xl[i] = rl[i]; }
-        } else {
-          from_uint4(xh, sm.rx[grp][(qd + j) & 3][0][lane]);
-          from_uint4(xl, sm.rx[grp][(qd + j) & 3][1][lane]);
+          for (int term = 0; term < 3; ++term) from_uint4(x[term], sm.rx[grp][qd - j][term][lane]);
+          times_t(x, qd - j, false);
         }
-        float(&d0_)[4] = p[j & 1][0];
-        float(&d1_)[4] = p[j & 1][1];
-        if (j < 2) {
-          mma_first(d0_, xh, yh[j][0], yh[j][1]);
-          mma_first(d1_, xh, yh[j][2], yh[j][3]);
-        } else {
-          mma_add(d0_, xh, yh[j][0], yh[j][1]);
-          mma_add(d1_, xh, yh[j][2], yh[j][3]);
-        }
-        mma_add(d0_, xl, yh[j][0], yh[j][1]);
-        mma_add(d1_, xl, yh[j][2], yh[j][3]);
-        mma_add(d0_, xh, yl[j][0], yl[j][1]);
-        mma_add(d1_, xh, yl[j][2], yl[j][3]);
-      }
       // k^T's fragments for the state's update
       uint32_t kt_[4][NT / 2][4];
 #pragma unroll
@@ -314,99 +263,81 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np)
           ldsm4t(kt_[b][np], kb + swz<DK * 2>(((qd + b) & 3) * 16 + (lane & 15), d0 / 8 + np * 2 + (lane >> 4)));
-      // d's scales come from bounds: R's times T's row sums, weighted (for the state, in two terms) and not
-      // (for the outputs, in one)
-      const float w_bound = r_bound * fe.w;
-      const int we = bound_exp(w_bound), de = bound_exp(r_bound * fm.x);
-      const float d_inv = w_bound > 0.f ? exp2i(-we) : 0.f;
-      const float c = exp2i(-re) * fe.y, c16 = c * exp2i(de), cw = c * exp2i(we);
       const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
       const bool any_bad = __any_sync(0xffffffffu, bad0 < C || bad1 < C);
-      uint32_t wh[4], wl[4], d16[4];
+      uint32_t wd[3][4];   // d, weighted for the state
+      float od[2][4];      // d for the outputs
       {
         float d[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[i][j] = p[0][i][j] + p[1][i][j];
-        if (any_bad) spoil_block(&d[0][0], qd, bad0, bad1, 0.f);
-        d16[0] = pack_h2(d[0][0] * c16, d[0][1] * c16);
-        d16[1] = pack_h2(d[0][2] * c16, d[0][3] * c16);
-        d16[2] = pack_h2(d[1][0] * c16, d[1][1] * c16);
-        d16[3] = pack_h2(d[1][2] * c16, d[1][3] * c16);
+          for (int j = 0; j < 4; ++j) od[i][j] = p[0][i][j] + (p[1][i][j] + p[2][i][j]);
+        if (any_bad) spoil_block(&od[0][0], qd, bad0, bad1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float2 fw = *reinterpret_cast<const float2*>(&sg.f[kFW + qd * 16 + i * 8 + 2 * t]);
-          const float wx = fw.x * cw, wy = fw.y * cw;
-          d[i][0] *= wx;
-          d[i][1] *= wy;
-          d[i][2] *= wx;
-          d[i][3] *= wy;
+          d[i][0] = od[i][0] * fw.x;
+          d[i][1] = od[i][1] * fw.y;
+          d[i][2] = od[i][2] * fw.x;
+          d[i][3] = od[i][3] * fw.y;
         }
-        if (any_bad) spoil_block(&d[0][0], qd, bad0, bad1, CUDART_NAN_F);
-        frag_split(d[0], d[1], wh, wl);
-        sm.dx[grp][qd][0][lane] = as_uint4(wh);
-        sm.dx[grp][qd][1][lane] = as_uint4(wl);
+        frag_split(d[0], d[1], wd);
+#pragma unroll
+        for (int term = 0; term < 3; ++term) sm.dx[grp][qd][term][lane] = as_uint4(wd[term]);
       }
-      quad_sync(grp);
-      // S = e^G64 S + d k^T for this quarter of dk.  Its scale comes from a bound: 64 products of d and
-      // k, both below 2^15 as f16.
-      const int e = bound_exp(fmaf(s_all, fe.x, d_inv * 0x1p36f));
-      const float s = exp2i(e), keep = fe.x * inv * s, gain = d_inv * s;
-      inv = exp2i(-e);
-      {
-        float u[NT][4];
+      // S = e^G64 S + d k^T for this quarter of dk
+      float u[NT][4];
+      auto times_k = [&](const uint32_t (&x)[3][4], int b) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint32_t xh[4], xl[4];
-          if (b == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { xh[i] = wh[i]; xl[i] = wl[i]; }
-          } else {
-            from_uint4(xh, sm.dx[grp][(qd + b) & 3][0][lane]);
-            from_uint4(xl, sm.dx[grp][(qd + b) & 3][1][lane]);
-          }
+        for (int term = 0; term < 3; ++term)
 #pragma unroll
           for (int np = 0; np < NT / 2; ++np) {
             const uint32_t(&y)[4] = kt_[b][np];
-            if (b == 0) {
-              mma_first(u[2 * np], xh, y[0], y[1]);
-              mma_first(u[2 * np + 1], xh, y[2], y[3]);
+            if (b == 0 && term == 0) {
+              mma_first(u[2 * np], x[term], y[0], y[1]);
+              mma_first(u[2 * np + 1], x[term], y[2], y[3]);
             } else {
-              mma_add(u[2 * np], xh, y[0], y[1]);
-              mma_add(u[2 * np + 1], xh, y[2], y[3]);
+              mma_add(u[2 * np], x[term], y[0], y[1]);
+              mma_add(u[2 * np + 1], x[term], y[2], y[3]);
             }
           }
+      };
+      times_k(wd, 0);
+      quad_sync(grp);
 #pragma unroll
-          for (int np = 0; np < NT / 2; ++np) {
-            mma_add(u[2 * np], xl, kt_[b][np][0], kt_[b][np][1]);
-            mma_add(u[2 * np + 1], xl, kt_[b][np][2], kt_[b][np][3]);
-          }
-        }
-        if (more) load_keys(it + 1);
+      for (int b = 1; b < 4; ++b) {
+        uint32_t x[3][4];
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) S[i][j] = fmaf(u[i][j], gain, S[i][j] * keep);
+        for (int term = 0; term < 3; ++term) from_uint4(x[term], sm.dx[grp][(qd + b) & 3][term][lane]);
+        times_k(x, b);
       }
-      // d for the outputs of this chunk
-      sm.d_hi[buf][grp][qd][lane] = make_uint4(d16[0], d16[1], d16[2], d16[3]);
-      if (qd == 0 && lane == 0) sm.d_inv[buf][grp] = exp2i(-de);
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.d_full[buf][grp]);
-        mbar_arrive(&sm.empty[st]);
+      // d for the outputs of this chunk, under the state's products; a d that overflowed is bad for them, too
+      if (any_not_finite(od)) take_out(od);
+      {
+        uint32_t o[2][4];
+        frag_split(od[0], od[1], o);
+#pragma unroll
+        for (int term = 0; term < 2; ++term) sm.d[buf][grp][qd][term][lane] = as_uint4(o[term]);
       }
+      warp_arrive(&sm.d_full[buf][grp]);
+      const float keep = sg.f[kFEnd];
+      if (more) load_keys(it + 1);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[i][j] = fmaf(S[i][j], keep, u[i][j]);
+      warp_arrive(&sm.empty[st]);
       if (more) times_keys(it + 1);
     }
     float* dst = a.s_out + s_at + grp * 16 + g;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int64_t r = static_cast<int64_t>(d0 + i * 8 + 2 * t) * a.dv;
-      dst[r] = S[i][0] * inv;
-      dst[r + a.dv] = S[i][1] * inv;
-      dst[r + 8] = S[i][2] * inv;
-      dst[r + a.dv + 8] = S[i][3] * inv;
+      dst[r] = S[i][0];
+      dst[r + a.dv] = S[i][1];
+      dst[r + 8] = S[i][2];
+      dst[r + a.dv + 8] = S[i][3];
     }
   } else {
     // ---- the outputs: columns grp * 16 .. + 15, half of the token blocks per warp; and the copies
@@ -422,14 +353,14 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
     };
     // chunk `it` of what the recurrence reads, its stage being free
     auto copy_in = [&](uint32_t it) {
-      QuadStage<DK>& sg = sm.stage[it % kQuadStages];
-      uint64_t* bar = &sm.full[it % kQuadStages];
+      QuadStage<DK>& sg = sm.stage[it % kQuadStages<DK>];
+      uint64_t* bar = &sm.full[it % kQuadStages<DK>];
       const int64_t t0 = begin + (first + it) * C;
       const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
       if (hl == 0) {
         mbar_arrive_expect_tx(bar, C * DK * 2 + kRecBytes);
         bulk_g2s(sg.k, keys_at(it), C * DK * 2, bar);
-        bulk_g2s(sg.t_hi, head_at(it), kRecBytes, bar);
+        bulk_g2s(sg.t, head_at(it), kRecBytes, bar);
       }
       __syncwarp();
       const uint16_t* v = a.v + t0 * a.v_row + h * a.v_head + c0;
@@ -460,80 +391,80 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
       QuadOutStage<DK>& og = sm.out_stage[it % kQuadOutStages];
       uint64_t* bar = &sm.out_full[it % kQuadOutStages];
       if (hl == 0) {
-        mbar_arrive_expect_tx(bar, C * DK * 2 + kMat);
+        mbar_arrive_expect_tx(bar, C * DK * 2 + kPBytes);
         bulk_g2s(og.q, keys_at(it) + C * DK * 2, C * DK * 2, bar);
-        bulk_g2s(og.p, head_at(it) + kRecBytes, kMat, bar);
+        bulk_g2s(og.p, head_at(it) + kRecBytes, kPBytes, bar);
       }
       __syncwarp();
     };
-    for (uint32_t i = 0; i < n && i < kQuadStages; ++i) copy_in(i);
+    for (uint32_t i = 0; i < n && i < kQuadStages<DK>; ++i) copy_in(i);
     for (uint32_t i = 0; i < n && i < kQuadOutStages; ++i) copy_out_operands(i);
     for (uint32_t it = 0; it < n; ++it) {
-      const uint32_t st = it % kQuadStages, so = it % kQuadOutStages, buf = it & 1;
+      const uint32_t st = it % kQuadStages<DK>, so = it % kQuadOutStages, buf = it & 1;
       QuadStage<DK>& sg = sm.stage[st];
       QuadOutStage<DK>& og = sm.out_stage[so];
       const int64_t t0 = begin + (first + it) * C;
       const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
-      wait(&sm.full[st], (it / kQuadStages) & 1);
+      wait(&sm.full[st], (it / kQuadStages<DK>) & 1);
       wait(&sm.out_full[so], (it / kQuadOutStages) & 1);
       wait(&sm.s_full[buf][grp], (it >> 1) & 1);
-      const uint32_t qb = smem_u32(og.q), pb = smem_u32(og.p);
-      float acc[4][4], o[4][4];
+      const uint32_t qb = smem_u32(og.q), pb = smem_u32(og.p) + lane * 16;
+      float o[4][4];   // o^T: rows are columns g and g + 8, tiles of 8 tokens
 #pragma unroll
       for (int kt = 0; kt < DK / 16; ++kt) {
-        uint32_t x[4];
-        from_uint4(x, sm.s_hi[buf][grp][kt / KT][kt % KT][lane]);
+        uint32_t x[2][4];
+#pragma unroll
+        for (int term = 0; term < 2; ++term) from_uint4(x[term], sm.s[buf][grp][kt / KT][kt % KT][term][lane]);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           uint32_t y[4];
           ldsm4(y, qb + swz<DK * 2>(block_of(half, b) * 16 + (lane & 7) + ((lane >> 4) << 3), kt * 2 + ((lane >> 3) & 1)));
-          if (kt == 0) {
-            mma_first(acc[2 * b], x, y[0], y[1]);
-            mma_first(acc[2 * b + 1], x, y[2], y[3]);
-          } else {
-            mma_add(acc[2 * b], x, y[0], y[1]);
-            mma_add(acc[2 * b + 1], x, y[2], y[3]);
+#pragma unroll
+          for (int term = 0; term < 2; ++term) {
+            if (kt == 0 && term == 0) {
+              mma_first(o[2 * b], x[term], y[0], y[1]);
+              mma_first(o[2 * b + 1], x[term], y[2], y[3]);
+            } else {
+              mma_add(o[2 * b], x[term], y[0], y[1]);
+              mma_add(o[2 * b + 1], x[term], y[2], y[3]);
+            }
           }
         }
       }
-      const float si = sm.s_inv[buf][grp];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 f = *reinterpret_cast<const float2*>(&sg.f[kFQ + block_of(half, i >> 1) * 16 + (i & 1) * 8 + 2 * t]);
-        const float fx = f.x * si, fy = f.y * si;
-        o[i][0] = acc[i][0] * fx;
-        o[i][1] = acc[i][1] * fy;
-        o[i][2] = acc[i][2] * fx;
-        o[i][3] = acc[i][3] * fy;
+        o[i][0] *= f.x;
+        o[i][1] *= f.y;
+        o[i][2] *= f.x;
+        o[i][3] *= f.y;
       }
       wait(&sm.d_full[buf][grp], (it >> 1) & 1);
-      const float ps = sm.d_inv[buf][grp] * sg.f[kFEnd + 2];
 #pragma unroll
-      for (int bj = 0; bj < 4; ++bj) {   // P is zero beyond the diagonal
-        uint32_t x[4];
-        from_uint4(x, sm.d_hi[buf][grp][bj][lane]);
+      for (int bj = 0; bj < 4; ++bj) {
+        uint32_t x[2][4];
+#pragma unroll
+        for (int term = 0; term < 2; ++term) from_uint4(x[term], sm.d[buf][grp][bj][term][lane]);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          uint32_t y[4];
-          ldsm4(y, pb + swz<128>(block_of(half, b) * 16 + (lane & 7) + ((lane >> 4) << 3), bj * 2 + ((lane >> 3) & 1)));
-          if (bj == 0) {
-            mma_first(acc[2 * b], x, y[0], y[1]);
-            mma_first(acc[2 * b + 1], x, y[2], y[3]);
-          } else {
-            mma_add(acc[2 * b], x, y[0], y[1]);
-            mma_add(acc[2 * b + 1], x, y[2], y[3]);
-          }
+          const int bi = block_of(half, b);
+          if (bj > bi) continue;
+          uint32_t y[2][4];
+#pragma unroll
+          for (int term = 0; term < 2; ++term) ldsm4(y[term], pb + term * kTermBytes + tri_block(bi, bj));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma_add(o[2 * b + j], x[1], y[0][2 * j], y[0][2 * j + 1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma_add(o[2 * b + j], x[0], y[1][2 * j], y[1][2 * j + 1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) mma_add(o[2 * b + j], x[0], y[0][2 * j], y[0][2 * j + 1]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = fmaf(acc[i][j], ps, o[i][j]);
       {
         const int bad0 = sm.bad[buf][grp][g], bad1 = sm.bad[buf][grp][g + 8];
         if (__any_sync(0xffffffffu, bad0 < C || bad1 < C)) {
-          spoil_block(&o[0][0], block_of(half, 0), bad0, bad1, CUDART_NAN_F);
-          spoil_block(&o[2][0], block_of(half, 1), bad0, bad1, CUDART_NAN_F);
+          spoil_block(&o[0][0], block_of(half, 0), bad0, bad1);
+          spoil_block(&o[2][0], block_of(half, 1), bad0, bad1);
         }
       }
       __syncwarp();
@@ -557,9 +488,9 @@ __global__ void __launch_bounds__(kQuadThreads, 1) dn_walk_quad_kernel(const DnR
         wait(&sm.out_empty[so], (it / kQuadOutStages) & 1);
         copy_out_operands(it + kQuadOutStages);
       }
-      if (it + kQuadStages < n) {
-        wait(&sm.empty[st], (it / kQuadStages) & 1);
-        copy_in(it + kQuadStages);
+      if (it + kQuadStages<DK> < n) {
+        wait(&sm.empty[st], (it / kQuadStages<DK>) & 1);
+        copy_in(it + kQuadStages<DK>);
       }
     }
     // nothing of these warps may still be on its way when the block ends

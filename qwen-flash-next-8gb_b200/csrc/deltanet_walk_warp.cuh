@@ -3,8 +3,8 @@
 //
 // No exchange and no barrier in a chunk, so a chunk takes longer than in the quads'
 // walk but a block holds two to four times the columns.  Four prompts of 2048
-// tokens, 32 heads of 128 x 128: 344 us a call against 505 with the quads' walk;
-// one prompt: 179 against 136.  Tensor pipe 57 % in blocks of 128 columns.
+// tokens, 32 heads of 128 x 128: 412 us a call against 522 with the quads' walk;
+// one prompt: 210 against 137.
 #pragma once
 
 #include "deltanet_chunk_parts.cuh"
@@ -19,9 +19,9 @@ constexpr int kWarpThreads = kWarpCols / 16 * 32;
 template <int DK>
 struct WarpStage {
   unsigned char k[C * DK * 2], q[C * DK * 2];
-  unsigned char t_hi[kMat], t_lo[kMat];
+  unsigned char t[3 * kTermBytes];
   float f[kFactors];
-  unsigned char p[kMat];
+  unsigned char p[kPBytes];
   unsigned char v[C * kWarpCols * 2];
 };
 
@@ -32,19 +32,19 @@ struct WarpSmem {
   int length[kSorted], seq;
 };
 
-// Values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become v.
-__device__ __forceinline__ void spoil(float (&d)[8][4], int bad0, int bad1, float v) {
+// Values of a lane's columns g (first token bad0) and g + 8 (bad1) from those tokens on become NaN.
+__device__ __forceinline__ void spoil(float (&d)[8][4], int bad0, int bad1) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int tok = i * 8 + 2 * (threadIdx.x & 3);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i][j] = v;
+      if (tok + (j & 1) >= (j < 2 ? bad0 : bad1)) d[i][j] = CUDART_NAN_F;
   }
 }
 
 // A warp walks 16 columns of S on its own, every product transposed so that the columns are the 16 rows
-// of the A operand: the accumulators of one product, split into f16 terms, are then the A fragments of
+// of the A operand: the accumulators of one product, split into bf16 terms, are then the A fragments of
 // the next, and S, R and d never leave the registers.  The k, q, T and P tiles are B operands that all
 // warps of the block read from shared memory.
 template <int DK>
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
   const bool ok = part.ok;
   const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
 
-  // Four warps have a scheduler each and walk a chunk in 3.9 us, eight in 5.9.  Blocks have 128 columns, and every
+  // Four warps have a scheduler each and walk a chunk of dk = 128 in 5.0 us, eight in 7.8.  Blocks have 128 columns, and every
   // second block of 64 none, but for sequences that would take longer so than their share of all SMs' time, where
   // these are few enough for all their blocks of 64 columns to run at once.
   bool wide = true;
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
     constexpr int NT = DK / 8, KT = DK / 16;
     const float* s_from = first > 0 ? a.s_out : a.s_in;
     const int64_t s_at = (seq * a.heads + h) * DK * static_cast<int64_t>(a.dv) + c0 + w * 16 + g;
-    float S[NT][4];   // S^T 2^e: rows are columns g and g + 8, columns are dk
+    float S[NT][4];   // S^T: rows are columns g and g + 8, columns are dk
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const float* src = s_from + s_at + static_cast<int64_t>(i * 8 + 2 * t) * a.dv;
@@ -99,16 +99,6 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
       S[i][2] = s_from ? src[8] : 0.f;
       S[i][3] = s_from ? src[a.dv + 8] : 0.f;
       if (!ok) S[i][0] = S[i][1] = S[i][2] = S[i][3] = CUDART_NAN_F;
-    }
-    float s_max = warp_max(S), inv;   // the largest of S; 2^-e
-    {
-      const int e = scale_exp(__float_as_uint(s_max));
-      const float s = exp2i(e);
-      inv = exp2i(-e);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) S[i][j] *= s;
     }
     const int64_t pitch = static_cast<int64_t>(a.heads) * a.dv;
     // where this lane's pieces of a tile's fragments lie: rows of N, and rows of K (transposed)
@@ -149,7 +139,7 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
           const unsigned char* head = work.heads + (slot * a.heads + h) * static_cast<int64_t>(kHeadBytes);
           mbar_arrive_expect_tx(&sm.full[st], 2 * C * DK * 2 + kHeadBytes);
           bulk_g2s(sg.k, work.kq + (slot * key_heads + h / a.ratio) * (2 * C * DK * 2), 2 * C * DK * 2, &sm.full[st]);
-          bulk_g2s(sg.t_hi, head, kHeadBytes, &sm.full[st]);
+          bulk_g2s(sg.t, head, kHeadBytes, &sm.full[st]);
         }
         __syncwarp();
       }
@@ -165,31 +155,30 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
       if (it + kStages - 1 < n) copy(it + kStages - 1);
       const float* f = sg.f;
       wait(&sm.full[st], (it / kStages) & 1);
-      // S^T k and, from S's hi terms alone, S^T q: token tiles of 8
+      // S^T k and, from S's first two terms, S^T q: token tiles of 8
       float x[8][4], o[8][4];
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        uint32_t hi[4], lo[4];
-        frag_split(S[2 * kt], S[2 * kt + 1], hi, lo);
+        uint32_t s3[3][4];
+        frag_split(S[2 * kt], S[2 * kt + 1], s3);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           uint32_t y[4], z[4];
           const uint32_t at = swz<DK * 2>(b * 16 + n_row, kt * 2 + n_ch);
           ldsm4(y, kb + at);
           ldsm4(z, qb + at);
-          if (kt == 0) {
-            mma_first(x[2 * b], hi, y[0], y[1]);
-            mma_first(x[2 * b + 1], hi, y[2], y[3]);
-            mma_first(o[2 * b], hi, z[0], z[1]);
-            mma_first(o[2 * b + 1], hi, z[2], z[3]);
-          } else {
-            mma_add(x[2 * b], hi, y[0], y[1]);
-            mma_add(x[2 * b + 1], hi, y[2], y[3]);
-            mma_add(o[2 * b], hi, z[0], z[1]);
-            mma_add(o[2 * b + 1], hi, z[2], z[3]);
-          }
-          mma_add(x[2 * b], lo, y[0], y[1]);
-          mma_add(x[2 * b + 1], lo, y[2], y[3]);
+#pragma unroll
+          for (int term = 0; term < 3; ++term)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (kt == 0 && term == 0) {
+                mma_first(x[2 * b + j], s3[term], y[2 * j], y[2 * j + 1]);
+                mma_first(o[2 * b + j], s3[term], z[2 * j], z[2 * j + 1]);
+              } else {
+                mma_add(x[2 * b + j], s3[term], y[2 * j], y[2 * j + 1]);
+                if (term < 2) mma_add(o[2 * b + j], s3[term], z[2 * j], z[2 * j + 1]);
+              }
+            }
         }
       }
       // R = beta v - beta e^G S^T k
@@ -202,137 +191,93 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
           const int i = 2 * b + j;
           const float2 fa = *reinterpret_cast<const float2*>(f + kFA + i * 8 + 2 * t);
           const float2 fb = *reinterpret_cast<const float2*>(f + kFB + i * 8 + 2 * t);
-          const float ax = fa.x * inv, ay = fa.y * inv;
-          x[i][0] = fmaf(ax, x[i][0], fb.x * __uint_as_float(v[2 * j] << 16));
-          x[i][1] = fmaf(ay, x[i][1], fb.y * __uint_as_float(v[2 * j] & 0xffff0000u));
-          x[i][2] = fmaf(ax, x[i][2], fb.x * __uint_as_float(v[2 * j + 1] << 16));
-          x[i][3] = fmaf(ay, x[i][3], fb.y * __uint_as_float(v[2 * j + 1] & 0xffff0000u));
+          x[i][0] = fmaf(fa.x, x[i][0], fb.x * __uint_as_float(v[2 * j] << 16));
+          x[i][1] = fmaf(fa.y, x[i][1], fb.y * __uint_as_float(v[2 * j] & 0xffff0000u));
+          x[i][2] = fmaf(fa.x, x[i][2], fb.x * __uint_as_float(v[2 * j + 1] << 16));
+          x[i][3] = fmaf(fa.y, x[i][3], fb.y * __uint_as_float(v[2 * j + 1] & 0xffff0000u));
         }
       }
-      float m0 = 0.f, m1 = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        m0 = max_abs_nan(m0, x[i][0], x[i][1]);
-        m1 = max_abs_nan(m1, x[i][2], x[i][3]);
-      }
-      uint32_t rm = __reduce_max_sync(0xffffffffu, __float_as_uint(max_abs_nan(m0, m1, 0.f)) & 0x7fffffffu);
+      // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros: it is taken out
+      // here and put back into d from that token on.
       int bad0 = C, bad1 = C;
-      const bool any_bad = rm >= 0x7f800000u;
-      if (any_bad) {
-        // A token's infinity or NaN may not reach the tokens before it through T's and P's zeros:
-        // it is taken out here and put back into d from that token on.
-        rm = 0;
+      auto take_out = [&]() {
 #pragma unroll
-        for (int i = 7; i >= 0; --i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int j = 3; j >= 0; --j) {
+          for (int j = 0; j < 4; ++j)
             if (!(fabsf(x[i][j]) < CUDART_INF_F)) {
               (j < 2 ? bad0 : bad1) = min(j < 2 ? bad0 : bad1, i * 8 + 2 * t + (j & 1));
               x[i][j] = 0.f;
             }
-            rm = max(rm, finite_bits(x[i][j]));
-          }
-        rm = __reduce_max_sync(0xffffffffu, rm);
 #pragma unroll
         for (int off = 1; off < 4; off <<= 1) {
           bad0 = min(bad0, __shfl_xor_sync(0xffffffffu, bad0, off));
           bad1 = min(bad1, __shfl_xor_sync(0xffffffffu, bad1, off));
         }
-      }
-      const float r_max = __uint_as_float(rm);
-      const int re = scale_exp(rm);
-      uint32_t rh[4][4], rl[4][4];
+      };
+      bool any_bad = any_not_finite(x);
+      if (any_bad) take_out();
+      // d = T R, blocks on and below the diagonal
       {
-        const float s = exp2i(re);
+        float d[8][4];
+        const uint32_t tb = smem_u32(sg.t) + lane * 16;
+#pragma unroll
+        for (int bj = 0; bj < 4; ++bj) {
+          uint32_t r[3][4];
+          frag_split(x[2 * bj], x[2 * bj + 1], r);
+#pragma unroll
+          for (int term = 2; term >= 0; --term) {   // of T, the smallest first; with it the terms of R that are not below 2^-24
+            uint32_t y[4][4];
+#pragma unroll
+            for (int bi = bj; bi < 4; ++bi) ldsm4(y[bi], tb + term * kTermBytes + tri_block(bi, bj));
+#pragma unroll
+            for (int i = 2 - term; i >= 0; --i)
+#pragma unroll
+              for (int bi = bj; bi < 4; ++bi)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  if (bj == 0 && term == 2) mma_first(d[2 * bi + j], r[i], y[bi][2 * j], y[bi][2 * j + 1]);
+                  else mma_add(d[2 * bi + j], r[i], y[bi][2 * j], y[bi][2 * j + 1]);
+                }
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[i][j] *= s;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) frag_split(x[2 * b], x[2 * b + 1], rh[b], rl[b]);
+          for (int j = 0; j < 4; ++j) x[i][j] = d[i][j];
       }
-      // d = T R, blocks on and below the diagonal
-      const uint32_t th = smem_u32(sg.t_hi), tl = smem_u32(sg.t_lo);
-#pragma unroll
-      for (int bj = 0; bj < 4; ++bj) {
-#pragma unroll
-        for (int bi = bj; bi < 4; ++bi) {
-          uint32_t y[4], z[4];
-          const uint32_t at = swz<128>(bi * 16 + n_row, bj * 2 + n_ch);
-          ldsm4(y, th + at);
-          ldsm4(z, tl + at);
-          if (bj == 0) {
-            mma_first(x[2 * bi], rh[bj], y[0], y[1]);
-            mma_first(x[2 * bi + 1], rh[bj], y[2], y[3]);
-          } else {
-            mma_add(x[2 * bi], rh[bj], y[0], y[1]);
-            mma_add(x[2 * bi + 1], rh[bj], y[2], y[3]);
-          }
-          mma_add(x[2 * bi], rl[bj], y[0], y[1]);
-          mma_add(x[2 * bi + 1], rl[bj], y[2], y[3]);
-          mma_add(x[2 * bi], rh[bj], z[0], z[1]);
-          mma_add(x[2 * bi + 1], rh[bj], z[2], z[3]);
-        }
-      }
-      // d's scales come from bounds: R's largest times T's row sums, weighted (for the state, in two terms) and
-      // not (for the outputs, in one)
-      const float4 fe = *reinterpret_cast<const float4*>(f + kFEnd);
-      const float w_bound = r_max * fe.w;
-      const int we = bound_exp(w_bound), de = bound_exp(r_max * f[kFEnd + 4]);
-      const float d_inv = w_bound > 0.f ? exp2i(-we) : 0.f;
-      const float c = exp2i(-re) * fe.y, c16 = c * exp2i(de), cw = c * exp2i(we);
-      if (any_bad) spoil(x, bad0, bad1, 0.f);
-      uint32_t d16[4][4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        d16[b][0] = pack_h2(x[2 * b][0] * c16, x[2 * b][1] * c16);
-        d16[b][1] = pack_h2(x[2 * b][2] * c16, x[2 * b][3] * c16);
-        d16[b][2] = pack_h2(x[2 * b + 1][0] * c16, x[2 * b + 1][1] * c16);
-        d16[b][3] = pack_h2(x[2 * b + 1][2] * c16, x[2 * b + 1][3] * c16);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 fw = *reinterpret_cast<const float2*>(f + kFW + i * 8 + 2 * t);
-        const float wx = fw.x * cw, wy = fw.y * cw;
-        x[i][0] *= wx;
-        x[i][1] *= wy;
-        x[i][2] *= wx;
-        x[i][3] *= wy;
-      }
-      if (any_bad) spoil(x, bad0, bad1, CUDART_NAN_F);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) frag_split(x[2 * b], x[2 * b + 1], rh[b], rl[b]);
+      if (any_bad) spoil(x, bad0, bad1);
+      any_bad = any_not_finite(x);   // a d that overflowed is bad from its token on, too
+      if (any_bad) take_out();
       // o = e^G S^T q + P d
       {
-        const float os = inv, ps = exp2i(-de) * fe.z;
-        const uint32_t pb = smem_u32(sg.p);
+        const uint32_t pb = smem_u32(sg.p) + lane * 16;
 #pragma unroll
-        for (int bi = 0; bi < 4; ++bi) {
-          float e[2][4];
+        for (int i = 0; i < 8; ++i) {
+          const float2 fq = *reinterpret_cast<const float2*>(f + kFQ + i * 8 + 2 * t);
+          o[i][0] *= fq.x;
+          o[i][1] *= fq.y;
+          o[i][2] *= fq.x;
+          o[i][3] *= fq.y;
+        }
 #pragma unroll
-          for (int bj = 0; bj <= bi; ++bj) {
-            uint32_t y[4];
-            ldsm4(y, pb + swz<128>(bi * 16 + n_row, bj * 2 + n_ch));
-            if (bj == 0) {
-              mma_first(e[0], d16[bj], y[0], y[1]);
-              mma_first(e[1], d16[bj], y[2], y[3]);
-            } else {
-              mma_add(e[0], d16[bj], y[0], y[1]);
-              mma_add(e[1], d16[bj], y[2], y[3]);
-            }
-          }
+        for (int bj = 0; bj < 4; ++bj) {
+          uint32_t d2[2][4];
+          frag_split(x[2 * bj], x[2 * bj + 1], d2);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int i = 2 * bi + j;
-            const float2 fq = *reinterpret_cast<const float2*>(f + kFQ + i * 8 + 2 * t);
-            const float qx = fq.x * os, qy = fq.y * os;
-            o[i][0] = fmaf(e[j][0], ps, o[i][0] * qx);
-            o[i][1] = fmaf(e[j][1], ps, o[i][1] * qy);
-            o[i][2] = fmaf(e[j][2], ps, o[i][2] * qx);
-            o[i][3] = fmaf(e[j][3], ps, o[i][3] * qy);
+          for (int term = 1; term >= 0; --term) {   // of P
+            uint32_t y[4][4];
+#pragma unroll
+            for (int bi = bj; bi < 4; ++bi) ldsm4(y[bi], pb + term * kTermBytes + tri_block(bi, bj));
+#pragma unroll
+            for (int i = 1 - term; i >= 0; --i)
+#pragma unroll
+              for (int bi = bj; bi < 4; ++bi)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mma_add(o[2 * bi + j], d2[i], y[bi][2 * j], y[bi][2 * j + 1]);
           }
         }
-        if (any_bad) spoil(o, bad0, bad1, CUDART_NAN_F);
+        if (any_bad) spoil(o, bad0, bad1);
         const int64_t t0 = begin + (first + it) * C;
         const int cnt = static_cast<int>(min(static_cast<int64_t>(C), begin + len - t0));
         uint16_t* dst = a.out + (t0 + g) * pitch + static_cast<int64_t>(h) * a.dv + c0 + w * 16 + 2 * t;
@@ -348,11 +293,22 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
           dst += 8 * pitch;
         }
       }
-      // S = e^G64 S + d k.  Its scale comes from a bound: 64 products of d and k, both below 2^15 as f16.
-      const int e = bound_exp(fmaf(s_max, fe.x, d_inv * 0x1p36f));
-      const float s = exp2i(e), keep = fe.x * inv * s, gain = d_inv * s;
-      inv = exp2i(-e);
-      m0 = m1 = 0.f;
+      // S = e^G64 S + d k
+      if (any_bad) spoil(x, bad0, bad1);
+      uint32_t wd[4][3][4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+#pragma unroll
+        for (int i = 2 * b; i < 2 * b + 2; ++i) {
+          const float2 fw = *reinterpret_cast<const float2*>(f + kFW + i * 8 + 2 * t);
+          x[i][0] *= fw.x;
+          x[i][1] *= fw.y;
+          x[i][2] *= fw.x;
+          x[i][3] *= fw.y;
+        }
+        frag_split(x[2 * b], x[2 * b + 1], wd[b]);
+      }
+      const float keep = f[kFEnd];
 #pragma unroll
       for (int np = 0; np < NT / 4; ++np) {   // 32 of dk at a time
         float u[4][4];
@@ -361,43 +317,36 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
           uint32_t y[4], z[4];
           ldsm4t(y, kb + swz<DK * 2>(b * 16 + k_row, np * 4 + k_ch));
           ldsm4t(z, kb + swz<DK * 2>(b * 16 + k_row, np * 4 + 2 + k_ch));
-          if (b == 0) {
-            mma_first(u[0], rh[b], y[0], y[1]);
-            mma_first(u[1], rh[b], y[2], y[3]);
-            mma_first(u[2], rh[b], z[0], z[1]);
-            mma_first(u[3], rh[b], z[2], z[3]);
-          } else {
-            mma_add(u[0], rh[b], y[0], y[1]);
-            mma_add(u[1], rh[b], y[2], y[3]);
-            mma_add(u[2], rh[b], z[0], z[1]);
-            mma_add(u[3], rh[b], z[2], z[3]);
+#pragma unroll
+          for (int term = 0; term < 3; ++term) {
+            if (b == 0 && term == 0) {
+              mma_first(u[0], wd[b][term], y[0], y[1]);
+              mma_first(u[1], wd[b][term], y[2], y[3]);
+              mma_first(u[2], wd[b][term], z[0], z[1]);
+              mma_first(u[3], wd[b][term], z[2], z[3]);
+            } else {
+              mma_add(u[0], wd[b][term], y[0], y[1]);
+              mma_add(u[1], wd[b][term], y[2], y[3]);
+              mma_add(u[2], wd[b][term], z[0], z[1]);
+              mma_add(u[3], wd[b][term], z[2], z[3]);
+            }
           }
-          mma_add(u[0], rl[b], y[0], y[1]);
-          mma_add(u[1], rl[b], y[2], y[3]);
-          mma_add(u[2], rl[b], z[0], z[1]);
-          mma_add(u[3], rl[b], z[2], z[3]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) S[np * 4 + i][j] = fmaf(u[i][j], gain, S[np * 4 + i][j] * keep);
-          m0 = max_abs(m0, S[np * 4 + i][0], S[np * 4 + i][1]);
-          m1 = max_abs(m1, S[np * 4 + i][2], S[np * 4 + i][3]);
-        }
+          for (int j = 0; j < 4; ++j) S[np * 4 + i][j] = fmaf(S[np * 4 + i][j], keep, u[i][j]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[st]);
-      s_max = fmaxf(m0, m1);
-      uint32_t sb = __reduce_max_sync(0xffffffffu, __float_as_uint(s_max));
-      s_max = sb < 0x7f800000u ? __uint_as_float(sb) * inv : warp_max(S) * inv;
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       float* dst = a.s_out + s_at + static_cast<int64_t>(i * 8 + 2 * t) * a.dv;
-      dst[0] = S[i][0] * inv;
-      dst[a.dv] = S[i][1] * inv;
-      dst[8] = S[i][2] * inv;
-      dst[a.dv + 8] = S[i][3] * inv;
+      dst[0] = S[i][0];
+      dst[a.dv] = S[i][1];
+      dst[8] = S[i][2];
+      dst[a.dv + 8] = S[i][3];
     }
     // nothing of this warp may still be on its way when the block ends
     asm volatile("cp.async.wait_all;" ::: "memory");

@@ -10,10 +10,16 @@ sequences of any length, ragged batches of them, with a state carried in and
 out.  step_gated_delta_rule (qfn_deltanet_step_batch) runs one token for each
 request of a batch, with the requests' states in slots of a pool.
 
-Per token and value head (value head h uses key head h // (H // Hq)), in fp32:
+Per token and value head (value head h uses key head h // (H // Hq)):
 
     q = l2norm(q) / sqrt(dk);  k = l2norm(k)       l2norm: x * rsqrt(sum x^2 + 1e-6)
     S = exp(g) * S;  d = beta * (v - S^T k);  S = S + k d^T;  out = bf16(S^T q)
+
+The states and every sum are fp32.  The prompts' chunks multiply on the tensor
+cores: what the state is made of is taken with fp32's 24 bits, what only reaches
+the bf16 outputs with 16 of them, each value with an exponent of its own.  -inf
+in g clears a finite state.  g is a decay, g <= 0; growth is taken too, as long as
+it stays below e^88 within 64 tokens.  q and k rows have norms below 2^63.
 
 All three are forward only.
 """
