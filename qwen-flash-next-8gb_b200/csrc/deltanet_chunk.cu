@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(kPrepThreads, 3) dn_prep_kernel(const DnRows a
         const double up = __shfl_up_sync(0xffffffffu, run, o);
         if (lane >= o) run += up;
       }
-      const double G[2] = {run - s[1], run};
+      const double before = __shfl_up_sync(0xffffffffu, run, 1);   // not run - s[1]: s[1] may be NaN
+      const double G[2] = {lane ? before + s[0] : s[0], run};
       const double last = __shfl_sync(0xffffffffu, run, 31);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {

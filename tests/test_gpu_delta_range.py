@@ -173,6 +173,21 @@ def test_not_finite_from_its_token_on(what, at, many):
 
 @pytest.mark.parametrize("many", [False, True])
 @pytest.mark.parametrize("bad", ["inf", "nan"])
+@pytest.mark.parametrize("at", [1, 5, 64, 127])
+def test_decay_not_finite_leaves_the_token_before(at, bad, many):
+    T, H = 150, 4
+    q, k, v, g, beta, S0 = inputs(T, H, H, 64, 128, seed=8)
+    clean = recurrence(q, k, v, g, beta, S0)
+    g[at, 2] = float(bad)
+    out, S = chunk(many, q, k, v, g, beta, S0)
+    close(out, None, clean, tokens=at)
+    heads = [0, 1, 3]
+    close(out[:, heads], S[heads], (clean[0][:, heads], clean[1][heads], clean[2][:, heads], clean[3][:, heads]))
+    assert not out[at:, 2].isfinite().any() and not S[2].isfinite().any()
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("bad", ["inf", "nan"])
 def test_not_finite_carried_column(bad, many):
     T, H = 100, 4
     q, k, v, g, beta, S0 = inputs(T, H, 2, 64, 128, seed=9)
