@@ -65,14 +65,16 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t i, const floa
   }
 }
 
-// 1 / (1 + e^-x) from the special-function unit's exp2 and reciprocal: each within 2 steps of fp32,
-// and the rounding of x log2(e) moves the exponential by |x| 2^-23 at most.  (With expf and a true
-// division the gated norm was bound by its instructions: 106 us for 16384 x 32 rows of 128, 79 with these.)
+// 1 / (1 + e^-x) from the special-function unit's exp2 and reciprocal, as 2^-24 / (2^-24 + 2^-24 e^-x): so neither the
+// exponential nor the reciprocal leaves fp32's normal numbers before the result is below 2^-149 (silu(-89) = -2e-37 is
+// a normal number although sigmoid(-89) is none).  The two are each within 2 steps of fp32; the rounding of
+// x log2(e) + 24 moves the exponential by 2^-20 at most around zero, by |x| 2^-23 far from it.  (With expf and a true
+// division the gated norm was bound by its instructions: 106 us for 16384 x 32 rows of 128.)
 __device__ __forceinline__ float sigmoidf(float x) {
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(x, -1.44269504f, -24.f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0x1p-24f + e));
+  return r * 0x1p-24f;
 }
 
 // ------------------------------------------------------------------ gated norm
@@ -87,7 +89,7 @@ struct GatedNorm {
 
 // LANES lanes of a warp share one row of dim <= 8 LANES; a thread takes its
 // piece of ROWS rows, one block's worth apart, and requests all of them first.
-// Measured: 16384 x 32 rows of 128 in 70 to 75 us, 5.4 to 5.8 TB/s (issue slots 70 %).
+// Measured: 16384 x 32 rows of 128 in 69 to 76 us, 5.3 to 5.8 TB/s (issue slots 70 %).
 template <int LANES, int ROWS>
 __global__ void __launch_bounds__(256) gated_norm_kernel(const GatedNorm a) {
   constexpr int kPer = 256 / LANES;   // rows of a block at a time
