@@ -259,7 +259,7 @@ int qfn_deltanet_step(const uint16_t* q, const uint16_t* k, const uint16_t* v, c
  *   out and touches no state.
  *   state_in, state_out: f32[n_slots][n_heads][dk][dv], 16-byte aligned, the
  *   same array or two that do not overlap; slots no row names are not written.
- *   out: bf16[rows][n_heads][dv].  dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.
+ *   out: bf16[rows][n_heads][dv], apart from both.  dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.
  */
 int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* g,
                             const uint16_t* beta, const int64_t* strides, const int32_t* state_index,
@@ -277,7 +277,7 @@ int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t
  *   Bounds that do not rise: no row is written and every final state is NaN.
  *   state_in: f32[n_seqs][n_heads][dk][dv] or NULL (zeros); state_out: the
  *   same shape, state_in itself or an array that does not overlap it; both
- *   16-byte aligned; out 4-byte aligned.  dk in {64, 128, 256}; dv % 32 == 0,
+ *   16-byte aligned; out 4-byte aligned and apart from both.  dk in {64, 128, 256}; dv % 32 == 0,
  *   dv <= 4096.  q, k and v are read in 16-byte pieces where their bases and
  *   strides allow it, else element by element.
  *   dk <= 128 and more than 8 tokens (of each sequence without cu_seqlens, in
@@ -322,7 +322,8 @@ int qfn_gated_norm(const uint16_t* x, int64_t x_row, int64_t x_head, const uint1
  *   gate_kind: 0 none, 1 one value per row (gate[row * gate_row]), 2 one per element.
  *   block, residual, gate, w_post, w_next: f32 or bf16 by their dtype codes,
  *   row strides in elements.  residual_out: [rows][dim] of residual's type
- *   (the residual's own array if that is dense); normed: bf16[rows][dim].
+ *   (the residual's own array if that is dense, else apart from every input);
+ *   normed: bf16[rows][dim], apart from all others.
  *   n is formed from r before its rounding.  1 <= dim <= 32768.
  */
 int qfn_norm_residual(const void* block, int block_dtype, int64_t block_row, const void* residual,

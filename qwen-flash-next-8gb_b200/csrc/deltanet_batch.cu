@@ -215,11 +215,22 @@ int dn_rows_check(const char* what, const uint16_t* q, const uint16_t* k, const 
 
 namespace {
 
+bool clash(const void* x, uintptr_t x_bytes, const void* y, uintptr_t y_bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+  return x && y && x_bytes && y_bytes && a < b + y_bytes && b < a + x_bytes;
+}
+
 // States that overlap without being the same would be read after they were written.
 bool states_clash(const float* in, const float* out, int64_t n) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(in), b = reinterpret_cast<uintptr_t>(out);
   const uintptr_t bytes = static_cast<uintptr_t>(n) * sizeof(float);
-  return in && a != b && a < b + bytes && b < a + bytes;
+  return in != out && clash(in, bytes, out, bytes);
+}
+
+// Outputs are written while other blocks still read states.
+bool out_clash(const DnRows& a, int64_t rows, int64_t states, int dk) {
+  const uintptr_t out = static_cast<uintptr_t>(rows) * a.heads * a.dv * sizeof(uint16_t),
+                  S = static_cast<uintptr_t>(states) * a.heads * dk * a.dv * sizeof(float);
+  return clash(a.out, out, a.s_in, S) || clash(a.out, out, a.s_out, S);
 }
 
 // The grid waits for the kernel before it (pdl_wait) and never releases the
@@ -263,6 +274,7 @@ extern "C" int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, con
               static_cast<long long>(rows), static_cast<long long>(n_slots));
   QFN_REQUIRE(!states_clash(state_in, state_out, n_slots * n_heads * dk * dv), QFN_ERR_INVALID_ARG,
               "%s: state_in and state_out overlap", what);
+  QFN_REQUIRE(!out_clash(a, rows, n_slots, dk), QFN_ERR_INVALID_ARG, "%s: out overlaps a state", what);
   if (rows == 0) return QFN_OK;
   DeviceInfo* dev;
   rc = current_device(&dev);
@@ -305,6 +317,7 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
     QFN_REQUIRE(aligned(workspace, 256), QFN_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", what);
     QFN_REQUIRE(aligned(out, 4), QFN_ERR_ALIGNMENT, "%s: out must be 4-byte aligned", what);
   }
+  QFN_REQUIRE(!out_clash(a, tokens, n_seqs, dk), QFN_ERR_INVALID_ARG, "%s: out overlaps a state", what);
   DeviceInfo* dev;
   rc = current_device(&dev);
   if (rc) return rc;

@@ -20,6 +20,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <initializer_list>
+#include <utility>
+
 #include "qfn.h"
 
 namespace {
@@ -184,6 +187,14 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   return x < y + (nb + 1) * b.element_size() && y < x + (na + 1) * a.element_size();
 }
 
+// `t` is written while others are still read.
+void req_apart(const at::Tensor& t, const char* name,
+               std::initializer_list<std::pair<const at::Tensor*, const char*>> others) {
+  for (const auto& o : others)
+    TORCH_CHECK_VALUE(!o.first || !o.first->defined() || !overlap(t, *o.first), name, " overlaps ", o.second);
+}
+const at::Tensor* given(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
+
 // One operand of the batched delta rule as rows: [.., heads(, d)] after one or two leading dimensions that
 // count as one.  Views are taken as they are if their last dimension is dense and their leading ones can be
 // counted as one; others are copied.
@@ -250,14 +261,21 @@ void req_state(const at::Tensor& S, const char* name, int64_t n, const DeltaRows
                     r.dk, ", ", r.dv, "], got ", S.sizes());
 }
 
-at::Tensor req_out(const std::optional<at::Tensor>& out, const at::Tensor& value, const DeltaRows& r) {
+// A state to be written.  It may be the state that is read, whose overlap the library checks.
+void req_new_state(const at::Tensor& S, const char* name, const DeltaRows& r, const std::optional<at::Tensor>& plan,
+                   const char* plan_name) {
+  req_apart(S, name, {{&r.q.t, "query"}, {&r.k.t, "key"}, {&r.v.t, "value"}, {&r.g.t, "g"}, {&r.beta.t, "beta"},
+                      {given(plan), plan_name}});
+}
+
+at::Tensor req_out(const std::optional<at::Tensor>& out, const at::Tensor& value, const DeltaRows& r,
+                   const std::optional<at::Tensor>& plan, const char* plan_name) {
   if (!out) return at::empty(value.sizes(), r.q_.options());
   req_view(*out, "out", at::kBFloat16, r.q_, "query");
   TORCH_CHECK_VALUE(out->is_contiguous() && out->sizes() == value.sizes(), "out must be a contiguous ", value.sizes(),
                     ", got ", out->sizes());
-  TORCH_CHECK_VALUE(!overlap(*out, r.q.t) && !overlap(*out, r.k.t) && !overlap(*out, r.v.t) && !overlap(*out, r.g.t) &&
-                        !overlap(*out, r.beta.t),
-                    "out overlaps an input");
+  req_apart(*out, "out", {{&r.q.t, "query"}, {&r.k.t, "key"}, {&r.v.t, "value"}, {&r.g.t, "g"}, {&r.beta.t, "beta"},
+                          {given(plan), plan_name}});   // states: the library
   return *out;
 }
 
@@ -282,9 +300,12 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
     n_seqs = cu->size(0) - 1;
   }
   if (s_in) req_state(*s_in, "initial_state", n_seqs, r);
-  if (s_out) req_state(*s_out, "final_state", n_seqs, r);
+  if (s_out) {
+    req_state(*s_out, "final_state", n_seqs, r);
+    req_new_state(*s_out, "final_state", r, cu, "cu_seqlens");
+  }
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = req_out(out_, v, r);
+  at::Tensor out = req_out(out_, v, r, cu, "cu_seqlens");
   at::Tensor S = s_out ? *s_out : at::empty({n_seqs, r.H, r.dk, r.dv}, g.options());
   // equal sequences need no workspace where one of them alone needs none
   const size_t nbytes = !cu && qfn_deltanet_chunk_workspace(q.size(1), 1, r.H, r.Hq, r.dk, r.dv) == 0
@@ -318,8 +339,9 @@ at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Ten
   }
   TORCH_CHECK_VALUE(index || R <= state.size(0), "state has ", state.size(0), " slots for ", R,
                     " tokens (pass state_index)");
+  req_new_state(out_state, "out_state", r, index, "state_index");
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = req_out(out_, v, r);
+  at::Tensor out = req_out(out_, v, r, index, "state_index");
   if (R == 0) return out;
   check_rc(qfn_deltanet_step_batch(u16(r.q.t), u16(r.k.t), u16(r.v.t), r.g.t.data_ptr<float>(), u16(r.beta.t), r.strides,
                                    index ? index->data_ptr<int32_t>() : nullptr, state.size(0),
@@ -397,7 +419,7 @@ std::tuple<at::Tensor, at::Tensor> norm_residual(const at::Tensor& block_, const
     // in place of the residual itself is fine: a thread writes what it has read
     TORCH_CHECK_VALUE((r.data_ptr() == residual.data_ptr() && residual.is_contiguous()) || !overlap(r, residual),
                       "out overlaps the residual without being it");
-    TORCH_CHECK_VALUE(!overlap(r, block) && !(kind && overlap(r, gate)), "out overlaps block or gate");
+    req_apart(r, "out", {{&block, "block"}, {&gate, "gate"}, {given(post), "post_weight"}, {given(next), "next_weight"}});
   }
   at::Tensor n = next ? at::empty({T, D}, block.options().dtype(at::kBFloat16)) : at::Tensor();
   if (T == 0 || D == 0) return {r, next ? n : r};
