@@ -75,7 +75,8 @@ def chunk_gated_delta_rule(query, key, value, g, beta, initial_state=None, cu_se
     initial_state [N, H, dk, dv] fp32 (None: zeros).  final_state and out may be
     given to be written; final_state may be initial_state itself.  Views with any
     row and head strides are taken as they are."""
-    return op("deltanet_chunk")(query, key, value, g, beta, cu_seqlens, initial_state, final_state, out)
+    o, S = op("deltanet_chunk")(query, key, value, g, beta, cu_seqlens, initial_state, final_state, out)
+    return o if out is None else out, S if final_state is None else final_state
 
 
 def step_gated_delta_rule(query, key, value, g, beta, state, state_index=None, out_state=None, out=None):
@@ -92,4 +93,4 @@ def step_gated_delta_rule(query, key, value, g, beta, state, state_index=None, o
     if out_state is None:
         out_state = state
     o = op("deltanet_step")(query, key, value, g, beta, state, state_index, out_state, out)
-    return o, out_state
+    return o if out is None else out, out_state

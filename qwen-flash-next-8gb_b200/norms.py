@@ -38,4 +38,4 @@ def norm_residual(block, residual, post_weight=None, gate=None, scale=1.0, next_
     if gate is not None and gate.dim() == 1:
         gate = gate[:, None]
     r, n = op("norm_residual")(block, residual, post_weight, gate, sigmoid, scale, next_weight, eps, out)
-    return r, (None if next_weight is None else n)
+    return r if out is None else out, None if next_weight is None else n

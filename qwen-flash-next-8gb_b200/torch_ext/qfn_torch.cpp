@@ -279,6 +279,10 @@ at::Tensor req_out(const std::optional<at::Tensor>& out, const at::Tensor& value
   return *out;
 }
 
+// What an operator returns in the place of a tensor that its caller gave to be written: a returned tensor shares no
+// memory with an argument and is returned once, as the schemas say.
+at::Tensor written(const at::Tensor& like) { return at::empty({0}, like.options()); }
+
 // query, key [B, T, Hq, dk], value [B, T, H, dv], g, beta [B, T, H]: B sequences, or (B = 1) those of cu_seqlens.
 std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                   const at::Tensor& g, const at::Tensor& beta,
@@ -319,7 +323,7 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
                               static_cast<uint16_t*>(out.data_ptr()), r.H, r.Hq, r.dk, r.dv,
                               nbytes ? ws.data_ptr() : nullptr, nbytes, stream_of(q)),
            "qfn_deltanet_chunk");
-  return {out, S};
+  return {out_ ? written(out) : out, s_out ? written(S) : S};
 }
 
 at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
@@ -342,13 +346,13 @@ at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Ten
   req_new_state(out_state, "out_state", r, index, "state_index");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = req_out(out_, v, r, index, "state_index");
-  if (R == 0) return out;
+  if (R == 0) return out_ ? written(out) : out;
   check_rc(qfn_deltanet_step_batch(u16(r.q.t), u16(r.k.t), u16(r.v.t), r.g.t.data_ptr<float>(), u16(r.beta.t), r.strides,
                                    index ? index->data_ptr<int32_t>() : nullptr, state.size(0),
                                    state.data_ptr<float>(), out_state.data_ptr<float>(),
                                    static_cast<uint16_t*>(out.data_ptr()), R, r.H, r.Hq, r.dk, r.dv, stream_of(q)),
            "qfn_deltanet_step_batch");
-  return out;
+  return out_ ? written(out) : out;
 }
 
 // x, z [R, H, D], w [D] -> [R, H, D]
@@ -374,7 +378,8 @@ at::Tensor gated_norm(const at::Tensor& x_, const at::Tensor& z_, const at::Tens
   return y;
 }
 
-// block, residual [T, D]; gate [T, 1] or [T, D]; residual_out: residual's type, contiguous.
+// block, residual [T, D]; gate [T, 1] or [T, D]; residual_out: residual's type, contiguous.  Without next the second
+// tensor is empty.
 std::tuple<at::Tensor, at::Tensor> norm_residual(const at::Tensor& block_, const at::Tensor& residual_,
                                                  const std::optional<at::Tensor>& post,
                                                  const std::optional<at::Tensor>& gate_, bool sigmoid, double scale,
@@ -421,8 +426,8 @@ std::tuple<at::Tensor, at::Tensor> norm_residual(const at::Tensor& block_, const
                       "out overlaps the residual without being it");
     req_apart(r, "out", {{&block, "block"}, {&gate, "gate"}, {given(post), "post_weight"}, {given(next), "next_weight"}});
   }
-  at::Tensor n = next ? at::empty({T, D}, block.options().dtype(at::kBFloat16)) : at::Tensor();
-  if (T == 0 || D == 0) return {r, next ? n : r};
+  at::Tensor n = at::empty(next ? at::IntArrayRef{T, D} : at::IntArrayRef{0}, block.options().dtype(at::kBFloat16));
+  if (T == 0 || D == 0) return {r_out ? written(r) : r, n};
   check_rc(qfn_norm_residual(block.data_ptr(), bd, block.stride(0), residual.data_ptr(), rd, residual.stride(0),
                              post ? post->data_ptr() : nullptr, pd, kind ? gate.data_ptr() : nullptr, kind, gd,
                              kind ? gate.stride(0) : 0, sigmoid, static_cast<float>(scale),
@@ -430,7 +435,7 @@ std::tuple<at::Tensor, at::Tensor> norm_residual(const at::Tensor& block_, const
                              next ? static_cast<uint16_t*>(n.data_ptr()) : nullptr, T, static_cast<int>(D),
                              static_cast<float>(eps), stream_of(r)),
            "qfn_norm_residual");
-  return {r, next ? n : r};
+  return {r_out ? written(r) : r, n};
 }
 
 }  // namespace
