@@ -21,7 +21,8 @@ the bf16 outputs with 16 of them, each value with an exponent of its own.  -inf
 in g clears a finite state.  g is a decay, g <= 0; growth is taken too, as long as
 it stays below e^88 within 64 tokens.  q and k rows have norms below 2^63.
 
-All three are forward only.
+All three are forward only; the batched two refuse a tensor that requires a
+gradient while gradients are recorded.
 """
 import torch
 

@@ -3,7 +3,8 @@ the residual add that follow them (libqfn's qfn_gated_norm and
 qfn_norm_residual).
 
 RMSNorm here is x * rsqrt(mean(x^2) + eps) * weight, computed in fp32; every
-output is rounded once.  Both are forward only.
+output is rounded once.  Both are forward only and refuse a tensor that requires
+a gradient while gradients are recorded.
 """
 from _lib import op
 

@@ -16,6 +16,7 @@
 //   qfn::gated_norm      -> qfn_gated_norm
 //   qfn::norm_residual   -> qfn_norm_residual
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -164,6 +165,16 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s)
   return y;
 }
 
+const at::Tensor* given(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
+
+// Forward only: a result without its gradient would look like one with it.
+void req_no_grad(const char* what, std::initializer_list<std::pair<const at::Tensor*, const char*>> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const auto& t : tensors)
+    TORCH_CHECK(!t.first || !t.first->requires_grad(), what, " is forward only and ", t.second,
+                " requires a gradient (call it under torch.no_grad(), or detach it)");
+}
+
 // A CUDA tensor of type dt on ref's device; views pass.
 void req_view(const at::Tensor& t, const char* name, at::ScalarType dt, const at::Tensor& ref, const char* ref_name) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor (libqfn has no CPU path)");
@@ -193,8 +204,6 @@ void req_apart(const at::Tensor& t, const char* name,
   for (const auto& o : others)
     TORCH_CHECK_VALUE(!o.first || !o.first->defined() || !overlap(t, *o.first), name, " overlaps ", o.second);
 }
-const at::Tensor* given(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
-
 // One operand of the batched delta rule as rows: [.., heads(, d)] after one or two leading dimensions that
 // count as one.  Views are taken as they are if their last dimension is dense and their leading ones can be
 // counted as one; others are copied.
@@ -290,6 +299,8 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
                                                   const std::optional<at::Tensor>& s_in,
                                                   const std::optional<at::Tensor>& s_out,
                                                   const std::optional<at::Tensor>& out_) {
+  req_no_grad("deltanet_chunk", {{&q, "query"}, {&k, "key"}, {&v, "value"}, {&g, "g"}, {&beta, "beta"},
+                                 {given(s_in), "initial_state"}, {given(s_out), "final_state"}, {given(out_), "out"}});
   TORCH_CHECK_VALUE(!cu || (q.dim() == 4 && q.size(0) == 1),
                     "cu_seqlens takes one batch row holding every sequence, got query ", q.sizes());
   TORCH_CHECK_VALUE(!out_ || out_->sizes() == v.sizes(), "out must be a contiguous ", v.sizes());
@@ -329,6 +340,8 @@ std::tuple<at::Tensor, at::Tensor> deltanet_chunk(const at::Tensor& q, const at:
 at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
                          const at::Tensor& beta, const at::Tensor& state, const std::optional<at::Tensor>& index,
                          at::Tensor out_state, const std::optional<at::Tensor>& out_) {
+  req_no_grad("deltanet_step", {{&q, "query"}, {&k, "key"}, {&v, "value"}, {&g, "g"}, {&beta, "beta"}, {&state, "state"},
+                                {&out_state, "out_state"}, {given(out_), "out"}});
   const DeltaRows r(q, k, v, g, beta, 1);
   const int64_t R = r.rows;
   req_state(state, "state", -1, r);
@@ -358,6 +371,7 @@ at::Tensor deltanet_step(const at::Tensor& q, const at::Tensor& k, const at::Ten
 // x, z [R, H, D], w [D] -> [R, H, D]
 at::Tensor gated_norm(const at::Tensor& x_, const at::Tensor& z_, const at::Tensor& w, double eps) {
   at::Tensor x = x_, z = z_;
+  req_no_grad("gated_norm", {{&x, "x"}, {&z, "z"}, {&w, "weight"}});
   req_view(x, "x", at::kBFloat16, x, "x");
   req_view(z, "z", at::kBFloat16, x, "x");
   req_cuda(w, "weight");
@@ -386,6 +400,8 @@ std::tuple<at::Tensor, at::Tensor> norm_residual(const at::Tensor& block_, const
                                                  const std::optional<at::Tensor>& next, double eps,
                                                  const std::optional<at::Tensor>& r_out) {
   at::Tensor block = block_, residual = residual_, gate;
+  req_no_grad("norm_residual", {{&block, "block"}, {&residual, "residual"}, {given(post), "post_weight"},
+                                {given(gate_), "gate"}, {given(next), "next_weight"}, {given(r_out), "out"}});
   TORCH_CHECK_VALUE(block.is_cuda(), "block must be a CUDA tensor (libqfn has no CPU path)");
   TORCH_CHECK_VALUE(residual.is_cuda(), "residual must be a CUDA tensor (libqfn has no CPU path)");
   same_device(residual, "residual", block, "block");
