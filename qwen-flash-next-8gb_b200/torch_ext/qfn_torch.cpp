@@ -188,8 +188,12 @@ int dtype_code(const at::Tensor& t, const char* name) {
   return t.scalar_type() == at::kFloat ? QFN_DTYPE_F32 : QFN_DTYPE_BF16;
 }
 
-// Whether two tensors' memory (as dense as their sizes say) shares a byte.
+// Whether two tensors' memory (as dense as their sizes say) shares a byte.  Most tensors have storages of their own,
+// which is told without their sizes (asking for those of a call's ten pairs took 0.3 us).
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const c10::StorageImpl *sa = a.storage().unsafeGetStorageImpl(), *sb = b.storage().unsafeGetStorageImpl();
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(sa->data()), pb = reinterpret_cast<uintptr_t>(sb->data());
+  if (pa >= pb + sb->nbytes() || pb >= pa + sa->nbytes()) return false;
   const uintptr_t x = reinterpret_cast<uintptr_t>(a.data_ptr()), y = reinterpret_cast<uintptr_t>(b.data_ptr());
   int64_t na = 0, nb = 0;
   if (a.numel() == 0 || b.numel() == 0) return false;
