@@ -238,8 +238,7 @@ int qfn_shared_expert_down(const uint16_t* w_down, int inter, int64_t T, const u
  *   v: bf16[n_heads][dv]; g: f32[n_heads]; beta: bf16[n_heads];
  *   S: f32[n_heads][dk][dv], updated in place; out: bf16[n_heads][dv].
  *   dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.  One launch (a
- *   programmatic dependent: the state is read before the dependency wait,
- *   so no earlier kernel of the stream may still write S).
+ *   programmatic dependent, which reads nothing before the dependency wait).
  */
 int qfn_deltanet_step(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* g,
                       const uint16_t* beta, float* S, uint16_t* out, int n_heads, int n_key_heads,

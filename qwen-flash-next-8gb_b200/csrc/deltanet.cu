@@ -46,10 +46,14 @@ __global__ void __launch_bounds__(kDnSlices * kDnCols) deltanet_step_kernel(
   const int h = blockIdx.x, c = blockIdx.y * kDnCols + (threadIdx.x & 31), sl = threadIdx.x >> 5;
   const int hk = h / hk_ratio;
   float* Sh = S + static_cast<int64_t>(h) * DK * dv;
+  // The state is asked for ahead of the wait, but only into L2: the kernel before may be the one that writes it (the
+  // step of the token before, a prompt's last chunk).
+  const int lane = threadIdx.x & 31;
+  if (lane < R) asm volatile("prefetch.global.L2 [%0];" ::"l"(Sh + static_cast<int64_t>(sl * R + lane) * dv + (c - lane)));
+  pdl_wait();
   float s[R];
 #pragma unroll
-  for (int j = 0; j < R; ++j) s[j] = Sh[static_cast<int64_t>(sl * R + j) * dv + c];   // issued first
-  pdl_wait();   // q, k, v, g, beta come from the previous kernels of the step
+  for (int j = 0; j < R; ++j) s[j] = Sh[static_cast<int64_t>(sl * R + j) * dv + c];
   pdl_launch_dependents();
   for (int i = threadIdx.x; i < DK; i += blockDim.x) {
     qs[i] = bf16_bits_to_f32(q[static_cast<int64_t>(hk) * DK + i]);
