@@ -279,8 +279,9 @@ int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t
  *   16-byte aligned; out 4-byte aligned and apart from both.  dk in {64, 128, 256}; dv % 32 == 0,
  *   dv <= 4096.  q, k and v are read in 16-byte pieces where their bases and
  *   strides allow it, else element by element.
- *   dk <= 128 and more than 8 tokens (of each sequence without cu_seqlens, in
- *   all with it) run 64 tokens at a time on the tensor cores (two launches for
+ *   dk <= 128 and more than 10 to 24 tokens, by the sizes (of each sequence
+ *   without cu_seqlens, in all with it, so that a ragged batch of many short
+ *   sequences pays for a chunk of 64 tokens each) run 64 tokens at a time on the tensor cores (two launches for
  *   each segment of the workspace); others token by token.  Both hold S and
  *   every sum in fp32.  The chunks' products take bf16 terms of their operands,
  *   each with fp32's range: three (24 bits) of all that S is made of, two (16 bits)

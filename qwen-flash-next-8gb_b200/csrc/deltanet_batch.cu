@@ -287,7 +287,9 @@ extern "C" int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, con
 
 extern "C" size_t qfn_deltanet_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk,
                                                int dv) {
-  if (tokens < 0 || n_seqs < 1 || n_heads < 1 || n_key_heads < 1 || !dn_chunk_takes(tokens, dk)) return 0;
+  if (tokens < 0 || n_seqs < 1 || n_heads < 1 || n_key_heads < 1 || dk < 1 || dv < 1 ||
+      !dn_chunk_takes(tokens, n_seqs, n_heads, dk, dv))
+    return 0;
   return dn_chunk_workspace(tokens, n_seqs, n_heads, n_key_heads, dk);
 }
 
@@ -309,7 +311,7 @@ extern "C" int qfn_deltanet_chunk(const uint16_t* q, const uint16_t* k, const ui
   QFN_REQUIRE(tokens < (int64_t{1} << 31) - 64, QFN_ERR_UNSUPPORTED, "%s: tokens=%lld", what,
               static_cast<long long>(tokens));
   if (n_seqs == 0) return QFN_OK;
-  const bool chunked = dn_chunk_takes(cu_seqlens ? tokens : tokens / n_seqs, dk);
+  const bool chunked = dn_chunk_takes(cu_seqlens ? tokens : tokens / n_seqs, n_seqs, n_heads, dk, dv);
   if (chunked) {
     const size_t need = dn_chunk_workspace(tokens, n_seqs, n_heads, n_key_heads, dk);
     QFN_REQUIRE(workspace && workspace_bytes >= need, QFN_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what,

@@ -396,7 +396,7 @@ cudaError_t launch(Kernel kernel, int64_t blocks, int threads, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Which walk: the quads' for few states, the warps' for many.  Blocks come in rounds of one per SM, and a chunk of
+// Which walk: the quads' for few states, the warps' for many, whatever their lengths (which only the device knows).  Blocks come in rounds of one per SM, and a chunk of
 // a block takes, in 0.1 us (one head, from 2048 to 6144 tokens): 32 columns in the quads' walk 29 for dk = 128 and
 // 23 for dk = 64, 64 columns in the warps' 50 and 36, 128 columns 78 and 54.
 template <int DK>
@@ -453,7 +453,11 @@ int run(const DnRows& a, const int32_t* cu, int64_t n_seqs, int64_t tokens, cons
 
 }  // namespace
 
-bool dn_chunk_takes(int64_t longest, int dk) { return dk <= 128 && longest > kRecurrenceTokens; }
+bool dn_chunk_takes(int64_t longest, int64_t n_seqs, int n_heads, int dk, int dv) {
+  const bool few = n_seqs * n_heads * (dv / 32) <= 300;   // blocks of the recurrence: up to two an SM
+  const int64_t by_size = 8 + 65536 / (static_cast<int64_t>(dk) * dv);
+  return dk <= 128 && longest > (few || by_size < 10 ? 10 : by_size < 24 ? by_size : 24);
+}
 
 size_t dn_chunk_workspace(int64_t tokens, int64_t n_seqs, int n_heads, int n_key_heads, int dk) {
   const int64_t slots = tokens / C + n_seqs;

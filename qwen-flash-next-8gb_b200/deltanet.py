@@ -74,8 +74,9 @@ def chunk_gated_delta_rule(query, key, value, g, beta, initial_state=None, cu_se
     through).
 
     initial_state [N, H, dk, dv] fp32 (None: zeros).  final_state and out may be
-    given to be written; final_state may be initial_state itself.  Views with any
-    row and head strides are taken as they are."""
+    given to be written; final_state may be initial_state itself.  Views of query,
+    key, value, g and beta with any row and head strides are taken as they are;
+    states start on 16 bytes, a given out on 4."""
     o, S = op("deltanet_chunk")(query, key, value, g, beta, cu_seqlens, initial_state, final_state, out)
     return o if out is None else out, S if final_state is None else final_state
 
@@ -90,7 +91,8 @@ def step_gated_delta_rule(query, key, value, g, beta, state, state_index=None, o
     r).  A negative index is a padding row: its out is zero and no state is
     touched.  An index past the pool, or one that an earlier row names too, gives NaN in
     that row's out and touches no state.  The new states are written to the same slots of out_state
-    (None: state itself, in place); slots that no row names are left as they were."""
+    (None: state itself, in place); slots that no row names are left as they were.
+    States start on 16 bytes."""
     if out_state is None:
         out_state = state
     o = op("deltanet_step")(query, key, value, g, beta, state, state_index, out_state, out)
