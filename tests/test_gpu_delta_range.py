@@ -23,6 +23,7 @@ import torch
 import _lib
 import deltanet
 import synthetic
+from test_gpu_delta_segments import walks
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -86,8 +87,9 @@ def close(out, S, ref, tokens=None):
 
 
 def chunk(many, q, k, v, g, beta, S0):
-    """One sequence (the walk of few states), or as the last of 40 (the walk of many)."""
-    N = 40 if many else 1
+    """One sequence (the walk of few states), or as the last of 32 (the walk of many: 128 states, a block of 128
+    columns each)."""
+    N = 32 if many else 1
     rep = [t.repeat(N, *[1] * (t.dim() - 1)).unflatten(0, (N, t.shape[0])) for t in (q, k, v, g, beta)]
     out, S = deltanet.chunk_gated_delta_rule(*rep, S0.repeat(N, 1, 1, 1))
     return out[N - 1], S[N - 1]
@@ -127,7 +129,17 @@ def arrange(case, q, k, v, g, beta, S0):
 CASES = ["columns", "token", "carried", "cleared", "cleared-late", "rise", "rising", "beta", "one-product"]
 
 
-@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 96)])
+SHAPES = [(128, 128), (64, 96), (64, 128)]   # those of the tests below
+
+
+@pytest.mark.parametrize("dk,dv", SHAPES)
+@pytest.mark.parametrize("many", [False, True])
+def test_the_walk_is_the_one_meant(many, dk, dv):
+    names, _ = walks(lambda: chunk(many, *inputs(150, 4, 2, dk, dv, seed=41)))
+    assert names <= {"walk_warp" if many else "walk_quad"}
+
+
+@pytest.mark.parametrize("dk,dv", SHAPES[:2])
 @pytest.mark.parametrize("many", [False, True])
 @pytest.mark.parametrize("case", CASES)
 def test_magnitudes(case, many, dk, dv):
@@ -144,20 +156,21 @@ def test_magnitudes_token_by_token(case):
     close(out, S, recurrence(*args))
 
 
+@pytest.mark.parametrize("dk", [64, 128])
 @pytest.mark.parametrize("many", [False, True])
-@pytest.mark.parametrize("what", ["g-nan", "g-inf", "beta-nan", "beta-inf", "q-nan", "overflow"])
+@pytest.mark.parametrize("what", ["g-nan", "g-inf", "beta-nan", "beta-inf", "q-nan", "k-nan", "k-inf", "v-nan", "v-inf", "overflow"])
 @pytest.mark.parametrize("at", [6, 40, 100])
-def test_not_finite_from_its_token_on(what, at, many):
-    """One head's decay, beta or query that is not finite, or products that overflow, leave its earlier tokens and the
-    other heads alone."""
+def test_not_finite_from_its_token_on(what, at, many, dk):
+    """One head's decay, beta, query, key or value that is not finite, or products that overflow, leave its earlier
+    tokens and the other heads alone."""
     T, H = 150, 4
-    q, k, v, g, beta, S0 = inputs(T, H, H, 64, 128, seed=7)
+    q, k, v, g, beta, S0 = inputs(T, H, H, dk, 128, seed=7)
     clean = recurrence(q, k, v, g, beta, S0)
     if what == "overflow":      # every step multiplies what the head holds along its key by -40
         k[at:at + 40, 1] = k[at, 1]
         beta[at:at + 40, 1] = 41
-    elif what == "q-nan":
-        q[at, 1, 3] = float("nan")
+    elif what[0] in "qkv":
+        {"q": q, "k": k, "v": v}[what[0]][at, 1, 3] = float(what.split("-")[1])
     else:
         (g if what[0] == "g" else beta)[at, 1] = float(what.split("-")[1])
     out, S = chunk(many, q, k, v, g, beta, S0)
@@ -167,6 +180,11 @@ def test_not_finite_from_its_token_on(what, at, many):
     if what == "q-nan":         # the state has no part in it
         assert out[at, 1].isnan().all()
         close(torch.where(out.isnan(), clean[0].to(out.dtype), out), S, clean)
+    elif what[0] == "v":        # nor have the other columns
+        keep = torch.ones(H, 128, dtype=torch.bool, device=DEV)
+        keep[1, 3] = False
+        assert not out[at:, 1, 3].isfinite().any() and not S[1, :, 3].isfinite().any()
+        close(torch.where(keep, out, clean[0].to(out.dtype)), torch.where(keep[:, None], S, clean[1].float()), clean)
     else:
         assert not out[-1, 1].isfinite().any() and not S[1].isfinite().all(0).any()
 

@@ -140,3 +140,35 @@ def test_walk_of_few_states(dv, dk):
     names, (out, S) = walks(lambda: deltanet.chunk_gated_delta_rule(*(t[None] for t in x), S0, cu))
     assert names <= {"walk_quad"}
     compare(list(range(H)), x, S0, cu.tolist(), out[0], S)
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_past_32_bits(many):
+    """Token rows 2^20 elements apart: the last ones lie past 2^31 elements."""
+    T, H, Hk, dk, dv, N = 2400, 4, 2, 128, 128, 32 if many else 1
+    x = inputs(T, H, Hk, dk, dv, seed=8)
+    S0 = torch.randn(N, H, dk, dv, device=DEV) * 0.05
+    cu = offsets([T // N] * N)
+    want, S_want = deltanet.chunk_gated_delta_rule(*(t[None] for t in x), S0, cu)
+    row = torch.empty(T, 2 ** 20, dtype=torch.bfloat16, device=DEV)
+    assert (T - 1) * 2 ** 20 > 2 ** 31
+    far, at = [], 0
+    for t in x[:3]:
+        far.append(row[:, at:at + t[0].numel()].view(t.shape))
+        far[-1].copy_(t)
+        at += t[0].numel()
+    names, (out, S) = walks(lambda: deltanet.chunk_gated_delta_rule(*(t[None] for t in far + x[3:]), S0, cu))
+    assert names <= {"walk_warp" if many else "walk_quad"} and torch.equal(out, want) and torch.equal(S, S_want)
+
+
+def test_states_past_32_bits():
+    H, dk, dv, N = 32, 128, 128, 2 ** 31 // (32 * 128 * 128) + 3
+    lens = [0] * (N - 2) + [70, 9]
+    cu = offsets(lens)
+    x = inputs(sum(lens), H, H, dk, dv, seed=9)
+    S = torch.zeros(N, H, dk, dv, device=DEV)
+    S[-2:] = torch.randn(2, H, dk, dv, device=DEV) * 0.05
+    first = S[-2:].clone()
+    out, got = deltanet.chunk_gated_delta_rule(*(t[None] for t in x), S, cu, S)
+    assert got is S and not S[:-2].any()
+    compare([0, 31], x, first, [0, 70, 79], out[0], S[-2:])
