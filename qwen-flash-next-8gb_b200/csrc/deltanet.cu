@@ -51,10 +51,10 @@ __global__ void __launch_bounds__(kDnSlices * kDnCols) deltanet_step_kernel(
   const int lane = threadIdx.x & 31;
   if (lane < R) asm volatile("prefetch.global.L2 [%0];" ::"l"(Sh + static_cast<int64_t>(sl * R + lane) * dv + (c - lane)));
   pdl_wait();
+  pdl_launch_dependents();
   float s[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) s[j] = Sh[static_cast<int64_t>(sl * R + j) * dv + c];
-  pdl_launch_dependents();
   for (int i = threadIdx.x; i < DK; i += blockDim.x) {
     qs[i] = bf16_bits_to_f32(q[static_cast<int64_t>(hk) * DK + i]);
     ks_[i] = bf16_bits_to_f32(k[static_cast<int64_t>(hk) * DK + i]);
