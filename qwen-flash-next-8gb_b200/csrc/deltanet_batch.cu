@@ -16,9 +16,9 @@
 // thread's rows, then two shuffles and four warps through shared memory in a
 // fixed order: results do not depend on the batch.
 //
-// Measured: 64 rows of 32 heads of 128 x 128 in 45 us, 6.0 TB/s; one row in 2.9 us
-// in a graph.  The states go past the caches (__ldcs, __stcs): 50 us with plain
-// loads and stores.
+// Measured: 64 rows of 32 heads of 128 x 128 in 45 to 47 us, 5.8 to 6.0 TB/s; one
+// row in 2.9 us in a graph.  The states go past the caches (__ldcs, __stcs): 50 us
+// with plain loads and stores where these take 45.
 #include "deltanet_batch.cuh"
 #include "deltanet_chunk.cuh"
 

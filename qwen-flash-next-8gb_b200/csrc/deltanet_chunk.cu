@@ -22,9 +22,9 @@
 // (Before, one power-of-two scale and two f16 terms served 16 columns and 64
 // tokens: values 2^-20 of the largest there lost their digits.)
 //
-// What bounds it: not the bytes (2048 tokens of 32 heads of 128 x 128 take 131 us,
-// their bytes 10.6) but the preparation's latency and instructions (44 us on its
-// own: 19,400 warp instructions a block, 47 % of the issue slots) and the walk's
+// What bounds it: not the bytes (2048 tokens of 32 heads of 128 x 128 take 137 us,
+// their bytes 10.6) but the preparation's latency and instructions (45 us on its
+// own: 17,000 warp instructions a block, 41 % of the issue slots) and the walk's
 // chain of chunks.  Chunks of 64 keep that chain short and T invertible in one block; token
 // by token the same call takes 3.6 ms.
 #include <atomic>
@@ -75,7 +75,7 @@ __device__ __forceinline__ float4 row_product(const float* row, const float* m, 
 
 // The inverse of I + A, A strictly lower triangular in t, in fp32: the four 16 x 16 blocks of the diagonal by
 // substitution, a column per lane, then T21 = -T22 (A21 T11) twice, for the two 32 x 32 halves and for the whole.
-// 4,400 of the block's 14,600 cycles where it has an SM to itself; two blocks of 32 and one merge take 7,200.
+// 4,400 cycles where the block has an SM to itself; two blocks of 32 and one merge take 7,200.
 template <int DK>
 __device__ __forceinline__ void invert(PrepSmem<DK>& sm) {
   const int tid = threadIdx.x;
@@ -396,9 +396,11 @@ cudaError_t launch(Kernel kernel, int64_t blocks, int threads, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Which walk: the quads' for few states, the warps' for many, whatever their lengths (which only the device knows).  Blocks come in rounds of one per SM, and a chunk of
-// a block takes, in 0.1 us (one head, from 2048 to 6144 tokens): 32 columns in the quads' walk 29 for dk = 128 and
-// 23 for dk = 64, 64 columns in the warps' 50 and 36, 128 columns 78 and 54.
+// Which walk: the quads' for few states, the warps' for many, whatever their lengths (which only the device knows).
+// Blocks come in rounds of one per SM, and a chunk of a block takes, in 0.1 us (one head, from 2048 to 6144 tokens):
+// 32 columns in the quads' walk 29 for dk = 128 and 23 for dk = 64, 64 columns in the warps' 50 and 36, 128 columns
+// 78 and 54.  Quads against warps, us: 32 / 64 / 128 states of 128 x 128 with 2048 tokens 137 / 210, 266 / 247,
+// 522 / 409; 160 with 1000 tokens 334 / 334-354; 512 of 64 x 32 with 1000 tokens 372 / 436.
 template <int DK>
 bool quad_walk(int64_t states, int dv, int sms) {
   auto rounds = [&](int cols) { return (states * ((dv + cols - 1) / cols) + sms - 1) / sms; };

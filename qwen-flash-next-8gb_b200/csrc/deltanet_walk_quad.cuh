@@ -6,8 +6,9 @@
 // behind them and copy the chunks to come.
 //
 // Bound by the chain of those exchanges: 2.9 us a chunk of dk = 128, 2.3 of dk = 64
-// (one head, slope from 2048 to 6144 tokens).  A warp per 16 columns (the walk for
-// many sequences) takes 5.0 and 3.6 there.
+// (one head, slope from 2048 to 6144 tokens), with the tensor pipe 51 % and the
+// issue slots 37 % busy.  A warp per 16 columns (the walk for many sequences) takes
+// 5.0 and 3.6 there.
 #pragma once
 
 #include "deltanet_chunk_parts.cuh"

@@ -3,8 +3,9 @@
 //
 // No exchange and no barrier in a chunk, so a chunk takes longer than in the quads'
 // walk but a block holds two to four times the columns.  Four prompts of 2048
-// tokens, 32 heads of 128 x 128: 412 us a call against 522 with the quads' walk;
-// one prompt: 210 against 137.
+// tokens, 32 heads of 128 x 128: 409 us a call against 522 with the quads' walk;
+// one prompt: 210 against 137.  Its 692 products a chunk and warp keep the tensor
+// pipe 60 % busy in blocks of 64 columns.
 #pragma once
 
 #include "deltanet_chunk_parts.cuh"
@@ -64,8 +65,8 @@ __global__ void __launch_bounds__(kWarpThreads, 1) dn_walk_warp_kernel(const DnR
   const bool ok = part.ok;
   const int n = static_cast<int>(max(last - first, static_cast<int64_t>(0)));
 
-  // Four warps have a scheduler each and walk a chunk of dk = 128 in 5.0 us, eight in 7.8.  Blocks have 128 columns, and every
-  // second block of 64 none, but for sequences that would take longer so than their share of all SMs' time, where
+  // Four warps have a scheduler each and walk a chunk of dk = 128 in 5.0 us, eight in 7.8.  Blocks have 128 columns, and
+  // every second block of 64 none, but for sequences that would take longer so than their share of all SMs' time, where
   // these are few enough for all their blocks of 64 columns to run at once.
   bool wide = true;
   if (plan.n_seqs <= kSorted && ok) {
