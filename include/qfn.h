@@ -258,7 +258,8 @@ int qfn_deltanet_step(const uint16_t* q, const uint16_t* k, const uint16_t* v, c
  *   out and touches no state.
  *   state_in, state_out: f32[n_slots][n_heads][dk][dv], 16-byte aligned, the
  *   same array or two that do not overlap; slots no row names are not written.
- *   out: bf16[rows][n_heads][dv], apart from both.  dk in {64, 128, 256}; dv % 32 == 0, dv <= 4096.
+ *   out: bf16[rows][n_heads][dv], apart from both.  dk in {64, 128, 256};
+ *   dv % 32 == 0, dv <= 4096.
  */
 int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* g,
                             const uint16_t* beta, const int64_t* strides, const int32_t* state_index,
@@ -276,18 +277,19 @@ int qfn_deltanet_step_batch(const uint16_t* q, const uint16_t* k, const uint16_t
  *   Bounds that do not rise: no row is written and every final state is NaN.
  *   state_in: f32[n_seqs][n_heads][dk][dv] or NULL (zeros); state_out: the
  *   same shape, state_in itself or an array that does not overlap it; both
- *   16-byte aligned; out 4-byte aligned and apart from both.  dk in {64, 128, 256}; dv % 32 == 0,
- *   dv <= 4096.  q, k and v are read in 16-byte pieces where their bases and
+ *   16-byte aligned; out 4-byte aligned and apart from both.  dk in {64, 128,
+ *   256}; dv % 32 == 0, dv <= 4096.  q, k and v are read in 16-byte pieces where their bases and
  *   strides allow it, else element by element.
  *   dk <= 128 and more than 10 to 24 tokens, by the sizes (of each sequence
  *   without cu_seqlens, in all with it, so that a ragged batch of many short
- *   sequences pays for a chunk of 64 tokens each) run 64 tokens at a time on the tensor cores (two launches for
- *   each segment of the workspace); others token by token.  Both hold S and
- *   every sum in fp32.  The chunks' products take bf16 terms of their operands,
+ *   sequences pays for a chunk of 64 tokens each) run 64 tokens at a time on
+ *   the tensor cores (two launches for each segment of the workspace); others
+ *   token by token.  Both hold S and every sum in fp32.  The chunks' products take bf16 terms of their operands,
  *   each with fp32's range: three (24 bits) of all that S is made of, two (16 bits)
  *   of what only reaches out.  g is the log of the decay, and -inf clears a
  *   finite state; where g rises, its sum stays below 88 within any 64 tokens.
- *   Rows of q and k have norms below 2^63.  Results do not depend on the other
+ *   Rows of q and k have norms below 2^63; where both are below 2^-50 their
+ *   products lose digits.  Results do not depend on the other
  *   sequences' contents; they differ in their last bits between calls of few and
  *   of many states, which run different kernels.
  *   workspace: device scratch of qfn_deltanet_chunk_workspace(...) bytes,

@@ -19,7 +19,8 @@ The states and every sum are fp32.  The prompts' chunks multiply on the tensor
 cores: what the state is made of is taken with fp32's 24 bits, what only reaches
 the bf16 outputs with 16 of them, each value with an exponent of its own.  -inf
 in g clears a finite state.  g is a decay, g <= 0; growth is taken too, as long as
-it stays below e^88 within 64 tokens.  q and k rows have norms below 2^63.
+it stays below e^88 within 64 tokens.  q and k rows have norms below 2^63; where
+both are below 2^-50 their products lose digits.
 
 All three are forward only; the batched two refuse a tensor that requires a
 gradient while gradients are recorded.
